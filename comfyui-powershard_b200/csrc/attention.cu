@@ -38,6 +38,17 @@
 // writes the second.  The exponentials use ex2.approx on the MUFU; measured on
 // B200, moving part of them to an FMA-pipe polynomial or fusing the row max
 // into the exponential pass made the softmax slower.
+//
+// Sparse form (kSparse): the keys of a CTA are the blocks that a list names for
+// its query block, so a key tile is one 128-row load or two 64-row loads from
+// anywhere in the sequence.  A query block is a multiple of 256 rows: both
+// query tiles of the CTA share the list, so each K/V tile is loaded once for
+// 256 queries, as in the dense form (a list for each 128 rows would double the
+// K/V loads: 64 KB per 128 x 128 tile pair is ~52 B/clk per SM, above the L2's
+// share).  The number of tiles is read from device memory and may be zero.
+// Rows past a sequence's key length are not used, whatever they hold: their
+// scores are masked, and as 0 * NaN is NaN in the PV product, V rows of a
+// partly used tile are overwritten with zeros in shared memory before it.
 #include "ptx.cuh"
 #include "ps_b200.h"
 #include "internal.h"
@@ -79,7 +90,8 @@ enum Bar : int {
   kBarPH = kBarP + 2,            // [2][kPParts-1] leading parts of P_t written
   kBarO = kBarPH + 2 * (kPParts - 1),  // O_0 and O_1 final
   kBarDrain = kBarO + 1,         // every UMMA of the issuer complete
-  kNumBars = kBarDrain + 1
+  kBarTail = kBarDrain + 1,      // sparse form: V rows of a partly used tile loaded
+  kNumBars = kBarTail + 1
 };
 constexpr int kSmemBytes = kSmemBarOff + 256 + 1024;  // barriers + TMEM slot + 1 KiB align slack
 static_assert(kNumBars * 8 + 8 <= 256, "barrier block overflow");
@@ -157,6 +169,53 @@ __device__ __forceinline__ void q_tile(const AttnArgs& a, int t, bool& prefix, i
   }
 }
 
+// Key tiles of one block list.  A block is cut into pieces of `piece` rows and
+// a 128-row tile holds 128 / piece consecutive pieces of the list.
+struct BlockList {
+  const int* list;
+  int count;   // entries in use
+  int len_k;   // key rows in use
+  int ppb;     // pieces of one block
+
+  BlockList() = default;
+  __device__ __forceinline__ BlockList(const AttnArgs& a, int batch, int head, int pair) {
+    const int qrows = a.q_len ? min(max(a.q_len[batch], 0), a.seg_rows_q) : a.seg_rows_q;
+    len_k = a.k_len ? min(max(a.k_len[batch], 0), a.seg_rows_k) : a.seg_rows_k;
+    const int64_t at = (static_cast<int64_t>(batch) * a.grid_heads + head) * a.list_rows + pair / a.pairs_per_list;
+    list = a.blocks + at * a.list_len;
+    count = a.counts ? min(max(a.counts[at], 0), a.list_len) : a.list_len;
+    if (pair * 2 * kBlockM >= qrows || len_k == 0) count = 0;
+    ppb = a.key_block / a.piece;
+  }
+  __device__ __forceinline__ int tiles(const AttnArgs& a) const {
+    return static_cast<int>((static_cast<int64_t>(count) * a.key_block + kBlockN - 1) / kBlockN);
+  }
+  // First row of piece p of key tile t, and in `valid` its rows in use.  A
+  // piece without any starts behind the tensor: its load fills with zeros.
+  __device__ __forceinline__ int row(const AttnArgs& a, int t, int p, int& valid) const {
+    const int g = t * (kBlockN / a.piece) + p;
+    const int e = g / ppb;
+    valid = 0;
+    if (e >= count) return a.seg_rows_k;
+    const int blk = list[e];
+    if (blk < 0 || blk >= a.key_blocks) return a.seg_rows_k;
+    const int64_t r = static_cast<int64_t>(blk) * a.key_block + (g - e * ppb) * a.piece;
+    if (r >= len_k) return a.seg_rows_k;
+    valid = min(a.piece, len_k - static_cast<int>(r));
+    return static_cast<int>(r);
+  }
+  // Rows in use of the tile's lower and upper 64.
+  __device__ __forceinline__ void halves(const AttnArgs& a, int t, int& lo, int& hi) const {
+    row(a, t, 0, lo);
+    if (a.piece == kBlockN) {
+      hi = max(lo - 64, 0);
+      lo = min(lo, 64);
+    } else {
+      row(a, t, 1, hi);
+    }
+  }
+};
+
 // Bounded wait whose outcome is uniform across the warp (a lane that timed
 // out drags the whole warp out, so .sync.aligned tcgen05 ops stay converged).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
@@ -177,6 +236,93 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, int* s
   }
 }
 
+// Producer of the sparse form, one warp: the dense producer's stage protocol
+// (see there) with each tile gathered from its pieces.  The rows of a tile are
+// looked up before the wait for its stage, off the critical path.
+__device__ __forceinline__ void sparse_producer(const AttnArgs& args, const BlockList& blocks, const CUtensorMap& tm_q,
+                                                const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* sQ,
+                                                uint8_t* sK, uint8_t* sV, uint64_t* bars, int tq0, int head,
+                                                int kv_head, int batch, int k_begin, int T, int lane,
+                                                volatile int* abort_flag) {
+  int* status = args.status;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  const int pieces = kBlockN / args.piece;
+  const int piece_bytes = args.piece * 128;  // of one 64-column half
+  if (lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+    const int tq1 = min(tq0 + 1, args.num_q_tiles - 1);  // no second tile: tile 0 again, never stored
+    mbar_arrive_expect_tx(bar(kBarQ), 2 * kTileBytes);
+    for (int c = 0; c < 2; ++c) {
+      tma_load_5d(smem_u32(sQ + c * kHalfTile), &tm_q, bar(kBarQ), c * 64, head, tq0 * kBlockM, 0, batch);
+      tma_load_5d(smem_u32(sQ + kTileBytes + c * kHalfTile), &tm_q, bar(kBarQ), c * 64, head, tq1 * kBlockM, 0, batch);
+    }
+  }
+  auto load = [&](uint8_t* stage, const CUtensorMap* map, int b, const int (&row)[2]) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bar(b), kTileBytes);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (p < pieces)
+          for (int c = 0; c < 2; ++c)
+            tma_load_5d(smem_u32(stage + c * kHalfTile + p * piece_bytes), map, bar(b), c * 64, kv_head, row[p], 0,
+                        batch);
+    }
+  };
+  int issued = 0;
+  uint32_t tail_phase = 0;
+  bool ok = true;
+  for (int i = 0; i < T; ++i) {
+    const int st = i % kKStages;
+    int row[2] = {0, 0}, valid[2] = {0, 0};
+    bool tail = false;  // rows of the tensor that are not in use reach the tile
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      if (p < pieces) row[p] = blocks.row(args, k_begin + i, p, valid[p]);
+      tail |= valid[p] > 0 && valid[p] < args.piece && blocks.len_k < args.seg_rows_k;
+    }
+    if (i >= kKStages) ok = warp_wait(bar(kBarFree + (i & 1)), ((i - 2) >> 1) & 1u, abort_flag, status, kErrEmpty);
+    if (!ok) break;
+    load(sK + st * kTileBytes, &tm_k, kBarKFull + st, row);
+    issued = 2 * i + 1;
+    if (i >= kVStages)
+      ok = warp_wait(bar(kBarFree + ((i - 1) & 1)), ((i - 1) >> 1) & 1u, abort_flag, status, kErrEmpty);
+    if (!ok) break;
+    if (!tail) {
+      load(sV + st * kTileBytes, &tm_v, kBarVFull + st, row);
+    } else {
+      uint8_t* stage = sV + st * kTileBytes;
+      load(stage, &tm_v, kBarTail, row);
+      drain_wait(bar(kBarTail), tail_phase, status);
+      tail_phase ^= 1u;
+      __syncwarp();
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        if (valid[p] == 0) continue;  // no such piece, or filled with zeros by its load
+        const int n = (args.piece - valid[p]) * 8;  // 16-byte chunks of one half
+        for (int c = 0; c < 2; ++c) {
+          uint4* dst = reinterpret_cast<uint4*>(stage + c * kHalfTile + p * piece_bytes + valid[p] * 128);
+          for (int u = lane; u < n; u += 32) dst[u] = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBarVFull + st));
+    }
+    issued = 2 * i + 2;
+  }
+  // Every copy issued must land before the CTA may exit.
+  drain_wait(bar(kBarQ), 0, status);
+  const int kv_issued = (issued + 1) / 2;
+  for (int i = max(0, kv_issued - kKStages); i < kv_issued; ++i) {
+    const int st = i % kKStages;
+    const uint32_t ph = (i / kKStages) & 1u;
+    drain_wait(bar(kBarKFull + st), ph, status);
+    if (2 * i + 2 <= issued) drain_wait(bar(kBarVFull + st), ph, status);
+  }
+}
+
 template <bool kFp16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return kFp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
@@ -194,7 +340,7 @@ __device__ __forceinline__ float row_max128(const float (&s)[128]) {
   return fmaxf(fmax3(mx0, mx1, mx2), mx3);
 }
 
-template <bool kFp16>
+template <bool kFp16, bool kSparse>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_qp,
@@ -226,8 +372,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kv_head = head / args.group;
   const int tq0 = pair * 2;
   const int tq1 = tq0 + 1;
-  const int k_begin = part * args.num_kv_tiles / nparts;
-  const int T = (part + 1) * args.num_kv_tiles / nparts - k_begin;
+  [[maybe_unused]] BlockList blocks;
+  if constexpr (kSparse) blocks = BlockList(args, batch, head, pair);
+  const int tiles = kSparse ? blocks.tiles(args) : args.num_kv_tiles;
+  const int k_begin = part * tiles / nparts;
+  const int T = (part + 1) * tiles / nparts - k_begin;
   int* status = args.status;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
@@ -244,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(bar(kBarO), 1);
     mbar_init(bar(kBarDrain), 1);
+    if constexpr (kSparse) mbar_init(bar(kBarTail), 1);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -255,7 +405,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 8) {
+  if (kSparse && T == 0) {
+    // No key: nothing to load or multiply, the epilogue writes zeros.
+  } else if (kSparse && warp == 8) {
+    sparse_producer(args, blocks, tm_q, tm_k, tm_v, sQ, sK, sV, bars, tq0, head, kv_head, batch, k_begin, T, lane,
+                    abort_flag);
+  } else if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
@@ -392,7 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(bar(kBarDrain));
       drain_wait(bar(kBarDrain), 0, status);
     }
-  } else if (warp < 8) {
+  }
+  if (warp < 8) {
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;
     const int quarter = warp & 3;
@@ -404,11 +560,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     KeyCursor cur;
-    cur.skip(args, k_begin);
+    if constexpr (!kSparse) cur.skip(args, k_begin);
+    [[maybe_unused]] uint32_t whole = 0;  // sparse: which of the next 32 key tiles are in use throughout
     for (int i = 0; i < T; ++i) {
-      bool pre_unused;
-      int seg_unused, row_unused, valid;
-      cur.next(args, pre_unused, seg_unused, row_unused, valid);
+      int valid = kBlockN;
+      [[maybe_unused]] bool part_used = false;
+      if constexpr (kSparse) {
+        if ((i & 31) == 0) {
+          int lo = 64, hi = 64;
+          if (i + lane < T) blocks.halves(args, k_begin + i + lane, lo, hi);
+          whole = __ballot_sync(0xffffffffu, lo + hi == kBlockN);
+        }
+        part_used = !((whole >> (i & 31)) & 1u);
+      } else {
+        bool pre_unused;
+        int seg_unused, row_unused;
+        cur.next(args, pre_unused, seg_unused, row_unused, valid);
+      }
       ok = warp_wait(bar(kBarS + t), i & 1u, abort_flag, status, kErrS);
       if (!ok) break;
       if (t == 1 && threadIdx.x == 128) mbar_arrive(bar(kBarFree + (i & 1)));
@@ -422,6 +590,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       float s[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) s[j] = __uint_as_float(sr[j]);
+      if constexpr (kSparse) {
+        if (part_used) {
+          int lo, hi;
+          blocks.halves(args, k_begin + i, lo, hi);
+#pragma unroll
+          for (int j = 0; j < 128; ++j)
+            if ((j < 64 ? j : j - 64) >= (j < 64 ? lo : hi)) s[j] = -INFINITY;
+        }
+      }
       const bool masked = valid < kBlockN;
       if (masked) {
 #pragma unroll
@@ -434,7 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // grew by > 8), then the exponentials.
       const float m_tile = row_max128(s) * scale_log2;
       if (i == 0) {
-        m = m_tile;
+        // A listed tile without a key in use leaves every score at -inf: a
+        // finite maximum makes its exponentials 0 instead of NaN.
+        m = kSparse ? fmaxf(m_tile, -1e30f) : m_tile;
       } else if (__any_sync(0xffffffffu, m_tile - m > 8.f)) {
         const float m_new = fmaxf(m, m_tile);
         alpha = ex2_approx(m - m_new);
@@ -484,13 +663,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(bar(kBarP + t));
     }
-    if (ok) ok = warp_wait(bar(kBarO), 0, abort_flag, status, kErrO);
+    if (ok && (!kSparse || T > 0)) ok = warp_wait(bar(kBarO), 0, abort_flag, status, kErrO);
     tc_fence_after();
     const int tq = t ? tq1 : tq0;
     bool pre = false;
     int seg = 0, row0 = 0, valid = 0;
     if (tq < args.num_q_tiles) q_tile(args, tq, pre, seg, row0, valid);
     const float inv_l = l > 0.f ? 1.f / l : 0.f;
+    // Sparse: rows behind the sequence's queries and rows that saw no key are
+    // zeros (the accumulator of a CTA without tiles was never written).
+    bool live = true;
+    if constexpr (kSparse) {
+      const int qrows = args.q_len ? args.q_len[batch] : args.seg_rows_q;
+      live = T > 0 && row0 + row < qrows;
+    }
     void* const obase = pre ? args.pre_out : args.seg_out[seg];
     const int64_t* ost = pre ? args.pre_o_stride : args.o_stride;
     const int64_t otile = batch * ost[0] + static_cast<int64_t>(row0) * ost[2] + head * ost[3];
@@ -504,13 +690,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
-          float4* dst = reinterpret_cast<float4*>(wrow + 32 * c);
+          if constexpr (kSparse) {
+            if (!live)
 #pragma unroll
-          for (int u = 0; u < 8; ++u)
-            dst[u] = make_float4(__uint_as_float(o[4 * u + 0]) * inv_l, __uint_as_float(o[4 * u + 1]) * inv_l,
-                                 __uint_as_float(o[4 * u + 2]) * inv_l, __uint_as_float(o[4 * u + 3]) * inv_l);
+              for (int j = 0; j < 32; ++j) o[j] = 0;
+          }
+          float4* dst = reinterpret_cast<float4*>(wrow + 32 * c);
+          if (!kSparse || row < valid) {  // the merge reads the rows of the tensor only
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+              dst[u] = make_float4(__uint_as_float(o[4 * u + 0]) * inv_l, __uint_as_float(o[4 * u + 1]) * inv_l,
+                                   __uint_as_float(o[4 * u + 2]) * inv_l, __uint_as_float(o[4 * u + 3]) * inv_l);
+          }
         }
-        args.ws_lse[(slot * 2 + t) * kBlockM + row] = l > 0.f ? m + __log2f(l) : -INFINITY;
+        args.ws_lse[(slot * 2 + t) * kBlockM + row] = live && l > 0.f ? m + __log2f(l) : -INFINITY;
       }
     } else if (args.out_fp32) {
       // tcgen05.ld is warp-collective: every lane loads, only valid rows store.
@@ -521,6 +714,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
+          if constexpr (kSparse) {
+            if (!live)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = 0;
+          }
           if (row < valid) {
             float4* dst = reinterpret_cast<float4*>(orow + 32 * c);
 #pragma unroll
@@ -544,6 +742,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
+          if constexpr (kSparse) {
+            if (!live)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = 0;
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint4 v;
@@ -648,16 +851,40 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnArgs args) 
 namespace {
 // Raises the kernel's dynamic shared memory limit once per device (outside
 // any stream capture that may follow: the first launch on a device does it).
-template <bool kFp16>
+template <bool kFp16, bool kSparse>
 int prepare_kernel() {
   static bool done[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (done[dev]) return 0;
-  const cudaError_t err = cudaFuncSetAttribute(attn::attn_fwd_kernel<kFp16>,
+  const cudaError_t err = cudaFuncSetAttribute(attn::attn_fwd_kernel<kFp16, kSparse>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, attn::kSmemBytes);
   if (err != cudaSuccess) return set_cuda_error("attention: cudaFuncSetAttribute", err);
   done[dev] = true;
+  return 0;
+}
+
+template <bool kFp16, bool kSparse>
+int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tqp,
+           const CUtensorMap& tkp, const CUtensorMap& tvp, const AttnArgs& args, int64_t total_units,
+           cudaStream_t stream) {
+  using namespace attn;
+  const int64_t split_units = args.split > 1 ? total_units - args.full_units : 0;
+  const int64_t ctas = split_units > 0 ? args.full_units + split_units * args.split : total_units;
+  if (ctas <= 0) return 0;
+  if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "attention grid above 2^31 CTAs");
+  if (int rc = prepare_kernel<kFp16, kSparse>()) return rc;
+  attn_fwd_kernel<kFp16, kSparse>
+      <<<static_cast<unsigned>(ctas), kThreads, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_cuda_error("attention launch", err);
+  count_launch();
+  if (split_units > 0) {
+    attn_combine_kernel<kFp16><<<static_cast<unsigned>(split_units * 2), 256, 0, stream>>>(args);
+    err = cudaGetLastError();
+    if (err != cudaSuccess) return set_cuda_error("attention combine launch", err);
+    count_launch();
+  }
   return 0;
 }
 }  // namespace
@@ -665,34 +892,14 @@ int prepare_kernel() {
 int launch_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                      const CUtensorMap& tqp, const CUtensorMap& tkp, const CUtensorMap& tvp,
                      const AttnArgs& args, int64_t total_units, bool fp16, cudaStream_t stream) {
-  using namespace attn;
-  const int64_t split_units = args.split > 1 ? total_units - args.full_units : 0;
-  const int64_t ctas = split_units > 0 ? args.full_units + split_units * args.split : total_units;
-  if (ctas <= 0) return 0;
-  if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "attention grid above 2^31 CTAs");
-  const dim3 grid(static_cast<unsigned>(ctas));
-  const dim3 block(kThreads);
-  if (fp16) {
-    if (int rc = prepare_kernel<true>()) return rc;
-    attn_fwd_kernel<true><<<grid, block, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
-  } else {
-    if (int rc = prepare_kernel<false>()) return rc;
-    attn_fwd_kernel<false><<<grid, block, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
-  }
-  cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_cuda_error("attention launch", err);
-  count_launch();
-  if (split_units > 0) {
-    const dim3 cgrid(static_cast<unsigned>(split_units * 2));
-    if (fp16)
-      attn_combine_kernel<true><<<cgrid, 256, 0, stream>>>(args);
-    else
-      attn_combine_kernel<false><<<cgrid, 256, 0, stream>>>(args);
-    err = cudaGetLastError();
-    if (err != cudaSuccess) return set_cuda_error("attention combine launch", err);
-    count_launch();
-  }
-  return 0;
+  return fp16 ? launch<true, false>(tq, tk, tv, tqp, tkp, tvp, args, total_units, stream)
+              : launch<false, false>(tq, tk, tv, tqp, tkp, tvp, args, total_units, stream);
+}
+
+int launch_sparse_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args,
+                            int64_t total_units, bool fp16, cudaStream_t stream) {
+  return fp16 ? launch<true, true>(tq, tk, tv, tq, tk, tv, args, total_units, stream)
+              : launch<false, true>(tq, tk, tv, tq, tk, tv, args, total_units, stream);
 }
 
 }  // namespace psb

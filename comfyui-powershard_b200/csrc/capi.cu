@@ -67,9 +67,9 @@ std::atomic<unsigned long long> g_launches{0};
 bool is16bit(int dtype) { return dtype == PS_B200_BF16 || dtype == PS_B200_FP16; }
 
 // 5-D map over [batch][seg][row][head][d] with a (64 x 1 x 128 x 1 x 1) box:
-// one 64-column, 128-row half tile with 128-byte swizzle.
+// one 64-column, 128-row half tile with 128-byte swizzle (64 rows: a piece of one).
 int make_map(CUtensorMap* m, const void* base, bool fp16, int head_dim, int heads, int seg_rows, int segs,
-             int batch, const int64_t st[4]) {
+             int batch, const int64_t st[4], int box_rows = 128) {
   auto fn = encode_fn();
   if (!fn) return set_error(PS_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   // Byte strides of the head, row, segment and batch axes.  Axes of extent 1
@@ -87,7 +87,7 @@ int make_map(CUtensorMap* m, const void* base, bool fp16, int head_dim, int head
   cuuint64_t dims[5] = {cuuint64_t(head_dim), cuuint64_t(heads), cuuint64_t(seg_rows), cuuint64_t(segs),
                         cuuint64_t(batch)};
   cuuint64_t strides[4] = {cuuint64_t(sh), cuuint64_t(sr), cuuint64_t(ss), cuuint64_t(sb)};
-  cuuint32_t box[5] = {64, 1, 128, 1, 1};
+  cuuint32_t box[5] = {64, 1, cuuint32_t(box_rows), 1, 1};
   cuuint32_t es[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(m, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                   const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -254,6 +254,46 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
   }
   return launch_attention(tq, tk, tv, tqp, tkp, tvp, a, units, fp16, static_cast<cudaStream_t>(stream));
 }
+
+// How block-sparse attention is cut into CTAs: the last, partial wave's units
+// (query tile pair, head, batch) run as `split` CTAs each over parts of their
+// lists, at least two key tiles a part by the lists' full length.
+struct SparsePlan {
+  int64_t units, rem;
+  int split;
+  size_t workspace_bytes() const { return split > 1 ? size_t(rem) * split * 2 * 128 * (128 + 1) * 4 : 0; }
+};
+
+SparsePlan sparse_plan(int64_t batch, int64_t heads, int64_t len_q, int64_t list_len, int64_t key_block, int sms) {
+  SparsePlan p{};
+  p.units = (len_q + 255) / 256 * heads * batch;
+  p.rem = p.units % sms;
+  p.split = 1;
+  if (p.rem > 0) {
+    const int64_t tiles = (list_len * key_block + 127) / 128;
+    int64_t split = sms / p.rem;
+    split = split < tiles / 2 ? split : tiles / 2;
+    split = split < kMaxSparseSplit ? split : kMaxSparseSplit;
+    if (split >= 2) p.split = static_cast<int>(split);
+  }
+  return p;
+}
+
+// Sizes that every entry on block lists checks.
+int check_blocks(int batch, int heads_q, int heads_kv, int head_dim, int query_block, int key_block) {
+  if (batch < 0 || batch > 65535) return set_error(PS_B200_ERR_INVALID, "batch must be in [0, 65535]");
+  if (heads_kv <= 0 || heads_q < 0 || heads_q % heads_kv != 0 || heads_q > 65535)
+    return set_error(PS_B200_ERR_INVALID, "heads_q must be a multiple of heads_kv and at most 65535");
+  if (head_dim != 128)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports head_dim 128 only (got %d)", head_dim);
+  if (query_block <= 0 || query_block % 256 != 0 || query_block > (1 << 20))
+    return set_error(PS_B200_ERR_UNSUPPORTED, "query blocks are multiples of 256 rows up to 2^20 (got %d)", query_block);
+  if (key_block <= 0 || key_block % 64 != 0 || key_block > (1 << 20))
+    return set_error(PS_B200_ERR_UNSUPPORTED, "key blocks are multiples of 64 rows up to 2^20 (got %d)", key_block);
+  return PS_B200_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 }  // namespace
 
@@ -924,6 +964,224 @@ int ps_b200_out_proj(const void* src, int64_t src_row_stride, int64_t src_block_
   }
   if (int rc = make_map_2d(&tw, w_o, fp16, in_features, out_features, in_features, 128)) return rc;
   return launch_proj(ta, tw, tw, tw, a, fp16, C, static_cast<cudaStream_t>(stream));
+}
+
+int ps_b200_block_means(int tensors, const void* const* x, const int64_t* strides, int dtype, int batch, const int* len,
+                        const int* heads, int head_dim, const int* block, const int* const* lens, float* const* out,
+                        void* stream) {
+  if (tensors < 1 || tensors > 2) return set_error(PS_B200_ERR_INVALID, "block_means takes one or two tensors");
+  if (!x || !strides || !len || !heads || !block || !out) return set_error(PS_B200_ERR_INVALID, "null table");
+  if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block_means supports bf16 and fp16 only");
+  if (head_dim != 128) return set_error(PS_B200_ERR_UNSUPPORTED, "block_means supports head_dim 128 only (got %d)", head_dim);
+  if (batch < 0 || batch > 65535) return set_error(PS_B200_ERR_INVALID, "batch must be in [0, 65535]");
+  MeansArgs a{};
+  for (int t = 0; t < tensors; ++t) {
+    MeansTensor& m = a.t[t];
+    if (len[t] < 0 || heads[t] < 0 || block[t] < 1) return set_error(PS_B200_ERR_INVALID, "negative size or empty block");
+    m.len = len[t];
+    m.heads = heads[t];
+    m.block = block[t];
+    m.blocks = static_cast<int>((int64_t(len[t]) + block[t] - 1) / block[t]);
+    m.head_pairs = (heads[t] + 1) / 2;
+    m.ctas = int64_t(batch) * m.blocks * m.head_pairs;
+    if (m.ctas == 0) continue;
+    if (!x[t] || !aligned16(x[t])) return set_error(PS_B200_ERR_INVALID, "tensor %d null or not 16-byte aligned", t);
+    if (!out[t] || !aligned4(out[t])) return set_error(PS_B200_ERR_INVALID, "means %d null or not 4-byte aligned", t);
+    for (int i = 0; i < 3; ++i) {
+      m.st[i] = strides[3 * t + i];
+      if (m.st[i] < 0 || m.st[i] % 8 != 0)
+        return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
+    }
+    m.x = x[t];
+    m.lens = lens ? lens[t] : nullptr;
+    if (!aligned4(m.lens)) return set_error(PS_B200_ERR_INVALID, "lengths must be 4-byte aligned");
+    m.out = out[t];
+  }
+  if (a.t[0].ctas + a.t[1].ctas == 0) return PS_B200_OK;
+  if (int rc = check_device()) return rc;
+  return launch_block_means(a, dtype == PS_B200_FP16, static_cast<cudaStream_t>(stream));
+}
+
+int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
+                         int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
+                         const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
+                         int key_block, int* blocks, int* counts, void* stream) {
+  if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
+  if (q_blocks < 0 || k_blocks < 0 || keep < 1) return set_error(PS_B200_ERR_INVALID, "keep must be positive, block counts not negative");
+  if (keep > k_blocks && k_blocks > 0) return set_error(PS_B200_ERR_INVALID, "keep %d above the %d key blocks", keep, k_blocks);
+  if (batch == 0 || heads_q == 0 || q_blocks == 0) return PS_B200_OK;
+  if (k_blocks == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
+  if (size_t(k_blocks) > kSelectSmemLimit / 8 - 128)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "%d key blocks: at most %d, take larger blocks", k_blocks,
+                     int(kSelectSmemLimit / 8 - 128));
+  if (!q_means || !k_means || !aligned16(q_means) || !aligned16(k_means))
+    return set_error(PS_B200_ERR_INVALID, "means null or not 16-byte aligned");
+  if (!blocks || !counts || !aligned4(blocks) || !aligned4(counts) || !aligned4(q_len) || !aligned4(k_len))
+    return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
+  if (allowed && !allowed_strides) return set_error(PS_B200_ERR_INVALID, "allowed needs strides");
+  if (int rc = check_device()) return rc;
+  SelectArgs a{};
+  a.q_means = q_means;
+  a.k_means = k_means;
+  a.batch = batch;
+  a.kv_heads = heads_kv;
+  a.group = heads_q / heads_kv;
+  a.q_blocks = q_blocks;
+  a.k_blocks = k_blocks;
+  a.keep = keep;
+  a.query_block = query_block;
+  a.key_block = key_block;
+  a.q_len = q_len;
+  a.k_len = k_len;
+  a.allowed = allowed;
+  for (int i = 0; i < 4; ++i) a.allowed_st[i] = allowed ? allowed_strides[i] : 0;
+  a.blocks = blocks;
+  a.counts = counts;
+  return launch_block_select(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block) {
+  if (batch <= 0 || heads_q <= 0 || len_q <= 0 || list_len <= 0 || key_block <= 0) return 0;
+  return sparse_plan(batch, heads_q, len_q, list_len, key_block, sm_count()).workspace_bytes();
+}
+
+int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                            const void* v, const int64_t v_strides[3], void* out, const int64_t out_strides[3],
+                            int dtype, int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k,
+                            const int* blocks, const int* counts, int list_len, int query_block, int key_block,
+                            const int* q_len, const int* k_len, float softmax_scale, void* workspace,
+                            size_t workspace_bytes, int* status, void* stream) {
+  if (!q_strides || !k_strides || !v_strides || !out_strides) return set_error(PS_B200_ERR_INVALID, "null strides");
+  if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
+  if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
+  if (len_q < 0 || len_k < 0 || len_q > (1 << 30) || len_k > (1 << 30))
+    return set_error(PS_B200_ERR_INVALID, "lengths must be in [0, 2^30]");
+  if (list_len < 1 || int64_t(list_len) * key_block > (1 << 30))
+    return set_error(PS_B200_ERR_INVALID, "lists must name between one block and 2^30 rows");
+  if (batch == 0 || heads_q == 0 || len_q == 0) return PS_B200_OK;
+  if (len_k == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
+  if (!std::isfinite(softmax_scale) || softmax_scale <= 0.f)
+    return set_error(PS_B200_ERR_INVALID, "softmax_scale must be positive and finite");
+  if (!q || !k || !v || !out) return set_error(PS_B200_ERR_INVALID, "null tensor pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return set_error(PS_B200_ERR_INVALID, "tensor pointers must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if (out_strides[i] < 0 || out_strides[i] % 8 != 0)
+      return set_error(PS_B200_ERR_INVALID, "output strides must be non-negative multiples of 8 elements");
+  if (!blocks || !aligned4(blocks) || !aligned4(counts) || !aligned4(q_len) || !aligned4(k_len))
+    return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
+  if (!aligned4(status)) return set_error(PS_B200_ERR_INVALID, "status word must be 4-byte aligned");
+  if (int rc = check_device()) return rc;
+  const bool fp16 = dtype == PS_B200_FP16;
+  AttnArgs a{};
+  a.piece = key_block % 128 == 0 ? 128 : 64;
+  CUtensorMap tq, tk, tv;
+  const int64_t qs[4] = {q_strides[0], 0, q_strides[1], q_strides[2]};
+  const int64_t ks[4] = {k_strides[0], 0, k_strides[1], k_strides[2]};
+  const int64_t vs[4] = {v_strides[0], 0, v_strides[1], v_strides[2]};
+  if (int rc = make_map(&tq, q, fp16, head_dim, heads_q, len_q, 1, batch, qs)) return rc;
+  if (int rc = make_map(&tk, k, fp16, head_dim, heads_kv, len_k, 1, batch, ks, a.piece)) return rc;
+  if (int rc = make_map(&tv, v, fp16, head_dim, heads_kv, len_k, 1, batch, vs, a.piece)) return rc;
+  a.seg_out[0] = a.pre_out = out;
+  a.o_stride[0] = out_strides[0];
+  a.o_stride[2] = out_strides[1];
+  a.o_stride[3] = out_strides[2];
+  a.seg_rows_q = a.valid_q[0] = len_q;
+  a.seg_rows_k = a.valid_k[0] = len_k;
+  a.nsegs_q = a.nsegs_k = 1;
+  a.q_tiles_per_seg = a.num_q_tiles = (len_q + 127) / 128;
+  a.group = heads_q / heads_kv;
+  a.scale_log2 = static_cast<float>(double(softmax_scale) * 1.4426950408889634);
+  a.status = status;
+  a.npairs = (a.num_q_tiles + 1) / 2;
+  a.grid_heads = heads_q;
+  a.blocks = blocks;
+  a.counts = counts;
+  a.pairs_per_list = query_block / 256;
+  a.list_rows = (a.npairs + a.pairs_per_list - 1) / a.pairs_per_list;
+  a.list_len = list_len;
+  a.key_block = key_block;
+  a.key_blocks = (len_k + key_block - 1) / key_block;
+  a.q_len = q_len;
+  a.k_len = k_len;
+  const SparsePlan plan = sparse_plan(batch, heads_q, len_q, list_len, key_block, sm_count());
+  if (plan.units > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "attention grid above 2^31 CTAs");
+  a.split = 1;
+  a.full_units = static_cast<int>(plan.units);
+  if (plan.split > 1) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < plan.workspace_bytes())
+      return set_error(PS_B200_ERR_INVALID, "this call needs a 16-byte aligned workspace of %zu bytes (got %zu)",
+                       plan.workspace_bytes(), workspace ? workspace_bytes : size_t(0));
+    a.split = plan.split;
+    a.full_units = static_cast<int>(plan.units - plan.rem);
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_lse = a.ws_o + plan.rem * plan.split * 2 * 128 * 128;
+  }
+  return launch_sparse_attention(tq, tk, tv, a, plan.units, fp16, static_cast<cudaStream_t>(stream));
+}
+
+static int cache_common(bool write, void* const pages[2], float* const scales[2], void* const rows[2],
+                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
+                        int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
+                        int table_len, const int* first, const int* count, void* stream) {
+  if (!pages || !scales || !rows || !strides) return set_error(PS_B200_ERR_INVALID, "null tensor table");
+  if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "the cache takes and gives bf16 and fp16 rows only");
+  if (cache_dtype != PS_B200_E4M3 && cache_dtype != PS_B200_INT8)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds e4m3 or int8 codes only");
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds heads of 64, 128 or 256 (got %d)", head_dim);
+  if (batch < 0 || batch > 65535 || heads < 0 || heads > 4096 || n < 0 || num_pages < 0 || page_rows < 1 ||
+      table_len < 0 || table_stride < 0)
+    return set_error(PS_B200_ERR_INVALID, "size out of range (batch <= 65535, heads <= 4096)");
+  if (batch == 0 || n == 0 || heads == 0) return PS_B200_OK;
+  if (!table || !aligned4(table) || !aligned4(first) || !aligned4(count))
+    return set_error(PS_B200_ERR_INVALID, "page table null or a table not 4-byte aligned");
+  if (!write && !count) return set_error(PS_B200_ERR_INVALID, "a read needs the lengths");
+  CacheArgs a{};
+  for (int t = 0; t < 2; ++t) {
+    if (!pages[t] || !scales[t] || !rows[t] || !aligned16(pages[t]) || !aligned4(scales[t]) || !aligned16(rows[t]))
+      return set_error(PS_B200_ERR_INVALID, "pages, scales or rows null or not aligned (16, 4 and 16 bytes)");
+    a.pages[t] = pages[t];
+    a.scales[t] = scales[t];
+    a.rows[t] = rows[t];
+    for (int i = 0; i < 3; ++i) {
+      a.st[t][i] = strides[3 * t + i];
+      if (a.st[t][i] < 0 || a.st[t][i] % 8 != 0)
+        return set_error(PS_B200_ERR_INVALID, "row strides must be non-negative multiples of 8 elements");
+    }
+  }
+  if (int rc = check_device()) return rc;
+  a.batch = batch;
+  a.n = n;
+  a.heads = heads;
+  a.head_dim = head_dim;
+  a.num_pages = num_pages;
+  a.page_rows = page_rows;
+  a.table = table;
+  a.table_st = table_stride;
+  a.table_len = table_len;
+  a.first = first;
+  a.count = count;
+  const bool fp16 = dtype == PS_B200_FP16, int8 = cache_dtype == PS_B200_INT8;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return write ? launch_cache_write(a, fp16, int8, s) : launch_cache_read(a, fp16, int8, s);
+}
+
+int ps_b200_cache_write(void* const pages[2], float* const scales[2], const void* const rows[2],
+                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads, int head_dim,
+                        int num_pages, int page_rows, const int* table, int64_t table_stride, int table_len,
+                        const int* first, const int* count, void* stream) {
+  return cache_common(true, pages, scales, const_cast<void* const*>(rows), strides, dtype, cache_dtype, batch, n, heads,
+                      head_dim, num_pages, page_rows, table, table_stride, table_len, first, count, stream);
+}
+
+int ps_b200_cache_read(const void* const pages[2], const float* const scales[2], void* const rows[2],
+                       const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads, int head_dim,
+                       int num_pages, int page_rows, const int* table, int64_t table_stride, int table_len,
+                       const int* first, const int* count, void* stream) {
+  return cache_common(false, const_cast<void* const*>(pages), const_cast<float* const*>(scales), rows, strides, dtype,
+                      cache_dtype, batch, n, heads, head_dim, num_pages, page_rows, table, table_stride, table_len,
+                      first, count, stream);
 }
 
 }  // extern "C"

@@ -44,9 +44,22 @@ struct AttnArgs {
   int split;             // 1: no split
   float* ws_o;           // [slot][2][128][128] fp32: O / l of one part, slot = (unit - full_units) * split + part
   float* ws_lse;         // [slot][2][128] fp32: m + log2(l) of one part (log2 units of the scaled scores)
+  // Block lists (the kernel's sparse form only).  Query block i of head h of batch row b attends the key
+  // blocks blocks[((b * grid_heads + h) * list_rows + i) * list_len + ...]; one segment of queries and keys.
+  const int* blocks;
+  const int* counts;     // [batch][heads][list_rows] entries in use of each list, or null: list_len
+  int list_rows;         // query blocks of one head
+  int list_len;          // entries of one list
+  int pairs_per_list;    // query block rows / 256
+  int key_block;         // rows of a key block
+  int key_blocks;        // ceil(seg_rows_k / key_block); a listed block outside [0, key_blocks) holds no key
+  int piece;             // rows of one K/V load: 128, or 64 when key_block is not a multiple of 128
+  const int* q_len;      // [batch] query rows in use, or null: all; output rows behind them are zero
+  const int* k_len;      // [batch] key rows in use, or null: all; what lies behind them is not used
 };
 
 constexpr int kMaxSplit = 8;
+constexpr int kMaxSparseSplit = 32;
 // Workspace bytes for up to 160 SMs: one partial (O, lse) per CTA of a wave.
 constexpr int64_t kAttnWorkspaceBytes = int64_t(160) * 2 * 128 * (128 + 1) * 4;
 
@@ -55,6 +68,9 @@ constexpr int64_t kAttnWorkspaceBytes = int64_t(160) * 2 * 128 * (128 + 1) * 4;
 int launch_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                      const CUtensorMap& tqp, const CUtensorMap& tkp, const CUtensorMap& tvp,
                      const AttnArgs& args, int64_t total_units, bool fp16, cudaStream_t stream);
+// The same over the block lists of `args` (attn_fwd_kernel's sparse form).
+int launch_sparse_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args,
+                            int64_t total_units, bool fp16, cudaStream_t stream);
 
 // Process-wide count of kernels this library launched (ps_b200_kernel_launches).
 void count_launch();
@@ -148,6 +164,55 @@ struct BroadcastArgs {
 };
 
 int launch_broadcast(const BroadcastArgs& a, cudaStream_t stream);
+
+// Block means (sparse.cu) of one tensor [batch][len][heads][128].
+struct MeansTensor {
+  const void* x;
+  int64_t st[3];           // batch, row, head strides in elements
+  int len, heads, block;
+  int blocks;              // ceil(len / block)
+  int head_pairs;          // ceil(heads / 2)
+  int64_t ctas;            // batch * blocks * head_pairs
+  const int* lens;         // [batch] rows in use, or null: len
+  float* out;              // [batch][blocks][heads][128]
+};
+struct MeansArgs {
+  MeansTensor t[2];        // the second one is empty (ctas 0) or of the same type and batch
+};
+int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream);
+
+constexpr size_t kSelectSmemLimit = 200 * 1024;
+struct SelectArgs {
+  const float* q_means;    // [batch][q_blocks][kv_heads * group][128]
+  const float* k_means;    // [batch][k_blocks][kv_heads][128]
+  int batch, kv_heads, group, q_blocks, k_blocks, keep;
+  int query_block, key_block;
+  const int* q_len;        // [batch] rows in use, or null
+  const int* k_len;
+  const uint8_t* allowed;  // truth value of (batch, head, query block, key block) under these strides, or null
+  int64_t allowed_st[4];
+  int* blocks;             // [batch][heads][q_blocks][keep]
+  int* counts;             // [batch][heads][q_blocks]
+};
+int launch_block_select(const SelectArgs& a, cudaStream_t stream);
+
+// 8-bit key/value cache (cache.cu).
+struct CacheArgs {
+  void* pages[2];          // K and V codes [pages][page_rows][heads][head_dim], 8 bits each
+  float* scales[2];        // [pages][page_rows][heads]
+  void* rows[2];           // 16-bit rows: read from by the write, written to by the read
+  int64_t st[2][3];        // batch, row, head strides of the 16-bit rows in elements
+  int batch, n;            // rows of each sequence in `rows`
+  int heads, head_dim;
+  int num_pages, page_rows;
+  const int* table;        // [batch][table_len] page of each page_rows positions
+  int64_t table_st;
+  int table_len;
+  const int* first;        // [batch] position of row 0, or null: 0
+  const int* count;        // write: [batch] rows in use, or null: n; read: [batch] positions held
+};
+int launch_cache_write(const CacheArgs& a, bool fp16, bool int8, cudaStream_t stream);
+int launch_cache_read(const CacheArgs& a, bool fp16, bool int8, cudaStream_t stream);
 
 // Error bookkeeping (thread-local message, returned code).
 int set_error(int code, const char* fmt, ...);

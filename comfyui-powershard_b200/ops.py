@@ -640,3 +640,194 @@ def out_projection(src, w_o, b_o, out, n_local: int, in_features: int, row_strid
     _lib.check(rc, "ps_b200_out_proj")
     if status is not None:
         status.arm()
+
+
+class PinnedStatus(DeviceStatus):
+    """A status word in pinned host memory that the kernels write directly (on
+    an expired wait only), so a call costs no copy and no event to arm it, and
+    ``poll`` sees the error of any finished launch, graph replays included."""
+
+    def __init__(self, device: torch.device):
+        self.device = device
+        self.word = self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        self.value = self.word.numpy()
+
+    def arm(self):
+        pass
+
+    def poll(self):
+        if self.value[0]:
+            self._raise_if_set(int(self.value[0]))
+
+
+def _lengths_arg(lengths, batch: int, device, what: str):
+    """Device address of an int32 [batch] table of rows in use (None: all)."""
+    if lengths is None:
+        return None
+    if (lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch or lengths.device != device
+            or not lengths.is_contiguous()):
+        raise ValueError(f"{what}: expected contiguous int32 [{batch}] on {device}, "
+                         f"got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
+    return lengths.data_ptr()
+
+
+def _row_strides(t: torch.Tensor, what: str):
+    """(batch, row, head) strides of a [B, L, H, D] tensor the kernels can read."""
+    _check16(t, what)
+    st = t.stride()
+    if t.dim() != 4 or st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{what}: expected [B, L, H, D] with unit head-dim stride, other strides multiples of 8 "
+                         f"elements and a 16-byte aligned base, got {tuple(t.shape)} / {st}")
+    return st[:3]
+
+
+def block_means(tensors, blocks, lengths, means):
+    """Mean row of each block of rows (one launch for one or two tensors).
+
+    tensors: x [B, L, H, 128] 16-bit each; blocks: rows of a block each;
+    lengths: int32 [B] rows in use or None each; means: fp32
+    [B, ceil(L/block), H, 128] each, written (a block without rows: zeros)."""
+    lib = _lib.load()
+    x = tensors[0]
+    device, batch = x.device, x.shape[0]
+    strides, lens = [], []
+    for t, block, n, out in zip(tensors, blocks, lengths, means):
+        strides += _row_strides(t, "block_means")
+        if block < 1:
+            raise ValueError(f"block_means: blocks of {block} rows")
+        if t.dtype != x.dtype or t.shape[0] != batch or t.device != device:
+            raise ValueError("block_means: the tensors need one dtype, batch and device")
+        shape = (batch, -(-t.shape[1] // block), t.shape[2], t.shape[3])
+        if tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or out.device != device:
+            raise ValueError(f"block_means: means must be contiguous fp32 {shape} on {device}")
+        lens.append(_lengths_arg(n, batch, device, "block_means lengths") or 0)
+    rc = lib.ps_b200_block_means(
+        len(tensors), _lib.ptrs([t.data_ptr() for t in tensors]), _lib.i64(strides), _lib.dtype_code(x.dtype), batch,
+        _lib.i32([t.shape[1] for t in tensors]), _lib.i32([t.shape[2] for t in tensors]), x.shape[3], _lib.i32(blocks),
+        _lib.ptrs(lens), _lib.ptrs([t.data_ptr() for t in means]), _lib.stream_handle(device))
+    _lib.check(rc, "ps_b200_block_means")
+
+
+def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, key_block: int, allowed=None,
+                 query_lengths=None, key_lengths=None):
+    """The ``keep`` best key blocks of each query block, by the score of their means.
+
+    q_means [B, nq, Hq, 128], k_means [B, nk, Hk, 128] fp32; allowed: bool
+    [B, Hq, nq, nk] under any strides (a broadcast view) or None; blocks int32
+    [B, Hq, nq, keep] and counts int32 [B, Hq, nq] are written."""
+    lib = _lib.load()
+    device = q_means.device
+    for t, name in ((q_means, "q_means"), (k_means, "k_means")):
+        _lib.require_cuda(t, f"block_select {name}")
+        if t.dim() != 4 or t.dtype != torch.float32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"block_select {name}: expected contiguous fp32 [B, blocks, H, D] on {device}")
+    batch, nq, hq, dim = q_means.shape
+    nk, hk = k_means.shape[1:3]
+    if k_means.shape[0] != batch or k_means.shape[3] != dim:
+        raise ValueError("block_select: q_means and k_means differ in batch or head_dim")
+    for t, shape, name in ((blocks, (batch, hq, nq, keep), "blocks"), (counts, (batch, hq, nq), "counts")):
+        if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"block_select {name}: expected contiguous int32 {shape} on {device}")
+    mask, strides = None, None
+    if allowed is not None:
+        if allowed.dtype != torch.bool or tuple(allowed.shape) != (batch, hq, nq, nk) or allowed.device != device:
+            raise ValueError(f"block_select: allowed must be bool {(batch, hq, nq, nk)} on {device}")
+        mask, strides = allowed.data_ptr(), _lib.i64(allowed.stride())
+    rc = lib.ps_b200_block_select(
+        q_means.data_ptr(), k_means.data_ptr(), batch, hq, hk, dim, nq, nk, keep, mask, strides,
+        _lengths_arg(query_lengths, batch, device, "block_select query_lengths"), query_block,
+        _lengths_arg(key_lengths, batch, device, "block_select key_lengths"), key_block, blocks.data_ptr(),
+        counts.data_ptr(), _lib.stream_handle(device))
+    _lib.check(rc, "ps_b200_block_select")
+
+
+def sparse_attention_workspace(batch: int, heads: int, len_q: int, list_len: int, key_block: int, device):
+    """Scratch of one ``sparse_attention`` call of these sizes on ``device``
+    (None when it needs none); one per call in flight."""
+    with torch.cuda.device(device):
+        n = _lib.load().ps_b200_sparse_attn_workspace_bytes(batch, heads, len_q, list_len, key_block)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: int, scale: float,
+                     status: DeviceStatus | None, workspace=None, query_lengths=None, key_lengths=None):
+    """Attention of each block of queries over the key blocks its list names.
+
+    q/out [B, Lq, Hq, 128], k/v [B, Lk, Hk, 128] 16-bit; blocks int32
+    [B, Hq, ceil(Lq/query_block), n] (an entry outside the key blocks names no
+    key), counts int32 [B, Hq, ceil(Lq/query_block)] entries in use or None."""
+    lib = _lib.load()
+    device = q.device
+    st = [_lib.i64(_row_strides(t, f"sparse attention {n}")) for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
+    batch, lq, hq, dim = q.shape
+    lk, hk = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim or out.shape != q.shape:
+        raise ValueError("sparse attention: incompatible q/k/v/out shapes")
+    if any(t.dtype != q.dtype or t.device != device for t in (k, v, out)):
+        raise ValueError("sparse attention: q/k/v/out need one dtype and device")
+    nq = -(-lq // query_block)
+    if (blocks.dtype != torch.int32 or blocks.dim() != 4 or tuple(blocks.shape[:3]) != (batch, hq, nq)
+            or not blocks.is_contiguous() or blocks.device != device):
+        raise ValueError(f"sparse attention: blocks must be contiguous int32 {(batch, hq, nq)} x n on {device}")
+    if counts is not None and (counts.dtype != torch.int32 or tuple(counts.shape) != (batch, hq, nq)
+                               or not counts.is_contiguous() or counts.device != device):
+        raise ValueError(f"sparse attention: counts must be contiguous int32 {(batch, hq, nq)} on {device}")
+    rc = lib.ps_b200_sparse_attn_fwd(
+        q.data_ptr(), st[0], k.data_ptr(), st[1], v.data_ptr(), st[2], out.data_ptr(), st[3], _lib.dtype_code(q.dtype),
+        batch, hq, hk, dim, lq, lk, blocks.data_ptr(), counts.data_ptr() if counts is not None else None,
+        blocks.shape[3], query_block, key_block,
+        _lengths_arg(query_lengths, batch, device, "sparse attention query_lengths"),
+        _lengths_arg(key_lengths, batch, device, "sparse attention key_lengths"), float(scale), *_ws(workspace),
+        status.ptr if status is not None else None, _lib.stream_handle(device))
+    _lib.check(rc, "ps_b200_sparse_attn_fwd")
+    if status is not None:
+        status.arm()
+
+
+_CODES = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.INT8}
+
+
+def _cache_call(name, pages, scales, rows, table, first, count):
+    lib = _lib.load()
+    k = pages[0]
+    device = k.device
+    _lib.require_cuda(k, name)
+    if k.dtype not in _CODES:
+        raise _lib.UnsupportedAttention(f"{name}: pages hold float8_e4m3fn or int8 codes, got {k.dtype}")
+    if k.dim() != 4:
+        raise ValueError(f"{name}: pages must be [pages, page_rows, H, D], got {tuple(k.shape)}")
+    for p, s in zip(pages, scales):
+        if p.shape != k.shape or p.dtype != k.dtype or p.device != device or not p.is_contiguous():
+            raise ValueError(f"{name}: K and V pages must be contiguous and alike")
+        if s.shape != k.shape[:3] or s.dtype != torch.float32 or s.device != device or not s.is_contiguous():
+            raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(k.shape[:3])} on {device}")
+    strides = []
+    x = rows[0]
+    for t in rows:
+        strides += _row_strides(t, name)
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != device or t.shape[2:] != k.shape[2:]:
+            raise ValueError(f"{name}: K and V rows must be alike, [B, n, {k.shape[2]}, {k.shape[3]}] on {device}")
+    batch, n = x.shape[:2]
+    if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.stride(1) != 1
+            or table.device != device):
+        raise ValueError(f"{name}: the page table must be int32 [{batch}, pages] with unit inner stride on {device}")
+    rc = getattr(lib, name)(
+        _lib.ptrs([t.data_ptr() for t in pages]), _lib.ptrs([t.data_ptr() for t in scales]),
+        _lib.ptrs([t.data_ptr() for t in rows]), _lib.i64(strides), _lib.dtype_code(x.dtype), _CODES[k.dtype], batch, n,
+        k.shape[2], k.shape[3], k.shape[0], k.shape[1], table.data_ptr(), table.stride(0), table.shape[1],
+        _lengths_arg(first, batch, device, f"{name} first"), _lengths_arg(count, batch, device, f"{name} count"),
+        _lib.stream_handle(device))
+    _lib.check(rc, name)
+
+
+def cache_write(pages, scales, rows, table, first=None, count=None):
+    """Quantise rows (K, V) [B, n, H, D] into pages (K, V) [P, page_rows, H, D]
+    and scales [P, page_rows, H]: row i < count[b] goes to position first[b]+i
+    of sequence b, row ``p % page_rows`` of page ``table[b, p // page_rows]``."""
+    _cache_call("ps_b200_cache_write", pages, scales, rows, table, first, count)
+
+
+def cache_read(pages, scales, rows, table, count, first=None):
+    """The positions first[b]+i < count[b] of the pages in row i of rows (K, V)
+    [B, n, H, D]; the other rows stay as they are."""
+    _cache_call("ps_b200_cache_read", pages, scales, rows, table, first, count)

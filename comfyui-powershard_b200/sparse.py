@@ -1,0 +1,176 @@
+"""Attention over the key blocks that a cheap score selects for each query block.
+
+``SparseProvider(keep)(q, k, v, options)`` has the calling convention of the
+dense ``B200Provider``, so a dispatcher (or the wrapper that H3 puts around
+it: VedaDispatch, powershard/veda/runtime.py:95-110) calls one like the other.
+It runs three steps, each also an entry point of its own for callers that keep
+a plan (the selected blocks) or the key means between calls:
+
+* ``block_means(x, block)`` - the mean row of each block, held in fp32;
+* ``select_blocks(query_means, key_means, keep)`` - the ``keep`` key blocks
+  with the largest <mean query, mean key> for each query block, among those
+  that ``allowed`` and the lengths leave (ties: the lower index);
+* ``sparse_attention(q, k, v, blocks, counts)`` - softmax attention of each
+  query block over its listed key blocks.
+
+Query blocks are multiples of 256 rows (the two query tiles of a CTA share
+their keys), key blocks multiples of 64.  Lengths are int32 device tensors
+[B]: rows behind them are not used whatever they hold, and are zeros in the
+output, as is a query that has no key.  Nothing here synchronises, so every
+call can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib, ops
+from .contract import AttentionOptions, UnsupportedAttention
+from .provider import B200Provider, _tma_ok
+
+NAME = "b200_sparse"
+QUERY_BLOCK, KEY_BLOCK = 256, 128
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy where its strides do not suit the kernels'
+    loads (an expanded axis has stride 0, which a tensor map cannot hold)."""
+    return t if _tma_ok(t) and all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape)) else t.contiguous()
+
+
+def _on(device: torch.device):
+    """Context in which `device` is current."""
+    return torch.cuda.device(device)
+
+
+def block_means(x, block: int, lengths=None):
+    """Mean over the rows in use of each block of ``block`` rows of x [B, L, H, 128]:
+    fp32 [B, ceil(L/block), H, 128] (a block without any row in use: zeros)."""
+    ops._check16(x, "block_means")
+    if x.dim() != 4 or block < 1:
+        raise ValueError(f"block_means: expected [B, L, H, D] and a positive block, got {tuple(x.shape)}, {block}")
+    x = _readable(x)
+    b, n, h, d = x.shape
+    out = torch.empty((b, -(-n // block), h, d), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        ops.block_means([x], [block], [lengths], [out])
+    return out
+
+
+def select_blocks(query_means, key_means, keep: int, *, allowed=None, query_block: int = QUERY_BLOCK,
+                  key_block: int = KEY_BLOCK, query_lengths=None, key_lengths=None):
+    """(blocks int32 [B, Hq, nq, n], counts int32 [B, Hq, nq]) with n = min(keep, nk): the chosen
+    key blocks of each query block in ascending order, -1 behind the first ``counts`` of them.
+
+    query_means [B, nq, Hq, 128], key_means [B, nk, Hk, 128] as ``block_means``
+    gives them; allowed: bool, broadcastable to [B, Hq, nq, nk]."""
+    if query_means.dim() != 4 or key_means.dim() != 4:
+        raise ValueError("select_blocks: means are [B, blocks, H, D]")
+    b, nq, h, _ = query_means.shape
+    nk = key_means.shape[1]
+    for t in (query_means, key_means):
+        _lib.require_cuda(t, "select_blocks")
+    if keep < 1:
+        raise ValueError(f"select_blocks: keep must be at least 1, got {keep}")
+    if allowed is not None:
+        if torch.broadcast_shapes(allowed.shape, (b, h, nq, nk)) != (b, h, nq, nk):
+            raise ValueError(f"select_blocks: allowed {tuple(allowed.shape)} does not broadcast to {(b, h, nq, nk)}")
+        allowed = allowed.broadcast_to(b, h, nq, nk)
+    keep = min(int(keep), nk)
+    device = query_means.device
+    blocks = torch.empty((b, h, nq, keep), dtype=torch.int32, device=device)
+    counts = torch.empty((b, h, nq), dtype=torch.int32, device=device)
+    with _on(device):
+        ops.block_select(query_means, key_means, keep, blocks, counts, query_block, key_block, allowed, query_lengths,
+                         key_lengths)
+    return blocks, counts
+
+
+_status: dict[int, ops.PinnedStatus] = {}
+
+
+def _status_for(device: torch.device) -> ops.PinnedStatus:
+    if device.index not in _status:
+        _status[device.index] = ops.PinnedStatus(device)
+    return _status[device.index]
+
+
+def sparse_attention(q, k, v, blocks, counts=None, *, query_block: int = QUERY_BLOCK, key_block: int = KEY_BLOCK,
+                     softmax_scale: float | None = None, query_lengths=None, key_lengths=None):
+    """Attention of q [B, Lq, Hq, 128] over the key blocks of k/v [B, Lk, Hk, 128] that ``blocks``
+    [B, Hq, ceil(Lq/query_block), n] names (``counts``: entries in use, None: all).  An entry
+    outside the key blocks names no key; an entry that occurs twice counts twice."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        ops._check16(t, f"sparse_attention {name}")
+        if t.dim() != 4:
+            raise ValueError(f"sparse_attention {name}: expected [B, L, H, D], got {tuple(t.shape)}")
+    status = _status_for(q.device)
+    status.poll()
+    q, k, v = _readable(q), _readable(k), _readable(v)
+    scale = q.shape[-1] ** -0.5 if softmax_scale is None else float(softmax_scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    with _on(q.device):
+        workspace = ops.sparse_attention_workspace(q.shape[0], q.shape[2], q.shape[1], blocks.shape[-1], key_block,
+                                                   q.device)
+        ops.sparse_attention(q, k, v, out, blocks, counts, query_block, key_block, scale, status, workspace,
+                             query_lengths, key_lengths)
+    return out
+
+
+class SparseProvider(B200Provider):
+    """Block-sparse attention behind the provider API.
+
+    keep: key blocks that each query block attends - a number of blocks, or a
+    fraction of them in (0, 1] as a float."""
+
+    name = NAME
+
+    def __init__(self, keep, *, query_block: int = QUERY_BLOCK, key_block: int = KEY_BLOCK):
+        super().__init__()
+        if isinstance(keep, float) and not 0 < keep <= 1 or not isinstance(keep, float) and keep < 1:
+            raise ValueError(f"keep: a positive number of blocks or a fraction in (0, 1], got {keep}")
+        if query_block < 256 or query_block % 256 or key_block < 64 or key_block % 64:
+            raise ValueError("query_block is a multiple of 256 and key_block of 64, "
+                             f"got {query_block} and {key_block}")
+        self.keep, self.query_block, self.key_block = keep, query_block, key_block
+        self.identity["provider"] = NAME
+
+    def check(self, q, k, v, o: AttentionOptions):
+        super().check(q, k, v, o)
+        if o.softmax_scale is not None and not o.softmax_scale > 0:
+            raise UnsupportedAttention("b200_sparse: the selection ranks by a positive softmax_scale")
+
+    def blocks_kept(self, key_blocks: int) -> int:
+        """Key blocks each query block attends, of ``key_blocks``."""
+        n = math.ceil(self.keep * key_blocks) if isinstance(self.keep, float) else self.keep
+        return min(n, key_blocks)
+
+    def __call__(self, q, k, v, o: AttentionOptions | None = None, *, allowed=None, key_means=None,
+                 query_lengths=None, key_lengths=None):
+        """q [B, Lq, Hq, 128], k/v [B, Lk, Hk, 128] -> [B, Lq, Hq, 128].
+
+        key_means: ``block_means(k, key_block, key_lengths)`` kept from an
+        earlier call (of a cache that grew, its new blocks' means appended);
+        allowed: bool, broadcastable to [B, Hq, query blocks, key blocks]."""
+        o = o or AttentionOptions()
+        self.check(q, k, v, o)
+        q, k, v = _readable(q), _readable(k), _readable(v)
+        b, lq, h, d = q.shape
+        lk, hk = k.shape[1:3]
+        nq, nk = -(-lq // self.query_block), -(-lk // self.key_block)
+        q_means = torch.empty((b, nq, h, d), dtype=torch.float32, device=q.device)
+        with _on(q.device):
+            if key_means is None:
+                key_means = torch.empty((b, nk, hk, d), dtype=torch.float32, device=q.device)
+                ops.block_means([q, k], [self.query_block, self.key_block], [query_lengths, key_lengths],
+                                [q_means, key_means])
+            else:
+                if tuple(key_means.shape) != (b, nk, hk, d):
+                    raise ValueError(f"key_means: expected {(b, nk, hk, d)}, got {tuple(key_means.shape)}")
+                ops.block_means([q], [self.query_block], [query_lengths], [q_means])
+        blocks, counts = select_blocks(
+            q_means, key_means, self.blocks_kept(nk), allowed=allowed, query_block=self.query_block,
+            key_block=self.key_block, query_lengths=query_lengths, key_lengths=key_lengths)
+        return sparse_attention(q, k, v, blocks, counts, query_block=self.query_block, key_block=self.key_block,
+                                softmax_scale=o.softmax_scale, query_lengths=query_lengths, key_lengths=key_lengths)

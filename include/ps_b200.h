@@ -56,6 +56,13 @@
  *                          one exchange, as the reference packs it: send
  *                          [W, T, B, width, h, D] (wan_model.py:350-362) and
  *                          output send [W, B, width, h, D] (:373-378).
+ *   ps_b200_block_means, ps_b200_block_select, ps_b200_sparse_attn_fwd
+ *                          block-sparse attention behind the provider call (a
+ *                          wrapper of the dispatcher there: VedaDispatch,
+ *                          powershard/veda/runtime.py:95-110); own formulas.
+ *   ps_b200_cache_write, ps_b200_cache_read
+ *                          no reference counterpart (8-bit cache of keys and
+ *                          values for streaming generation).
  *   ps_b200_kernel_launches, ps_b200_selftest_bounded_wait,
  *   ps_b200_block_fwd_static  no reference counterpart (instrumentation,
  *                          failure-detection self-test, allocation-free block).
@@ -87,6 +94,8 @@ extern "C" {
 #define PS_B200_BF16 0
 #define PS_B200_FP16 1
 #define PS_B200_FP32 2
+#define PS_B200_E4M3 3 /* codes of the 8-bit cache */
+#define PS_B200_INT8 4
 
 /* Device status codes written to *status by the attention kernel when one of
  * its bounded internal waits expires (the launch then returns early, the
@@ -411,6 +420,84 @@ int ps_b200_qkv_proj_batch(const void* x, int64_t x_row_stride, const void* w_q,
 int ps_b200_out_proj(const void* src, int64_t src_row_stride, int64_t src_block_stride, int src_block_cols,
                      const void* w_o, const void* b_o, int b_dtype, void* out, int64_t out_row_stride, int dtype,
                      int out_dtype, int n_local, int in_features, int out_features, int* status, void* stream);
+
+/*
+ * ps_b200_block_means: the mean row of each block of rows, per head.
+ *   One or two tensors (tensors = 1 or 2; tables of that many entries), each
+ *   x[t] [batch][len[t]][heads[t]][head_dim 128] in dtype (bf16/fp16) under
+ *   strides[3t..3t+2] (batch, row, head, elements); out[t] fp32
+ *   [batch][ceil(len[t]/block[t])][heads[t]][head_dim].  lens (may be NULL, as
+ *   may lens[t]): device int [batch], rows in use (clamped to [0, len]); only
+ *   those count, and a block without any has mean zero.
+ */
+int ps_b200_block_means(int tensors, const void* const* x, const int64_t* strides, int dtype, int batch,
+                        const int* len, const int* heads, int head_dim, const int* block, const int* const* lens,
+                        float* const* out, void* stream);
+
+/*
+ * ps_b200_block_select: for each block of queries the `keep` key blocks with
+ *   the largest score <q_means, k_means> (64-bit sums; of equal scores the
+ *   lower index).  q_means [batch][q_blocks][heads_q][128], k_means
+ *   [batch][k_blocks][heads_kv][128] fp32; query head h scores against key head
+ *   h / (heads_q / heads_kv).  allowed (may be NULL): one byte per (batch,
+ *   head, query block, key block) under allowed_strides, 0 = never chosen.
+ *   q_len / k_len (device int [batch], may be NULL): rows in use; key blocks
+ *   behind them are never chosen, query blocks behind them choose none.  A
+ *   score of NaN ranks above all numbers.  blocks [batch][heads_q][q_blocks]
+ *   [keep]: the chosen in ascending order, -1 behind them; counts
+ *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 25472.
+ */
+int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv,
+                         int head_dim, int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
+                         const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
+                         int key_block, int* blocks, int* counts, void* stream);
+
+/*
+ * ps_b200_sparse_attn_fwd: softmax attention of each block of query_block rows
+ *   (a multiple of 256) over the key blocks of key_block rows (a multiple of
+ *   64) that its list names: blocks [batch][heads_q][ceil(len_q/query_block)]
+ *   [list_len], counts (may be NULL: list_len) entries of each list in use.
+ *   q/out [batch][len_q][heads_q][128], k/v [batch][len_k][heads_kv][128] under
+ *   strides (batch, row, head; multiples of 8 elements).  A list entry outside
+ *   the key blocks names no key; one that occurs twice counts twice.  q_len /
+ *   k_len as above: keys behind k_len are not used whatever they hold, output
+ *   rows behind q_len and rows without a key are zeros.  workspace: device
+ *   scratch of ps_b200_sparse_attn_workspace_bytes(...) bytes (0: none), owned
+ *   by one call at a time.  status: device or pinned host int (may be NULL).
+ */
+size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block);
+int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                            const void* v, const int64_t v_strides[3], void* out, const int64_t out_strides[3],
+                            int dtype, int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k,
+                            const int* blocks, const int* counts, int list_len, int query_block, int key_block,
+                            const int* q_len, const int* k_len, float softmax_scale, void* workspace,
+                            size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * 8-bit key/value cache in pages.  pages: K and V codes
+ *   [num_pages][page_rows][heads][head_dim] (cache_dtype PS_B200_E4M3 or _INT8),
+ *   scales fp32 [num_pages][page_rows][heads].  Position p of sequence b lives
+ *   in row p % page_rows of page table[b*table_stride + p / page_rows] (device
+ *   ints).  rows: K and V [batch][n][heads][head_dim] bf16/fp16 under strides
+ *   (batch, row, head of K, then of V; multiples of 8 elements); head_dim 64,
+ *   128 or 256.
+ * ps_b200_cache_write stores row i < count[b] (NULL: n) of sequence b at position
+ *   first[b] + i (NULL: i): scale = max(max|x|, 2^-100) / M over the head's
+ *   values, code = round(x * (M / max(..))), M = 448 or 127.  Rows whose position
+ *   or page is out of range are dropped.  Two rows of one call must not name
+ *   the same position of the same page.
+ * ps_b200_cache_read gives position first[b] + i in row i, for positions below
+ *   count[b]; the rows behind them stay as they are, a position whose page is
+ *   out of range reads as zeros.
+ */
+int ps_b200_cache_write(void* const pages[2], float* const scales[2], const void* const rows[2],
+                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
+                        int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
+                        int table_len, const int* first, const int* count, void* stream);
+int ps_b200_cache_read(const void* const pages[2], const float* const scales[2], void* const rows[2],
+                       const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
+                       int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
+                       int table_len, const int* first, const int* count, void* stream);
 
 /*
  * Self-test of the bounded waits (no counterpart in the reference): one warp

@@ -1,0 +1,409 @@
+"""Block-sparse attention: block means, selection, attention over listed blocks.
+
+The references are plain 64-bit computations on the CPU, one head and query
+block at a time.  Tolerances:
+* means: one rounding to fp32 (2^-24 of the mean) and the 32-bit sums of four
+  values (3 * 2^-24 of the mean magnitude);
+* selection: equal (whole numbers);
+* attention: with A = sum p |v| / sum p, the probabilities' rounding to 16 bits
+  (u = eps/2) gives u A, the output's u |out|; a score is a 32-bit sum of 128
+  products, off by at most 128 * 2^-23 * sum |q k| * scale <= 2^-12 for rows of
+  this size (sum |q k| * scale <= 16), which enters numerator and denominator:
+  2^-11 A.
+"""
+import math
+
+import pytest
+import torch
+
+DEV = "cuda"
+
+
+def rows(seed, *shape, dtype=torch.bfloat16, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def ref_means(x, block, lengths=None):
+    b, n, h, d = x.shape
+    out = torch.zeros(b, -(-n // block), h, d, dtype=torch.float64)
+    for i in range(b):
+        used = n if lengths is None else min(max(int(lengths[i]), 0), n)
+        for j in range(out.shape[1]):
+            part = x[i, j * block:min((j + 1) * block, used)].double()
+            if len(part):
+                out[i, j] = part.mean(0)
+    return out
+
+
+def ref_select(q_means, k_means, keep, allowed=None, q_used=None, k_used=None):
+    """q_used / k_used: blocks in use of each sequence."""
+    b, nq, h, _ = q_means.shape
+    nk, hk = k_means.shape[1:3]
+    keep = min(keep, nk)
+    blocks = torch.full((b, h, nq, keep), -1, dtype=torch.int32)
+    counts = torch.zeros(b, h, nq, dtype=torch.int32)
+    for i in range(b):
+        for j in range(h):
+            for t in range(nq if q_used is None else q_used[i]):
+                s = k_means[i, :, j // (h // hk)].double() @ q_means[i, t, j].double()
+                may = [n for n in range(nk if k_used is None else k_used[i])
+                       if allowed is None or bool(allowed.broadcast_to(b, h, nq, nk)[i, j, t, n])]
+                key = lambda n: (0 if math.isnan(s[n]) else 1, 0 if math.isnan(s[n]) else -float(s[n]), n)  # noqa: E731
+                best = sorted(sorted(may, key=key)[:keep])
+                counts[i, j, t] = len(best)
+                blocks[i, j, t, :len(best)] = torch.tensor(best, dtype=torch.int32)
+    return blocks, counts
+
+
+def ref_attention(q, k, v, blocks, counts=None, query_block=256, key_block=128, scale=None, q_len=None, k_len=None):
+    """(out, A) in 64 bits: A bounds what a relative error of the probabilities can move."""
+    b, lq, h, d = q.shape
+    lk, hk = k.shape[1:3]
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.zeros(b, lq, h, d, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    for i in range(b):
+        ql = lq if q_len is None else min(max(int(q_len[i]), 0), lq)
+        kl = lk if k_len is None else min(max(int(k_len[i]), 0), lk)
+        for j in range(h):
+            for t in range(blocks.shape[2]):
+                r = slice(t * query_block, min((t + 1) * query_block, ql))
+                if r.start >= ql:
+                    continue
+                n = blocks.shape[3] if counts is None else min(max(int(counts[i, j, t]), 0), blocks.shape[3])
+                at = [p for e in blocks[i, j, t, :n].tolist() if e >= 0
+                      for p in range(e * key_block, min((e + 1) * key_block, kl))]
+                if not at:
+                    continue
+                kk, vv = k[i, at, j // (h // hk)].double(), v[i, at, j // (h // hk)].double()
+                p = torch.softmax(q[i, r, j].double() @ kk.T * scale, -1)
+                out[i, r, j], mag[i, r, j] = p @ vv, p @ vv.abs()
+    return out, mag
+
+
+def assert_attention(got, want, mag):
+    u = torch.finfo(got.dtype).eps / 2
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    bound = (u + 2.0 ** -11) * mag + u * want.abs() + 1e-30
+    worst = ((got - want).abs() / bound).max()
+    assert worst <= 1.0, f"{float(worst):.2f} of the bound"
+
+
+def cuda(*ts):
+    return [t if t is None else t.to(DEV) for t in ts]
+
+
+def lens(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+# ------------------------------------------------------------------ refusals (CPU)
+def test_refusals_before_any_launch():
+    from powershard_b200 import sparse
+    from powershard_b200.contract import AttentionOptions, UnsupportedAttention
+    x = rows(0, 1, 300, 2, 128)
+    with pytest.raises(UnsupportedAttention):
+        sparse.block_means(x, 64)  # CPU tensors
+    with pytest.raises(UnsupportedAttention):
+        sparse.sparse_attention(x, x, x, torch.zeros(1, 2, 2, 1, dtype=torch.int32))
+    with pytest.raises(UnsupportedAttention):
+        sparse.select_blocks(torch.zeros(1, 2, 2, 128), torch.zeros(1, 3, 2, 128), 1)
+    for keep in (0, -1, 0.0, 1.5):
+        with pytest.raises(ValueError):
+            sparse.SparseProvider(keep)
+    for blocks in ((128, 128), (256, 32), (300, 64), (256, 100)):
+        with pytest.raises(ValueError):
+            sparse.SparseProvider(4, query_block=blocks[0], key_block=blocks[1])
+    p = sparse.SparseProvider(0.25)
+    assert [p.blocks_kept(n) for n in (1, 3, 4, 5, 256)] == [1, 1, 1, 2, 64]
+    assert sparse.SparseProvider(7).blocks_kept(5) == 5
+    for o in (AttentionOptions(causal=True), AttentionOptions(softmax_scale=-1.0), AttentionOptions()):
+        with pytest.raises(UnsupportedAttention):
+            p(x, x, x, o)  # the last one: CPU tensors
+
+
+def test_entries_validate_on_the_host():
+    from powershard_b200 import _lib
+    lib = _lib.load()
+    st = _lib.i64([0, 256, 128])
+
+    def fwd(dtype=_lib.BF16, heads=2, kv=2, dim=128, lq=300, lk=300, blocks=16, n=4, qb=256, kb=64, scale=0.1, q=16,
+            ws=None):
+        return lib.ps_b200_sparse_attn_fwd(q, st, 16, st, 16, st, 16, st, dtype, 1, heads, kv, dim, lq, lk, blocks,
+                                           None, n, qb, kb, None, None, scale, ws, 0, None, None)
+
+    assert fwd(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED
+    assert fwd(dim=64) == _lib.ERR_UNSUPPORTED and b"head_dim" in lib.ps_b200_last_error()
+    assert fwd(qb=128) == _lib.ERR_UNSUPPORTED and fwd(kb=32) == _lib.ERR_UNSUPPORTED
+    assert fwd(heads=3) == _lib.ERR_INVALID and fwd(n=0) == _lib.ERR_INVALID and fwd(lk=0) == _lib.ERR_INVALID
+    assert fwd(scale=0.0) == _lib.ERR_INVALID and fwd(scale=float("nan")) == _lib.ERR_INVALID
+    assert fwd(q=18) == _lib.ERR_INVALID and fwd(blocks=None) == _lib.ERR_INVALID and fwd(blocks=18) == _lib.ERR_INVALID
+    assert fwd(n=1 << 25) == _lib.ERR_INVALID  # names more than 2^30 rows
+    assert fwd(lq=0) == _lib.OK
+
+    def select(heads=2, kv=2, dim=128, nq=2, nk=5, keep=3, means=16, lists=16):
+        return lib.ps_b200_block_select(means, 16, 1, heads, kv, dim, nq, nk, keep, None, None, None, 256, None, 64,
+                                        lists, 16, None)
+
+    assert select(keep=0) == _lib.ERR_INVALID and select(keep=6) == _lib.ERR_INVALID
+    assert select(heads=3) == _lib.ERR_INVALID and select(dim=64) == _lib.ERR_UNSUPPORTED
+    assert select(nk=30000) == _lib.ERR_UNSUPPORTED and b"larger blocks" in lib.ps_b200_last_error()
+    assert select(means=20) == _lib.ERR_INVALID and select(lists=None) == _lib.ERR_INVALID
+    assert select(nq=0) == _lib.OK
+
+    def means(n=1, dtype=_lib.BF16, dim=128, block=64, length=100, x=16, stride=128):
+        return lib.ps_b200_block_means(n, _lib.ptrs([x]), _lib.i64([0, stride, 128]), dtype, 1, _lib.i32([length]),
+                                       _lib.i32([1]), dim, _lib.i32([block]), None, _lib.ptrs([16]), None)
+
+    assert means(n=3) == _lib.ERR_INVALID and means(block=0) == _lib.ERR_INVALID and means(x=24) == _lib.ERR_INVALID
+    assert means(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED and means(dim=64) == _lib.ERR_UNSUPPORTED
+    assert means(stride=130) == _lib.ERR_INVALID and means(length=0) == _lib.OK
+    assert lib.ps_b200_kernel_launches() == 0
+
+
+# ------------------------------------------------------------------ means
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,heads,block", [(1, 1, 64), (300, 3, 64), (1000, 4, 256), (517, 5, 128), (130, 2, 7)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_block_means(cuda_lib, n, heads, block, dtype):
+    from powershard_b200 import sparse
+    x = rows(1, 2, n, heads, 128, dtype=dtype)
+    used = lens(n, n // 3)
+    x[1, n // 3:] = float("nan")
+    got = sparse.block_means(x.to(DEV), block, used.to(DEV)).double().cpu()
+    want, size = ref_means(x, block, used), ref_means(x.abs(), block, used)
+    assert ((got - want).abs() <= 2.0 ** -24 * want.abs() + 3 * 2.0 ** -24 * size).all()
+    strided = torch.cat([x, x], 2).transpose(1, 2).contiguous().transpose(1, 2)[:, :, :heads].to(DEV)
+    assert torch.equal(sparse.block_means(strided, block, used.to(DEV)).double().cpu(), got)
+    wide = x[:, :, :1].to(DEV).expand(-1, -1, 3, -1)  # heads that share their rows
+    assert torch.equal(sparse.block_means(wide, block, used.to(DEV))[:, :, 2].double().cpu(), got[:, :, 0])
+
+
+# ------------------------------------------------------------------ selection
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,nq,nk,heads,kv,keep", [
+    (1, 1, 1, 1, 1, 1), (2, 3, 7, 4, 2, 3), (1, 9, 300, 2, 2, 40), (1, 1, 513, 5, 1, 100), (2, 1, 64, 2, 2, 64),
+    (1, 2, 2600, 1, 1, 260), (1, 5, 4000, 1, 1, 17), (1, 17, 33, 3, 3, 32)])
+def test_select_blocks(cuda_lib, b, nq, nk, heads, kv, keep):
+    from powershard_b200 import sparse
+    qm, km = rows(2, b, nq, heads, 128, dtype=torch.float32), rows(3, b, nk, kv, 128, dtype=torch.float32)
+    got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
+    want = ref_select(qm, km, keep)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    allowed = torch.rand(nq, nk, generator=torch.Generator().manual_seed(4)) < 0.5
+    allowed[0] = False  # a block of queries that may see nothing
+    ql, kl = [0 if i else nq for i in range(b)], [max(1, nk - 5 * i - 1) for i in range(b)]
+    got = [t.cpu() for t in sparse.select_blocks(
+        *cuda(qm, km), keep, allowed=allowed.to(DEV), query_lengths=(lens(*ql) * 256).to(DEV),
+        key_lengths=(lens(*kl) * 128 - 127).to(DEV))]
+    want = ref_select(qm, km, keep, allowed, ql, kl)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert not got[1][:, :, 0].any() and (got[0][:, :, 0] == -1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nq", [1, 6])
+def test_select_ties_and_nan(cuda_lib, nq):
+    """Equal scores go to the lower index (0 and -0 among them), NaN is chosen, infinities rank as they are."""
+    from powershard_b200 import sparse
+    qm, km = torch.zeros(1, nq, 1, 128), torch.zeros(1, 40, 1, 128)
+    qm[..., 0] = 1.0
+    km[0, :, 0, 0] = torch.tensor([0.0, -0.0] * 10 + [1.0] * 12 + [-1.0] * 8)
+    for keep in (1, 5, 12, 13, 20, 32, 35, 40):
+        got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
+        want = ref_select(qm, km, keep)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
+    qm[..., 1] = 1.0
+    km[0, 37, 0, 0], km[0, 38, 0, 0] = float("nan"), float("-inf")
+    km[0, 36, 0, 0] = float("inf")
+    for keep in (1, 2, 3, 39, 40):
+        got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
+        want = ref_select(qm, km, keep)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
+
+
+# ------------------------------------------------------------------ attention over lists
+def random_lists(seed, b, h, nq, nk, n):
+    g = torch.Generator().manual_seed(seed)
+    return torch.stack([torch.randperm(nk, generator=g)[:n] for _ in range(b * h * nq)]).view(b, h, nq, n).to(torch.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk,heads,kv,key_block,n", [
+    (256, 256, 1, 1, 128, 1), (256, 512, 2, 2, 64, 3), (300, 1000, 2, 1, 128, 5), (1, 1, 1, 1, 64, 1),
+    (1, 700, 4, 2, 64, 9), (513, 257, 2, 2, 64, 5), (130, 2000, 3, 1, 192, 10), (257, 1300, 2, 2, 256, 4),
+    (70, 5000, 2, 2, 64, 70)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_sparse_attention(cuda_lib, lq, lk, heads, kv, key_block, n, dtype):
+    from powershard_b200 import sparse
+    b = 2
+    q, k, v = (rows(s, b, m, h, 128, dtype=dtype) for s, m, h in ((5, lq, heads), (6, lk, kv), (7, lk, kv)))
+    blocks = random_lists(8, b, heads, -(-lq // 256), -(-lk // key_block), n)
+    got = sparse.sparse_attention(*cuda(q, k, v, blocks), key_block=key_block)
+    torch.cuda.synchronize()
+    sparse._status_for(got.device).check()
+    assert_attention(got, *ref_attention(q, k, v, blocks, key_block=key_block))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("key_block", [64, 128])
+def test_sparse_attention_lists_of_any_kind(cuda_lib, key_block):
+    """Short and empty lists, entries that name no block, repeated and unordered entries, and what lies behind
+    the lengths (NaN and infinities), in the whole and in the split form."""
+    from powershard_b200 import sparse
+    for b, heads, lq, lk, n in ((2, 3, 600, 1111, 7), (3, 2, 40, 3000, 20)):
+        q, k, v = (rows(s, b, m, heads, 128) for s, m in ((9, lq), (10, lk), (11, lk)))
+        nq, nk = -(-lq // 256), -(-lk // key_block)
+        blocks = random_lists(12, b, heads, nq, nk, n)
+        blocks[0, 0, 0, :3] = torch.tensor([-1, nk, 2 ** 31 - 1])
+        blocks[0, 1, 0, :] = -5                       # nothing but entries without a block
+        blocks[1, 0, 0, :4] = torch.tensor([3, 3, 0, 3])  # counts each time
+        blocks[1, 1, 0, 0] = nk - 1                   # the block that ends inside the tensor
+        counts = torch.full((b, heads, nq), n, dtype=torch.int32)
+        counts[0, 0, -1], counts[1, 1, -1], counts[1, 0, 0] = 1, 0, n + 9  # clamped to the list
+        q_len, k_len = lens(lq, lq - 7, 0)[:b], lens(lk - 70, lk, 33)[:b]
+        for i in range(b):
+            q[i, int(q_len[i]):] = float("nan")
+            k[i, int(k_len[i]):] = float("inf")
+            v[i, int(k_len[i]):] = float("nan")
+        got = sparse.sparse_attention(*cuda(q, k, v, blocks, counts), key_block=key_block,
+                                      query_lengths=q_len.to(DEV), key_lengths=k_len.to(DEV))
+        assert_attention(got, *ref_attention(q, k, v, blocks, counts, 256, key_block, None, q_len, k_len))
+        assert not got[0, :256, 1].any()  # only invalid entries: zeros
+        for i in range(b):
+            assert not got[i, int(q_len[i]):].any()
+
+
+@pytest.mark.gpu
+def test_sparse_attention_all_blocks_is_dense(cuda_lib):
+    """With every block listed in order the result is the dense kernel's."""
+    from powershard_b200 import sparse
+    from powershard_b200.provider import B200Provider
+    q, k, v = (rows(s, 1, 1500, 4, 128).to(DEV) for s in (13, 14, 15))
+    blocks = torch.arange(12, dtype=torch.int32, device=DEV).expand(1, 4, 6, 12).contiguous()
+    out = sparse.sparse_attention(q, k, v, blocks, softmax_scale=0.05)
+    from powershard_b200 import ops
+    dense = torch.empty_like(q)
+    ops.attention_blhd(q, k, v, dense, 0.05, None, None)
+    # both walk the keys in the same order; only the split of the last wave differs
+    err = (out.double() - dense.double()).abs().max()
+    assert err <= 2 * 2.0 ** -8 * v.abs().max().double()
+    assert_attention(out, *ref_attention(q.cpu(), k.cpu(), v.cpu(), blocks.cpu(), scale=0.05))
+    assert isinstance(B200Provider().identity, dict)
+
+
+@pytest.mark.gpu
+def test_arguments_are_checked(cuda_lib):
+    from powershard_b200 import sparse
+    qm, km = torch.zeros(1, 2, 2, 128, device=DEV), torch.zeros(1, 3, 2, 128, device=DEV)
+    with pytest.raises(ValueError):
+        sparse.select_blocks(qm, km, 0)
+    for bad in (dict(allowed=torch.ones(5, 3, dtype=torch.bool, device=DEV)), dict(allowed=torch.ones(2, 3, device=DEV)),
+                dict(key_lengths=lens(3)), dict(key_lengths=torch.tensor([3], device=DEV)),
+                dict(query_lengths=lens(3, 3).to(DEV))):
+        with pytest.raises((ValueError, RuntimeError)):
+            sparse.select_blocks(qm, km, 1, **bad)
+    x = rows(0, 1, 300, 2, 128).to(DEV)
+    ok = torch.zeros(1, 2, 2, 1, dtype=torch.int32, device=DEV)
+    for q, k, lists in ((x, x[:, :, :, :64], ok), (x, x, ok.long()), (x, x, ok[:, :1]), (x, x.half(), ok), (x, x[:, :0], ok)):
+        with pytest.raises((ValueError, RuntimeError)):
+            sparse.sparse_attention(q, k, k, lists)
+    with pytest.raises(ValueError):
+        sparse.SparseProvider(1)(x, x, x, key_means=torch.zeros(1, 2, 2, 128, device=DEV))  # of another length
+    assert sparse.SparseProvider(1)(x[:, :0], x, x).shape == (1, 0, 2, 128)
+
+
+@pytest.mark.gpu
+def test_nan_keys_are_not_hidden(cuda_lib):
+    from powershard_b200 import sparse
+    q, k, v = (rows(s, 1, 512, 1, 128) for s in (16, 17, 18))
+    k[0, 200, 0, 5] = float("nan")
+    out = sparse.SparseProvider(1)(*cuda(q, k, v))
+    assert torch.isnan(out).all()
+
+
+# ------------------------------------------------------------------ the provider
+def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_len=None, k_len=None, scale=None):
+    used = lambda n, block: None if n is None else [-(-int(x) // block) for x in n]  # noqa: E731
+    qm = ref_means(q, query_block, q_len).float()
+    km = ref_means(k, key_block, k_len).float()
+    blocks, counts = ref_select(qm, km, keep, allowed, used(q_len, query_block), used(k_len, key_block))
+    return ref_attention(q, k, v, blocks, counts, query_block, key_block, scale, q_len, k_len)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,lq,lk,heads,kv,qb,kb,keep,ragged", [
+    (1, 1000, 1000, 2, 2, 256, 128, 3, False), (2, 777, 777, 4, 2, 256, 64, 5, True), (1, 1, 4096, 3, 1, 256, 128, 8, False),
+    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (5, 1, 1, 2, 2, 256, 64, 1, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_provider(cuda_lib, b, lq, lk, heads, kv, qb, kb, keep, ragged, dtype):
+    from powershard_b200 import sparse
+    from powershard_b200.contract import AttentionOptions
+    q, k, v = (rows(s, b, m, h, 128, dtype=dtype) for s, m, h in ((19, lq, heads), (20, lk, kv), (21, lk, kv)))
+    k += rows(22, b, -(-lk // 64), kv, 128, dtype=dtype).repeat_interleave(64, 1)[:, :lk]
+    q_len = k_len = None
+    if ragged:
+        q_len = lens(*[max(0, lq - i * (lq // 2 + 1)) for i in range(b)])
+        k_len = lens(*[max(0, lk - i * (lk // 2 + 1)) for i in range(b)])
+    p = sparse.SparseProvider(keep, query_block=qb, key_block=kb)
+    got = p(*cuda(q, k, v), AttentionOptions(softmax_scale=0.07), query_lengths=None if q_len is None else q_len.to(DEV),
+            key_lengths=None if k_len is None else k_len.to(DEV))
+    assert got.shape == q.shape and got.dtype == dtype
+    assert_attention(got, *ref_provider(q, k, v, keep, qb, kb, None, q_len, k_len, 0.07))
+    if not ragged:  # kept means give the same
+        kept = sparse.block_means(k.to(DEV), kb)
+        again = p(*cuda(q, k, v), AttentionOptions(softmax_scale=0.07), key_means=kept)
+        assert torch.equal(got, again)
+
+
+@pytest.mark.gpu
+def test_provider_on_strided_inputs_streams_and_graphs(cuda_lib):
+    """Views into a fused projection, a mask that leaves a block empty, another stream, and a captured call
+    replayed on new inputs next to a second captured call."""
+    from powershard_b200 import sparse
+    from powershard_b200.graphs import GraphedCall
+    qkv = rows(23, 1, 700, 3, 4, 128).to(DEV)
+    q, k, v = qkv.unbind(2)
+    allowed = torch.ones(3, 6, dtype=torch.bool)
+    allowed[1] = False
+    allowed[2, 3:] = False
+    p = sparse.SparseProvider(0.5)
+    want = ref_provider(q.cpu(), k.cpu(), v.cpu(), 3, allowed=allowed)
+    mask = allowed.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = p(q, k, v, allowed=mask)
+    side.synchronize()
+    assert_attention(out, *want)
+    assert not out[:, 256:512].any()
+    first = GraphedCall(p, q, k, v, allowed=mask)
+    other = [x.flip(1).contiguous() for x in (q, k, v)]
+    second = GraphedCall(p, *other)
+    for _ in range(2):  # the two graphs in flight on two streams
+        with torch.cuda.stream(side):
+            a = first()
+        b = second()
+        torch.cuda.synchronize()
+        assert torch.equal(a, out)
+        assert_attention(b, *ref_provider(*(x.cpu() for x in other), 3))
+    qkv.copy_(rows(24, 1, 700, 3, 4, 128))
+    first()
+    torch.cuda.synchronize()
+    assert_attention(first.out, *ref_provider(q.cpu(), k.cpu(), v.cpu(), 3, allowed=allowed))
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_what_memory_held(cuda_lib):
+    """Two runs give the same bits, with the allocator's blocks full of NaN in between."""
+    from powershard_b200 import sparse
+    q, k, v = (rows(s, 2, 1300, 3, 128).to(DEV) for s in (25, 26, 27))
+    used = lens(1300, 0).to(DEV)
+    p = sparse.SparseProvider(4, key_block=64)
+    a = p(q, k, v, query_lengths=used, key_lengths=used).clone()
+    junk = [torch.full((1 << 24,), float("nan"), device=DEV) for _ in range(4)]
+    del junk
+    b = p(q, k, v, query_lengths=used, key_lengths=used)
+    assert torch.equal(a, b) and not b[1].any()
