@@ -126,14 +126,10 @@ SIGNATURES = {
         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
         ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, _c_intp, ctypes.c_void_p]),
-    "ps_b200_cache_write": (ctypes.c_int, [
-        _c_ptrs, _c_ptrs, _c_ptrs, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
-        ctypes.c_void_p, ctypes.c_void_p]),
-    "ps_b200_cache_read": (ctypes.c_int, [
-        _c_ptrs, _c_ptrs, _c_ptrs, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
-        ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
-        ctypes.c_void_p, ctypes.c_void_p]),
+    "ps_b200_sparse_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int] * 9),
+    "ps_b200_sparse_fwd": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),  # a packed ps_b200_sparse_call
+    "ps_b200_cache_write": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),  # a packed ps_b200_cache_call
+    "ps_b200_cache_read": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
 }
 ATTN_WORKSPACE_BYTES = 160 * 2 * 128 * 129 * 4
 IPC_HANDLE_BYTES = 64
@@ -215,6 +211,8 @@ def i64(values):
 
 
 def stream_handle(device: torch.device) -> int:
+    if device.index is not None:  # the raw handle, without a Stream object around it (2 us a call)
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -16,8 +16,8 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 ROOT = HERE.parent
 SOURCES = ["csrc/attention.cu", "csrc/prepass.cu", "csrc/proj.cu", "csrc/capi.cu", "csrc/static_block.cu",
-           "csrc/selftest.cu", "csrc/sparse.cu", "csrc/cache.cu"]
-HEADERS = ["csrc/ptx.cuh", "csrc/internal.h"]
+           "csrc/selftest.cu", "csrc/sparse.cu", "csrc/sparse_attn.cu", "csrc/cache.cu"]
+HEADERS = ["csrc/ptx.cuh", "csrc/internal.h", "csrc/attn_tile.cuh"]
 OUTPUT = HERE / "lib" / "libps_b200.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", f"-I{ROOT / 'include'}"]

@@ -17,7 +17,7 @@ import torch
 
 from . import _lib, ops
 from .contract import AttentionOptions
-from .sparse import SparseProvider
+from .sparse import SparseProvider, _on
 
 
 class KVCache:
@@ -52,14 +52,14 @@ class KVCache:
         """Rows i < lengths[b] (None: all) of k, v [B, n, heads, head_dim] to
         positions start[b] + i (None: i) of sequence b.  Rows without a page are dropped."""
         _lib.require_cuda(self.k, "cache pages")
-        with torch.cuda.device(self.k.device):
+        with _on(self.k.device):
             ops.cache_write((self.k, self.v), (self.k_scale, self.v_scale), (k, v), table, start, lengths)
 
     def read(self, table, lengths, k_out, v_out, first=None):
         """Positions first[b] + i (None: i) below lengths[b] into row i of k_out,
         v_out [B, n, heads, head_dim] (bf16 or fp16); the other rows stay as they are."""
         _lib.require_cuda(self.k, "cache pages")
-        with torch.cuda.device(self.k.device):
+        with _on(self.k.device):
             ops.cache_read((self.k, self.v), (self.k_scale, self.v_scale), (k_out, v_out), table, lengths, first)
 
 

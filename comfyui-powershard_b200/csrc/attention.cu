@@ -38,47 +38,12 @@
 // writes the second.  The exponentials use ex2.approx on the MUFU; measured on
 // B200, moving part of them to an FMA-pipe polynomial or fusing the row max
 // into the exponential pass made the softmax slower.
-//
-// Sparse form (kSparse): the keys of a CTA are the blocks that a list names for
-// its query block, so a key tile is one 128-row load or two 64-row loads from
-// anywhere in the sequence.  A query block is a multiple of 256 rows: both
-// query tiles of the CTA share the list, so each K/V tile is loaded once for
-// 256 queries, as in the dense form (a list for each 128 rows would double the
-// K/V loads: 64 KB per 128 x 128 tile pair is ~52 B/clk per SM, above the L2's
-// share).  The number of tiles is read from device memory and may be zero.
-// Rows past a sequence's key length are not used, whatever they hold: their
-// scores are masked, and as 0 * NaN is NaN in the PV product, V rows of a
-// partly used tile are overwritten with zeros in shared memory before it.
-#include "ptx.cuh"
-#include "ps_b200.h"
-#include "internal.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "attn_tile.cuh"
 
 namespace psb {
 namespace attn {
 
-constexpr int kBlockM = 128;
-constexpr int kBlockN = 128;
-constexpr int kHeadDim = 128;
-constexpr int kKStages = 2;                          // K ring
-constexpr int kVStages = 2;                          // V ring
-constexpr int kTileBytes = kBlockN * kHeadDim * 2;   // 32 KiB: one Q, K or V tile
-constexpr int kHalfTile = kTileBytes / 2;            // one 64-column SW128 half
-constexpr int kThreads = 320;                        // 10 warps
-constexpr int kSmemQ = 2 * kTileBytes;
-constexpr int kSmemK = kKStages * kTileBytes;
-constexpr int kSmemV = kVStages * kTileBytes;
 constexpr int kSmemBarOff = kSmemQ + kSmemK + kSmemV;
-// P_t is released to the PV UMMAs in kPParts parts of 128/kPParts keys, so
-// the tensor pipe starts on the first keys while the softmax writes the rest.
-#ifndef PSB_P_PARTS
-#define PSB_P_PARTS 2
-#endif
-constexpr int kPParts = PSB_P_PARTS;
-static_assert(kPParts == 1 || kPParts == 2 || kPParts == 4, "P parts: 1, 2 or 4");
-constexpr int kChunksPerPart = 4 / kPParts;  // 32-key chunks per part
 
 enum Bar : int {
   kBarQ = 0,
@@ -90,22 +55,10 @@ enum Bar : int {
   kBarPH = kBarP + 2,            // [2][kPParts-1] leading parts of P_t written
   kBarO = kBarPH + 2 * (kPParts - 1),  // O_0 and O_1 final
   kBarDrain = kBarO + 1,         // every UMMA of the issuer complete
-  kBarTail = kBarDrain + 1,      // sparse form: V rows of a partly used tile loaded
-  kNumBars = kBarTail + 1
+  kNumBars = kBarDrain + 1
 };
 constexpr int kSmemBytes = kSmemBarOff + 256 + 1024;  // barriers + TMEM slot + 1 KiB align slack
 static_assert(kNumBars * 8 + 8 <= 256, "barrier block overflow");
-
-// Device status codes written on a bounded-wait timeout (first error wins).
-enum Err : int {
-  kErrQ = 101,
-  kErrEmpty = 102,
-  kErrFull = 103,
-  kErrP = 104,
-  kErrS = 105,
-  kErrO = 106,
-  kErrDrain = 107,
-};
 
 // Walks the key tiles - the prefix range first, then the segmented range
 // segment by segment (skipping empty segments) - returning each tile's
@@ -169,178 +122,7 @@ __device__ __forceinline__ void q_tile(const AttnArgs& a, int t, bool& prefix, i
   }
 }
 
-// Key tiles of one block list.  A block is cut into pieces of `piece` rows and
-// a 128-row tile holds 128 / piece consecutive pieces of the list.
-struct BlockList {
-  const int* list;
-  int count;   // entries in use
-  int len_k;   // key rows in use
-  int ppb;     // pieces of one block
-
-  BlockList() = default;
-  __device__ __forceinline__ BlockList(const AttnArgs& a, int batch, int head, int pair) {
-    const int qrows = a.q_len ? min(max(a.q_len[batch], 0), a.seg_rows_q) : a.seg_rows_q;
-    len_k = a.k_len ? min(max(a.k_len[batch], 0), a.seg_rows_k) : a.seg_rows_k;
-    const int64_t at = (static_cast<int64_t>(batch) * a.grid_heads + head) * a.list_rows + pair / a.pairs_per_list;
-    list = a.blocks + at * a.list_len;
-    count = a.counts ? min(max(a.counts[at], 0), a.list_len) : a.list_len;
-    if (pair * 2 * kBlockM >= qrows || len_k == 0) count = 0;
-    ppb = a.key_block / a.piece;
-  }
-  __device__ __forceinline__ int tiles(const AttnArgs& a) const {
-    return static_cast<int>((static_cast<int64_t>(count) * a.key_block + kBlockN - 1) / kBlockN);
-  }
-  // First row of piece p of key tile t, and in `valid` its rows in use.  A
-  // piece without any starts behind the tensor: its load fills with zeros.
-  __device__ __forceinline__ int row(const AttnArgs& a, int t, int p, int& valid) const {
-    const int g = t * (kBlockN / a.piece) + p;
-    const int e = g / ppb;
-    valid = 0;
-    if (e >= count) return a.seg_rows_k;
-    const int blk = list[e];
-    if (blk < 0 || blk >= a.key_blocks) return a.seg_rows_k;
-    const int64_t r = static_cast<int64_t>(blk) * a.key_block + (g - e * ppb) * a.piece;
-    if (r >= len_k) return a.seg_rows_k;
-    valid = min(a.piece, len_k - static_cast<int>(r));
-    return static_cast<int>(r);
-  }
-  // Rows in use of the tile's lower and upper 64.
-  __device__ __forceinline__ void halves(const AttnArgs& a, int t, int& lo, int& hi) const {
-    row(a, t, 0, lo);
-    if (a.piece == kBlockN) {
-      hi = max(lo - 64, 0);
-      lo = min(lo, 64);
-    } else {
-      row(a, t, 1, hi);
-    }
-  }
-};
-
-// Bounded wait whose outcome is uniform across the warp (a lane that timed
-// out drags the whole warp out, so .sync.aligned tcgen05 ops stay converged).
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          int* status, int code) {
-  bool ok = mbar_wait(bar, parity, abort_flag, status, code);
-  return __all_sync(0xffffffffu, ok);
-}
-
-// Wait used only while tearing down: ignores the abort flag (copies/UMMAs in
-// flight must land before shared memory / TMEM is released) but is bounded.
-__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, int* status) {
-  const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer() - t0 > kWaitLimitNs) {
-      if (status) atomicCAS(status, 0, kErrDrain);
-      return;
-    }
-  }
-}
-
-// Producer of the sparse form, one warp: the dense producer's stage protocol
-// (see there) with each tile gathered from its pieces.  The rows of a tile are
-// looked up before the wait for its stage, off the critical path.
-__device__ __forceinline__ void sparse_producer(const AttnArgs& args, const BlockList& blocks, const CUtensorMap& tm_q,
-                                                const CUtensorMap& tm_k, const CUtensorMap& tm_v, uint8_t* sQ,
-                                                uint8_t* sK, uint8_t* sV, uint64_t* bars, int tq0, int head,
-                                                int kv_head, int batch, int k_begin, int T, int lane,
-                                                volatile int* abort_flag) {
-  int* status = args.status;
-  auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  const int pieces = kBlockN / args.piece;
-  const int piece_bytes = args.piece * 128;  // of one 64-column half
-  if (lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-    const int tq1 = min(tq0 + 1, args.num_q_tiles - 1);  // no second tile: tile 0 again, never stored
-    mbar_arrive_expect_tx(bar(kBarQ), 2 * kTileBytes);
-    for (int c = 0; c < 2; ++c) {
-      tma_load_5d(smem_u32(sQ + c * kHalfTile), &tm_q, bar(kBarQ), c * 64, head, tq0 * kBlockM, 0, batch);
-      tma_load_5d(smem_u32(sQ + kTileBytes + c * kHalfTile), &tm_q, bar(kBarQ), c * 64, head, tq1 * kBlockM, 0, batch);
-    }
-  }
-  auto load = [&](uint8_t* stage, const CUtensorMap* map, int b, const int (&row)[2]) {
-    if (lane == 0) {
-      mbar_arrive_expect_tx(bar(b), kTileBytes);
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        if (p < pieces)
-          for (int c = 0; c < 2; ++c)
-            tma_load_5d(smem_u32(stage + c * kHalfTile + p * piece_bytes), map, bar(b), c * 64, kv_head, row[p], 0,
-                        batch);
-    }
-  };
-  int issued = 0;
-  uint32_t tail_phase = 0;
-  bool ok = true;
-  for (int i = 0; i < T; ++i) {
-    const int st = i % kKStages;
-    int row[2] = {0, 0}, valid[2] = {0, 0};
-    bool tail = false;  // rows of the tensor that are not in use reach the tile
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      if (p < pieces) row[p] = blocks.row(args, k_begin + i, p, valid[p]);
-      tail |= valid[p] > 0 && valid[p] < args.piece && blocks.len_k < args.seg_rows_k;
-    }
-    if (i >= kKStages) ok = warp_wait(bar(kBarFree + (i & 1)), ((i - 2) >> 1) & 1u, abort_flag, status, kErrEmpty);
-    if (!ok) break;
-    load(sK + st * kTileBytes, &tm_k, kBarKFull + st, row);
-    issued = 2 * i + 1;
-    if (i >= kVStages)
-      ok = warp_wait(bar(kBarFree + ((i - 1) & 1)), ((i - 1) >> 1) & 1u, abort_flag, status, kErrEmpty);
-    if (!ok) break;
-    if (!tail) {
-      load(sV + st * kTileBytes, &tm_v, kBarVFull + st, row);
-    } else {
-      uint8_t* stage = sV + st * kTileBytes;
-      load(stage, &tm_v, kBarTail, row);
-      drain_wait(bar(kBarTail), tail_phase, status);
-      tail_phase ^= 1u;
-      __syncwarp();
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        if (valid[p] == 0) continue;  // no such piece, or filled with zeros by its load
-        const int n = (args.piece - valid[p]) * 8;  // 16-byte chunks of one half
-        for (int c = 0; c < 2; ++c) {
-          uint4* dst = reinterpret_cast<uint4*>(stage + c * kHalfTile + p * piece_bytes + valid[p] * 128);
-          for (int u = lane; u < n; u += 32) dst[u] = make_uint4(0, 0, 0, 0);
-        }
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kBarVFull + st));
-    }
-    issued = 2 * i + 2;
-  }
-  // Every copy issued must land before the CTA may exit.
-  drain_wait(bar(kBarQ), 0, status);
-  const int kv_issued = (issued + 1) / 2;
-  for (int i = max(0, kv_issued - kKStages); i < kv_issued; ++i) {
-    const int st = i % kKStages;
-    const uint32_t ph = (i / kKStages) & 1u;
-    drain_wait(bar(kBarKFull + st), ph, status);
-    if (2 * i + 2 <= issued) drain_wait(bar(kBarVFull + st), ph, status);
-  }
-}
-
 template <bool kFp16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return kFp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
-}
-
-__device__ __forceinline__ float row_max128(const float (&s)[128]) {
-  float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < 128; j += 8) {
-    mx0 = fmax3(mx0, s[j], s[j + 1]);
-    mx1 = fmax3(mx1, s[j + 2], s[j + 3]);
-    mx2 = fmax3(mx2, s[j + 4], s[j + 5]);
-    mx3 = fmax3(mx3, s[j + 6], s[j + 7]);
-  }
-  return fmaxf(fmax3(mx0, mx1, mx2), mx3);
-}
-
-template <bool kFp16, bool kSparse>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_qp,
@@ -372,11 +154,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kv_head = head / args.group;
   const int tq0 = pair * 2;
   const int tq1 = tq0 + 1;
-  [[maybe_unused]] BlockList blocks;
-  if constexpr (kSparse) blocks = BlockList(args, batch, head, pair);
-  const int tiles = kSparse ? blocks.tiles(args) : args.num_kv_tiles;
-  const int k_begin = part * tiles / nparts;
-  const int T = (part + 1) * tiles / nparts - k_begin;
+  const int k_begin = part * args.num_kv_tiles / nparts;
+  const int T = (part + 1) * args.num_kv_tiles / nparts - k_begin;
   int* status = args.status;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
@@ -393,7 +172,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(bar(kBarO), 1);
     mbar_init(bar(kBarDrain), 1);
-    if constexpr (kSparse) mbar_init(bar(kBarTail), 1);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -405,12 +183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (kSparse && T == 0) {
-    // No key: nothing to load or multiply, the epilogue writes zeros.
-  } else if (kSparse && warp == 8) {
-    sparse_producer(args, blocks, tm_q, tm_k, tm_v, sQ, sK, sV, bars, tq0, head, kv_head, batch, k_begin, T, lane,
-                    abort_flag);
-  } else if (warp == 8) {
+  if (warp == 8) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&tm_q);
@@ -481,33 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 9) {
     // ------------------------------------------------------------ UMMA issuer (one lane)
     if (lane == 0) {
-      const uint32_t id_qk = idesc_f16(kBlockM, kBlockN, !kFp16, false, false);
-      const uint32_t id_pv = idesc_f16(kBlockM, kHeadDim, !kFp16, false, true);
-      // Descriptor bases; per-UMMA offsets are added to the start-address field
-      // (all shared addresses stay below 256 KiB, so the 14-bit field never carries).
-      const uint64_t dq0 = sdesc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t dq1 = sdesc_sw128(smem_u32(sQ + kTileBytes), 16, 1024);
-      const uint64_t dk = sdesc_sw128(smem_u32(sK), 16, 1024);
-      const uint64_t dv = sdesc_sw128(smem_u32(sV), kHalfTile, 1024);
-      auto mma_s = [&](int t, int st) {
-        const uint64_t dq = t ? dq1 : dq0;
-        const uint64_t dks = dk + static_cast<uint64_t>(st * (kTileBytes >> 4));
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const uint32_t off = ((s >> 2) * kHalfTile + (s & 3) * 32) >> 4;
-          umma_ss(tmem + 128 * t, dq + off, dks + off, id_qk, s > 0);
-        }
-      };
-      // O_t (+)= P_t V for the keys of part q (8/kPParts UMMAs of K=16).
-      auto mma_pv = [&](int t, int st, int q, bool accumulate) {
-        const uint64_t dvs = dv + static_cast<uint64_t>(st * (kTileBytes >> 4));
-#pragma unroll
-        for (int k = 0; k < 8 / kPParts; ++k) {
-          const int s = (8 / kPParts) * q + k;
-          umma_ts(tmem + 256 + 128 * t, tmem + 128 * t + s * 8, dvs + ((s * 2048) >> 4), id_pv,
-                  (accumulate || s > 0) ? 1u : 0u);
-        }
-      };
+      const TileMma mma = TileMma::make<kFp16>(tmem, sQ, sK, sV);
       // P_t arrives in parts; each part's UMMAs are issued as soon as it is written.
       auto pv_both = [&](int t, int st, uint32_t parity, bool accumulate) -> bool {
 #pragma unroll
@@ -515,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int b = q + 1 < kPParts ? kBarPH + t * (kPParts - 1) + q : kBarP + t;
           if (!mbar_wait(bar(b), parity, abort_flag, status, kErrP)) return false;
           tc_fence_after();
-          mma_pv(t, st, q, accumulate);
+          mma.pv(t, st, q, accumulate);
         }
         return true;
       };
@@ -527,13 +274,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = mbar_wait(bar(kBarKFull + st), ph, abort_flag, status, kErrFull);
         if (!ok) break;
         tc_fence_after();
-        mma_s(0, st);
+        mma.s(0, st);
         umma_commit(bar(kBarS + 0));
         if (i > 0) {
           ok = pv_both(1, (i - 1) % kVStages, (i - 1) & 1u, i > 1);
           if (!ok) break;
         }
-        mma_s(1, st);
+        mma.s(1, st);
         umma_commit(bar(kBarS + 1));
         ok = mbar_wait(bar(kBarVFull + st), ph, abort_flag, status, kErrFull);
         if (ok) ok = pv_both(0, st, i & 1u, i > 0);
@@ -547,8 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(bar(kBarDrain));
       drain_wait(bar(kBarDrain), 0, status);
     }
-  }
-  if (warp < 8) {
+  } else if (warp < 8) {
     // ------------------------------------------------------------ softmax
     const int t = warp >> 2;
     const int quarter = warp & 3;
@@ -560,23 +306,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     KeyCursor cur;
-    if constexpr (!kSparse) cur.skip(args, k_begin);
-    [[maybe_unused]] uint32_t whole = 0;  // sparse: which of the next 32 key tiles are in use throughout
+    cur.skip(args, k_begin);
     for (int i = 0; i < T; ++i) {
-      int valid = kBlockN;
-      [[maybe_unused]] bool part_used = false;
-      if constexpr (kSparse) {
-        if ((i & 31) == 0) {
-          int lo = 64, hi = 64;
-          if (i + lane < T) blocks.halves(args, k_begin + i + lane, lo, hi);
-          whole = __ballot_sync(0xffffffffu, lo + hi == kBlockN);
-        }
-        part_used = !((whole >> (i & 31)) & 1u);
-      } else {
-        bool pre_unused;
-        int seg_unused, row_unused;
-        cur.next(args, pre_unused, seg_unused, row_unused, valid);
-      }
+      bool pre_unused;
+      int seg_unused, row_unused, valid;
+      cur.next(args, pre_unused, seg_unused, row_unused, valid);
       ok = warp_wait(bar(kBarS + t), i & 1u, abort_flag, status, kErrS);
       if (!ok) break;
       if (t == 1 && threadIdx.x == 128) mbar_arrive(bar(kBarFree + (i & 1)));
@@ -590,93 +324,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       float s[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) s[j] = __uint_as_float(sr[j]);
-      if constexpr (kSparse) {
-        if (part_used) {
-          int lo, hi;
-          blocks.halves(args, k_begin + i, lo, hi);
-#pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if ((j < 64 ? j : j - 64) >= (j < 64 ? lo : hi)) s[j] = -INFINITY;
-        }
-      }
       const bool masked = valid < kBlockN;
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 128; ++j)
           if (j >= valid) s[j] = -INFINITY;
       }
-      float alpha = 1.f, sum;
-      bool rescale = false;
-      // Row max first (lazy running max: raised warp-uniformly only when it
-      // grew by > 8), then the exponentials.
-      const float m_tile = row_max128(s) * scale_log2;
-      if (i == 0) {
-        // A listed tile without a key in use leaves every score at -inf: a
-        // finite maximum makes its exponentials 0 instead of NaN.
-        m = kSparse ? fmaxf(m_tile, -1e30f) : m_tile;
-      } else if (__any_sync(0xffffffffu, m_tile - m > 8.f)) {
-        const float m_new = fmaxf(m, m_tile);
-        alpha = ex2_approx(m - m_new);
-        m = m_new;
-        rescale = true;
-      }
-      {
-        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float p0 = ex2_approx(fmaf(s[32 * c + 2 * j], scale_log2, -m));
-            const float p1 = ex2_approx(fmaf(s[32 * c + 2 * j + 1], scale_log2, -m));
-            sum0 += p0;
-            sum1 += p1;
-            pk[j] = pack2<kFp16>(p0, p1);
-          }
-          tmem_st16(s_addr + 16 * c, pk);
-          if (c == (kPParts > 1 ? kChunksPerPart - 1 : 3)) {
-            // The rare O rescale goes here, before the first PV part of this
-            // tile is released (O_t's last update completed before S_t was
-            // signalled); the row's first chunks are dead by now.
-            if (rescale) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t o[32];
-                tmem_ld32(o_addr + 32 * q, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-                tmem_st32(o_addr + 32 * q, o);
-              }
-            }
-          }
-          if ((c + 1) % kChunksPerPart == 0 && c < 3) {  // part (c+1)/kChunksPerPart - 1 written
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(bar(kBarPH + t * (kPParts - 1) + (c + 1) / kChunksPerPart - 1));
-          }
-        }
-        sum = sum0 + sum1;
-      }
-      l = fmaf(l, alpha, sum);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(bar(kBarP + t));
+      softmax_row<kFp16, false>(s, i == 0, scale_log2, s_addr, o_addr, bar(kBarPH + t * (kPParts - 1)), bar(kBarP + t),
+                                m, l);
     }
-    if (ok && (!kSparse || T > 0)) ok = warp_wait(bar(kBarO), 0, abort_flag, status, kErrO);
+    if (ok) ok = warp_wait(bar(kBarO), 0, abort_flag, status, kErrO);
     tc_fence_after();
     const int tq = t ? tq1 : tq0;
     bool pre = false;
     int seg = 0, row0 = 0, valid = 0;
     if (tq < args.num_q_tiles) q_tile(args, tq, pre, seg, row0, valid);
     const float inv_l = l > 0.f ? 1.f / l : 0.f;
-    // Sparse: rows behind the sequence's queries and rows that saw no key are
-    // zeros (the accumulator of a CTA without tiles was never written).
-    bool live = true;
-    if constexpr (kSparse) {
-      const int qrows = args.q_len ? args.q_len[batch] : args.seg_rows_q;
-      live = T > 0 && row0 + row < qrows;
-    }
     void* const obase = pre ? args.pre_out : args.seg_out[seg];
     const int64_t* ost = pre ? args.pre_o_stride : args.o_stride;
     const int64_t otile = batch * ost[0] + static_cast<int64_t>(row0) * ost[2] + head * ost[3];
@@ -690,20 +353,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
-          if constexpr (kSparse) {
-            if (!live)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = 0;
-          }
           float4* dst = reinterpret_cast<float4*>(wrow + 32 * c);
-          if (!kSparse || row < valid) {  // the merge reads the rows of the tensor only
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-              dst[u] = make_float4(__uint_as_float(o[4 * u + 0]) * inv_l, __uint_as_float(o[4 * u + 1]) * inv_l,
-                                   __uint_as_float(o[4 * u + 2]) * inv_l, __uint_as_float(o[4 * u + 3]) * inv_l);
-          }
+          for (int u = 0; u < 8; ++u)
+            dst[u] = make_float4(__uint_as_float(o[4 * u + 0]) * inv_l, __uint_as_float(o[4 * u + 1]) * inv_l,
+                                 __uint_as_float(o[4 * u + 2]) * inv_l, __uint_as_float(o[4 * u + 3]) * inv_l);
         }
-        args.ws_lse[(slot * 2 + t) * kBlockM + row] = live && l > 0.f ? m + __log2f(l) : -INFINITY;
+        args.ws_lse[(slot * 2 + t) * kBlockM + row] = l > 0.f ? m + __log2f(l) : -INFINITY;
       }
     } else if (args.out_fp32) {
       // tcgen05.ld is warp-collective: every lane loads, only valid rows store.
@@ -714,11 +370,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
-          if constexpr (kSparse) {
-            if (!live)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = 0;
-          }
           if (row < valid) {
             float4* dst = reinterpret_cast<float4*>(orow + 32 * c);
 #pragma unroll
@@ -742,11 +393,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t o[32];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_wait_ld();
-          if constexpr (kSparse) {
-            if (!live)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = 0;
-          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint4 v;
@@ -786,12 +432,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Merges the split parts of the last wave's units: for each valid query row,
 // out = sum_p w_p o_p / sum_p w_p with w_p = 2^(lse_p - max lse), the
-// log-sum-exp combination of partial softmax results.  One CTA per (unit,
-// query tile); 16 threads per row, 8 columns each.
+// log-sum-exp combination of partial softmax results.  16 threads per row, 8
+// columns each; a CTA takes 16 rows, so the few split units spread over the SMs.
 template <bool kFp16>
 __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnArgs args) {
-  const int u = blockIdx.x >> 1;
-  const int t = blockIdx.x & 1;
+  wait_for_previous();
+  const int u = blockIdx.x >> 4;
+  const int t = (blockIdx.x >> 3) & 1;
   const int unit = args.full_units + u;
   const int pair = unit % args.npairs;
   const int head = (unit / args.npairs) % args.grid_heads;
@@ -805,10 +452,9 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnArgs args) 
   const int64_t* ost = pre ? args.pre_o_stride : args.o_stride;
   const int64_t otile = batch * ost[0] + static_cast<int64_t>(row0) * ost[2] + head * ost[3];
   const int S = args.split;
-  for (int idx = threadIdx.x; idx < kBlockM * 16; idx += 256) {
-    const int r = idx >> 4;
-    const int c = (idx & 15) * 8;
-    if (r >= valid) continue;
+  const int r = (blockIdx.x & 7) * 16 + (threadIdx.x >> 4);
+  const int c = (threadIdx.x & 15) * 8;
+  if (r < valid) {
     float mx = -INFINITY;
     for (int p = 0; p < S; ++p) mx = fmaxf(mx, args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r]);
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -851,55 +497,51 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnArgs args) 
 namespace {
 // Raises the kernel's dynamic shared memory limit once per device (outside
 // any stream capture that may follow: the first launch on a device does it).
-template <bool kFp16, bool kSparse>
+template <bool kFp16>
 int prepare_kernel() {
   static bool done[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (done[dev]) return 0;
-  const cudaError_t err = cudaFuncSetAttribute(attn::attn_fwd_kernel<kFp16, kSparse>,
+  const cudaError_t err = cudaFuncSetAttribute(attn::attn_fwd_kernel<kFp16>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, attn::kSmemBytes);
   if (err != cudaSuccess) return set_cuda_error("attention: cudaFuncSetAttribute", err);
   done[dev] = true;
   return 0;
 }
+}  // namespace
 
-template <bool kFp16, bool kSparse>
-int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tqp,
-           const CUtensorMap& tkp, const CUtensorMap& tvp, const AttnArgs& args, int64_t total_units,
-           cudaStream_t stream) {
+int launch_combine(const AttnArgs& args, int64_t split_units, bool fp16, bool overlap, cudaStream_t stream) {
+  const cudaError_t err =
+      launch_after(fp16 ? attn::attn_combine_kernel<true> : attn::attn_combine_kernel<false>,
+                   dim3(static_cast<unsigned>(split_units * 16)), dim3(256), 0, stream, overlap, args);
+  if (err != cudaSuccess) return set_cuda_error("attention combine launch", err);
+  count_launch();
+  return 0;
+}
+
+int launch_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+                     const CUtensorMap& tqp, const CUtensorMap& tkp, const CUtensorMap& tvp,
+                     const AttnArgs& args, int64_t total_units, bool fp16, cudaStream_t stream) {
   using namespace attn;
   const int64_t split_units = args.split > 1 ? total_units - args.full_units : 0;
   const int64_t ctas = split_units > 0 ? args.full_units + split_units * args.split : total_units;
   if (ctas <= 0) return 0;
   if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "attention grid above 2^31 CTAs");
-  if (int rc = prepare_kernel<kFp16, kSparse>()) return rc;
-  attn_fwd_kernel<kFp16, kSparse>
-      <<<static_cast<unsigned>(ctas), kThreads, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
+  const dim3 grid(static_cast<unsigned>(ctas));
+  const dim3 block(kThreads);
+  if (fp16) {
+    if (int rc = prepare_kernel<true>()) return rc;
+    attn_fwd_kernel<true><<<grid, block, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
+  } else {
+    if (int rc = prepare_kernel<false>()) return rc;
+    attn_fwd_kernel<false><<<grid, block, kSmemBytes, stream>>>(tq, tk, tv, tqp, tkp, tvp, args);
+  }
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return set_cuda_error("attention launch", err);
   count_launch();
-  if (split_units > 0) {
-    attn_combine_kernel<kFp16><<<static_cast<unsigned>(split_units * 2), 256, 0, stream>>>(args);
-    err = cudaGetLastError();
-    if (err != cudaSuccess) return set_cuda_error("attention combine launch", err);
-    count_launch();
-  }
+  if (split_units > 0) return launch_combine(args, split_units, fp16, false, stream);
   return 0;
-}
-}  // namespace
-
-int launch_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
-                     const CUtensorMap& tqp, const CUtensorMap& tkp, const CUtensorMap& tvp,
-                     const AttnArgs& args, int64_t total_units, bool fp16, cudaStream_t stream) {
-  return fp16 ? launch<true, false>(tq, tk, tv, tqp, tkp, tvp, args, total_units, stream)
-              : launch<false, false>(tq, tk, tv, tqp, tkp, tvp, args, total_units, stream);
-}
-
-int launch_sparse_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args,
-                            int64_t total_units, bool fp16, cudaStream_t stream) {
-  return fp16 ? launch<true, true>(tq, tk, tv, tq, tk, tv, args, total_units, stream)
-              : launch<false, true>(tq, tk, tv, tq, tk, tv, args, total_units, stream);
 }
 
 }  // namespace psb

@@ -293,6 +293,34 @@ int check_blocks(int batch, int heads_q, int heads_kv, int head_dim, int query_b
   return PS_B200_OK;
 }
 
+// Where one block-sparse call keeps what its three steps hand on, each on a 256-byte boundary.
+struct SparseScratch {
+  int64_t q_blocks, k_blocks;
+  size_t q_means, k_means, blocks, counts, workspace, workspace_bytes, total;
+};
+
+SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t len_q, int64_t len_k,
+                             int64_t keep, int64_t query_block, int64_t key_block, bool key_means) {
+  SparseScratch s{};
+  s.q_blocks = (len_q + query_block - 1) / query_block;
+  s.k_blocks = (len_k + key_block - 1) / key_block;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t lists = size_t(batch * heads_q * s.q_blocks);
+  s.q_means = take(lists * 128 * sizeof(float));
+  s.k_means = take(key_means ? 0 : size_t(batch * heads_kv * s.k_blocks) * 128 * sizeof(float));
+  s.blocks = take(lists * keep * sizeof(int));
+  s.counts = take(lists * sizeof(int));
+  s.workspace_bytes = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count()).workspace_bytes();
+  s.workspace = take(s.workspace_bytes);
+  s.total = at;
+  return s;
+}
+
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 }  // namespace
@@ -1002,25 +1030,25 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
   return launch_block_means(a, dtype == PS_B200_FP16, static_cast<cudaStream_t>(stream));
 }
 
-int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
-                         int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
-                         const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
-                         int key_block, int* blocks, int* counts, void* stream) {
+// `from`: what a combined call adds (queries whose means the kernel takes itself; a launch that follows the means).
+static int block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
+                        int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
+                        const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
+                        int key_block, int* blocks, int* counts, void* stream, SelectArgs from = {}) {
   if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
   if (q_blocks < 0 || k_blocks < 0 || keep < 1) return set_error(PS_B200_ERR_INVALID, "keep must be positive, block counts not negative");
   if (keep > k_blocks && k_blocks > 0) return set_error(PS_B200_ERR_INVALID, "keep %d above the %d key blocks", keep, k_blocks);
   if (batch == 0 || heads_q == 0 || q_blocks == 0) return PS_B200_OK;
   if (k_blocks == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
-  if (size_t(k_blocks) > kSelectSmemLimit / 8 - 128)
-    return set_error(PS_B200_ERR_UNSUPPORTED, "%d key blocks: at most %d, take larger blocks", k_blocks,
-                     int(kSelectSmemLimit / 8 - 128));
-  if (!q_means || !k_means || !aligned16(q_means) || !aligned16(k_means))
+  if (k_blocks > kSelectMaxBlocks)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "%d key blocks: at most %d, take larger blocks", k_blocks, kSelectMaxBlocks);
+  if ((!q_means && !from.q) || !k_means || !aligned16(q_means) || !aligned16(k_means))
     return set_error(PS_B200_ERR_INVALID, "means null or not 16-byte aligned");
   if (!blocks || !counts || !aligned4(blocks) || !aligned4(counts) || !aligned4(q_len) || !aligned4(k_len))
     return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
   if (allowed && !allowed_strides) return set_error(PS_B200_ERR_INVALID, "allowed needs strides");
   if (int rc = check_device()) return rc;
-  SelectArgs a{};
+  SelectArgs a = from;
   a.q_means = q_means;
   a.k_means = k_means;
   a.batch = batch;
@@ -1040,17 +1068,25 @@ int ps_b200_block_select(const float* q_means, const float* k_means, int batch, 
   return launch_block_select(a, static_cast<cudaStream_t>(stream));
 }
 
+int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
+                         int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
+                         const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
+                         int key_block, int* blocks, int* counts, void* stream) {
+  return block_select(q_means, k_means, batch, heads_q, heads_kv, head_dim, q_blocks, k_blocks, keep, allowed,
+                      allowed_strides, q_len, query_block, k_len, key_block, blocks, counts, stream);
+}
+
 size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block) {
   if (batch <= 0 || heads_q <= 0 || len_q <= 0 || list_len <= 0 || key_block <= 0) return 0;
   return sparse_plan(batch, heads_q, len_q, list_len, key_block, sm_count()).workspace_bytes();
 }
 
-int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
-                            const void* v, const int64_t v_strides[3], void* out, const int64_t out_strides[3],
-                            int dtype, int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k,
-                            const int* blocks, const int* counts, int list_len, int query_block, int key_block,
-                            const int* q_len, const int* k_len, float softmax_scale, void* workspace,
-                            size_t workspace_bytes, int* status, void* stream) {
+static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                       const void* v, const int64_t v_strides[3], void* out, const int64_t out_strides[3], int dtype,
+                       int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k, const int* blocks,
+                       const int* counts, int list_len, int query_block, int key_block, const int* q_len,
+                       const int* k_len, float softmax_scale, void* workspace, size_t workspace_bytes, int* status,
+                       void* stream, bool after_select) {
   if (!q_strides || !k_strides || !v_strides || !out_strides) return set_error(PS_B200_ERR_INVALID, "null strides");
   if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
   if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
@@ -1117,71 +1153,146 @@ int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const voi
     a.ws_o = static_cast<float*>(workspace);
     a.ws_lse = a.ws_o + plan.rem * plan.split * 2 * 128 * 128;
   }
-  return launch_sparse_attention(tq, tk, tv, a, plan.units, fp16, static_cast<cudaStream_t>(stream));
+  return launch_sparse_attention(tq, tk, tv, a, plan.units, fp16, after_select, static_cast<cudaStream_t>(stream));
 }
 
-static int cache_common(bool write, void* const pages[2], float* const scales[2], void* const rows[2],
-                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
-                        int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
-                        int table_len, const int* first, const int* count, void* stream) {
-  if (!pages || !scales || !rows || !strides) return set_error(PS_B200_ERR_INVALID, "null tensor table");
-  if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "the cache takes and gives bf16 and fp16 rows only");
-  if (cache_dtype != PS_B200_E4M3 && cache_dtype != PS_B200_INT8)
+int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                            const void* v, const int64_t v_strides[3], void* out, const int64_t out_strides[3],
+                            int dtype, int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k,
+                            const int* blocks, const int* counts, int list_len, int query_block, int key_block,
+                            const int* q_len, const int* k_len, float softmax_scale, void* workspace,
+                            size_t workspace_bytes, int* status, void* stream) {
+  return sparse_attn(q, q_strides, k, k_strides, v, v_strides, out, out_strides, dtype, batch, heads_q, heads_kv,
+                     head_dim, len_q, len_k, blocks, counts, list_len, query_block, key_block, q_len, k_len,
+                     softmax_scale, workspace, workspace_bytes, status, stream, false);
+}
+
+size_t ps_b200_sparse_scratch_bytes(int batch, int heads_q, int heads_kv, int len_q, int len_k, int keep,
+                                    int query_block, int key_block, int with_key_means) {
+  if (batch <= 0 || heads_q <= 0 || heads_kv <= 0 || len_q <= 0 || len_k <= 0 || keep <= 0 || query_block <= 0 ||
+      key_block <= 0)
+    return 0;
+  return sparse_scratch(batch, heads_q, heads_kv, len_q, len_k, keep, query_block, key_block, with_key_means != 0).total;
+}
+
+int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
+  if (!c) return set_error(PS_B200_ERR_INVALID, "null call");
+  const int64_t sizes[] = {c->dtype, c->batch, c->heads_q, c->heads_kv, c->head_dim, c->len_q, c->len_k, c->keep,
+                           c->query_block, c->key_block};
+  for (int64_t n : sizes)
+    if (n < 0 || n > (1 << 30)) return set_error(PS_B200_ERR_INVALID, "size %lld outside [0, 2^30]", (long long)n);
+  const int batch = int(c->batch), hq = int(c->heads_q), hk = int(c->heads_kv), dim = int(c->head_dim);
+  const int lq = int(c->len_q), lk = int(c->len_k), qb = int(c->query_block), kb = int(c->key_block);
+  const int keep = int(c->keep), dtype = int(c->dtype);
+  if (int rc = check_blocks(batch, hq, hk, dim, qb, kb)) return rc;
+  if (batch == 0 || hq == 0 || lq == 0) return PS_B200_OK;
+  if (lk == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
+  const SparseScratch s = sparse_scratch(batch, hq, hk, lq, lk, keep, qb, kb, c->key_means != nullptr);
+  if (keep < 1 || keep > s.k_blocks)
+    return set_error(PS_B200_ERR_INVALID, "keep %d outside [1, %lld key blocks]", keep, (long long)s.k_blocks);
+  if (!c->scratch || (reinterpret_cast<uintptr_t>(c->scratch) & 255u) || c->scratch_bytes < int64_t(s.total))
+    return set_error(PS_B200_ERR_INVALID, "this call needs a 256-byte aligned scratch of %zu bytes", s.total);
+  char* base = static_cast<char*>(c->scratch);
+  float* q_means = reinterpret_cast<float*>(base + s.q_means);
+  float* k_means = reinterpret_cast<float*>(base + s.k_means);
+  int* blocks = reinterpret_cast<int*>(base + s.blocks);
+  int* counts = reinterpret_cast<int*>(base + s.counts);
+  // The means of a few query rows are taken by the selection itself (one launch
+  // less: 2.4 us on the GPU and 3 us on the host for one row; at 32 rows their
+  // reading, one row after the other, takes as long as the launch saved).
+  SelectArgs from{};
+  if (lq <= 32) {
+    if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
+    if (!c->q || !aligned16(c->q)) return set_error(PS_B200_ERR_INVALID, "queries null or not 16-byte aligned");
+    from.q = c->q;
+    for (int i = 0; i < 3; ++i) {
+      from.q_st[i] = c->q_strides[i];
+      if (from.q_st[i] < 0 || from.q_st[i] % 8 != 0)
+        return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
+    }
+    from.len_q = lq;
+    from.fp16 = dtype == PS_B200_FP16;
+  }
+  const void* x[2];
+  int64_t st[6];
+  int len[2], heads[2], block[2], n = 0;
+  const int* lens[2];
+  float* means[2];
+  auto mean_of = [&](const void* t, const int64_t* strides, int l, int h, int b, const int* used, float* m) {
+    x[n] = t;
+    for (int i = 0; i < 3; ++i) st[3 * n + i] = strides[i];
+    len[n] = l;
+    heads[n] = h;
+    block[n] = b;
+    lens[n] = used;
+    means[n++] = m;
+  };
+  if (!from.q) mean_of(c->q, c->q_strides, lq, hq, qb, c->q_len, q_means);
+  if (!c->key_means) mean_of(c->k, c->k_strides, lk, hk, kb, c->k_len, k_means);
+  if (n)
+    if (int rc = ps_b200_block_means(n, x, st, dtype, batch, len, heads, dim, block, lens, means, stream)) return rc;
+  from.after_means = n > 0;
+  if (int rc = block_select(q_means, c->key_means ? c->key_means : k_means, batch, hq, hk, dim, int(s.q_blocks),
+                            int(s.k_blocks), keep, c->allowed, c->allowed_strides, c->q_len, qb, c->k_len, kb, blocks,
+                            counts, stream, from))
+    return rc;
+  return sparse_attn(c->q, c->q_strides, c->k, c->k_strides, c->v, c->v_strides, c->out, c->out_strides, dtype, batch,
+                     hq, hk, dim, lq, lk, blocks, counts, keep, qb, kb, c->q_len, c->k_len,
+                     static_cast<float>(c->softmax_scale), s.workspace_bytes ? base + s.workspace : nullptr,
+                     s.workspace_bytes, c->status, stream, true);
+}
+
+static int cache_common(bool write, const ps_b200_cache_call* c, void* stream) {
+  if (!c) return set_error(PS_B200_ERR_INVALID, "null call");
+  if (!is16bit(int(c->dtype)) || c->dtype != int(c->dtype))
+    return set_error(PS_B200_ERR_UNSUPPORTED, "the cache takes and gives bf16 and fp16 rows only");
+  if (c->cache_dtype != PS_B200_E4M3 && c->cache_dtype != PS_B200_INT8)
     return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds e4m3 or int8 codes only");
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
-    return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds heads of 64, 128 or 256 (got %d)", head_dim);
-  if (batch < 0 || batch > 65535 || heads < 0 || heads > 4096 || n < 0 || num_pages < 0 || page_rows < 1 ||
-      table_len < 0 || table_stride < 0)
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds heads of 64, 128 or 256 (got %lld)",
+                     (long long)c->head_dim);
+  const int64_t most = (int64_t(1) << 31) - 64;
+  if (c->batch < 0 || c->batch > 65535 || c->heads < 0 || c->heads > 4096 || c->n < 0 || c->n > most ||
+      c->num_pages < 0 || c->num_pages > most || c->page_rows < 1 || c->page_rows > most || c->table_len < 0 ||
+      c->table_len > most || c->table_stride < 0)
     return set_error(PS_B200_ERR_INVALID, "size out of range (batch <= 65535, heads <= 4096)");
-  if (batch == 0 || n == 0 || heads == 0) return PS_B200_OK;
-  if (!table || !aligned4(table) || !aligned4(first) || !aligned4(count))
+  if (c->batch == 0 || c->n == 0 || c->heads == 0) return PS_B200_OK;
+  if (!c->table || !aligned4(c->table) || !aligned4(c->first) || !aligned4(c->count))
     return set_error(PS_B200_ERR_INVALID, "page table null or a table not 4-byte aligned");
-  if (!write && !count) return set_error(PS_B200_ERR_INVALID, "a read needs the lengths");
+  if (!write && !c->count) return set_error(PS_B200_ERR_INVALID, "a read needs the lengths");
   CacheArgs a{};
   for (int t = 0; t < 2; ++t) {
-    if (!pages[t] || !scales[t] || !rows[t] || !aligned16(pages[t]) || !aligned4(scales[t]) || !aligned16(rows[t]))
+    if (!c->pages[t] || !c->scales[t] || !c->rows[t] || !aligned16(c->pages[t]) || !aligned4(c->scales[t]) ||
+        !aligned16(c->rows[t]))
       return set_error(PS_B200_ERR_INVALID, "pages, scales or rows null or not aligned (16, 4 and 16 bytes)");
-    a.pages[t] = pages[t];
-    a.scales[t] = scales[t];
-    a.rows[t] = rows[t];
+    a.pages[t] = c->pages[t];
+    a.scales[t] = c->scales[t];
+    a.rows[t] = c->rows[t];
     for (int i = 0; i < 3; ++i) {
-      a.st[t][i] = strides[3 * t + i];
+      a.st[t][i] = c->strides[3 * t + i];
       if (a.st[t][i] < 0 || a.st[t][i] % 8 != 0)
         return set_error(PS_B200_ERR_INVALID, "row strides must be non-negative multiples of 8 elements");
     }
   }
   if (int rc = check_device()) return rc;
-  a.batch = batch;
-  a.n = n;
-  a.heads = heads;
-  a.head_dim = head_dim;
-  a.num_pages = num_pages;
-  a.page_rows = page_rows;
-  a.table = table;
-  a.table_st = table_stride;
-  a.table_len = table_len;
-  a.first = first;
-  a.count = count;
-  const bool fp16 = dtype == PS_B200_FP16, int8 = cache_dtype == PS_B200_INT8;
+  a.batch = int(c->batch);
+  a.n = int(c->n);
+  a.heads = int(c->heads);
+  a.head_dim = int(c->head_dim);
+  a.num_pages = int(c->num_pages);
+  a.page_rows = int(c->page_rows);
+  a.table = c->table;
+  a.table_st = c->table_stride;
+  a.table_len = int(c->table_len);
+  a.first = c->first;
+  a.count = c->count;
+  const bool fp16 = c->dtype == PS_B200_FP16, int8 = c->cache_dtype == PS_B200_INT8;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return write ? launch_cache_write(a, fp16, int8, s) : launch_cache_read(a, fp16, int8, s);
 }
 
-int ps_b200_cache_write(void* const pages[2], float* const scales[2], const void* const rows[2],
-                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads, int head_dim,
-                        int num_pages, int page_rows, const int* table, int64_t table_stride, int table_len,
-                        const int* first, const int* count, void* stream) {
-  return cache_common(true, pages, scales, const_cast<void* const*>(rows), strides, dtype, cache_dtype, batch, n, heads,
-                      head_dim, num_pages, page_rows, table, table_stride, table_len, first, count, stream);
-}
+int ps_b200_cache_write(const ps_b200_cache_call* call, void* stream) { return cache_common(true, call, stream); }
 
-int ps_b200_cache_read(const void* const pages[2], const float* const scales[2], void* const rows[2],
-                       const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads, int head_dim,
-                       int num_pages, int page_rows, const int* table, int64_t table_stride, int table_len,
-                       const int* first, const int* count, void* stream) {
-  return cache_common(false, const_cast<void* const*>(pages), const_cast<float* const*>(scales), rows, strides, dtype,
-                      cache_dtype, batch, n, heads, head_dim, num_pages, page_rows, table, table_stride, table_len,
-                      first, count, stream);
-}
+int ps_b200_cache_read(const ps_b200_cache_call* call, void* stream) { return cache_common(false, call, stream); }
 
 }  // extern "C"

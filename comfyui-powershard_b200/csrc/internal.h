@@ -44,7 +44,7 @@ struct AttnArgs {
   int split;             // 1: no split
   float* ws_o;           // [slot][2][128][128] fp32: O / l of one part, slot = (unit - full_units) * split + part
   float* ws_lse;         // [slot][2][128] fp32: m + log2(l) of one part (log2 units of the scaled scores)
-  // Block lists (the kernel's sparse form only).  Query block i of head h of batch row b attends the key
+  // Block lists (sparse_attn.cu only).  Query block i of head h of batch row b attends the key
   // blocks blocks[((b * grid_heads + h) * list_rows + i) * list_len + ...]; one segment of queries and keys.
   const int* blocks;
   const int* counts;     // [batch][heads][list_rows] entries in use of each list, or null: list_len
@@ -68,9 +68,11 @@ constexpr int64_t kAttnWorkspaceBytes = int64_t(160) * 2 * 128 * (128 + 1) * 4;
 int launch_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
                      const CUtensorMap& tqp, const CUtensorMap& tkp, const CUtensorMap& tvp,
                      const AttnArgs& args, int64_t total_units, bool fp16, cudaStream_t stream);
-// The same over the block lists of `args` (attn_fwd_kernel's sparse form).
+// Merges the parts of `split_units` units (overlap: right after the kernel that writes them).
+int launch_combine(const AttnArgs& args, int64_t split_units, bool fp16, bool overlap, cudaStream_t stream);
+// The same over the block lists of `args` (sparse_attn.cu).
 int launch_sparse_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args,
-                            int64_t total_units, bool fp16, cudaStream_t stream);
+                            int64_t total_units, bool fp16, bool after_select, cudaStream_t stream);
 
 // Process-wide count of kernels this library launched (ps_b200_kernel_launches).
 void count_launch();
@@ -182,6 +184,7 @@ struct MeansArgs {
 int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream);
 
 constexpr size_t kSelectSmemLimit = 200 * 1024;
+constexpr int kSelectMaxBlocks = 16384;  // 12 bytes of shared memory each
 struct SelectArgs {
   const float* q_means;    // [batch][q_blocks][kv_heads * group][128]
   const float* k_means;    // [batch][k_blocks][kv_heads][128]
@@ -193,8 +196,16 @@ struct SelectArgs {
   int64_t allowed_st[4];
   int* blocks;             // [batch][heads][q_blocks][keep]
   int* counts;             // [batch][heads][q_blocks]
+  int rows_per_cta;        // set by the launch
+  // Queries [batch][len_q][kv_heads * group][128] (16-bit) whose means the kernel takes itself, in the
+  // place of q_means, or null.
+  const void* q;
+  int64_t q_st[3];         // batch, row, head strides in elements
+  int len_q;
+  int fp16;
+  bool after_means;        // launched right after the kernel that writes the means
 };
-int launch_block_select(const SelectArgs& a, cudaStream_t stream);
+int launch_block_select(SelectArgs a, cudaStream_t stream);
 
 // 8-bit key/value cache (cache.cu).
 struct CacheArgs {

@@ -373,6 +373,56 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster) {
                : "memory");
 }
 
+// ------------------------------------------------ work taken from the grid
+// Asks for a CTA of this grid that has not started, to do its work here: the
+// answer (16 bytes at `dst`) completes on `bar`.  After a refusal there must be
+// no further request.
+__device__ __forceinline__ void request_cta(uint32_t dst, uint32_t bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst),
+               "r"(bar)
+               : "memory");
+}
+
+// x index of the CTA that the answer grants, or -1.
+__device__ __forceinline__ int granted_cta(uint32_t src) {
+  int x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%1];\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n\t}"
+      : "=r"(x)
+      : "r"(src)
+      : "memory");
+  return x;
+}
+
+// ------------------------------------------- launches that follow one another
+// A kernel launched by launch_after may start while the kernel before it in the
+// stream still runs: wait_for_previous returns when that one is complete and
+// its writes are visible, and comes before every access to memory that it or
+// its predecessors touch.  launch_dependents lets the next such kernel start
+// once every CTA of this one has.  Both do nothing in a plain launch.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                         bool overlap, const Args&... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = overlap ? 1 : 0;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // ---------------------------------------------------------------- numerics
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   uint32_t r;

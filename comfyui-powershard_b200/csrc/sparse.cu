@@ -13,6 +13,7 @@
 // pair in every few thousand lists.
 #include "ps_b200.h"
 #include "internal.h"
+#include "ptx.cuh"
 
 #include <cuda_fp16.h>
 
@@ -47,6 +48,7 @@ __device__ __forceinline__ void add8(float (&a)[8], const uint4& v) {
 template <bool kFp16>
 __global__ void __launch_bounds__(kThreads) block_means_kernel(const MeansArgs args) {
   __shared__ double part[kWarps][32 * 9];
+  launch_dependents();
   int64_t cta = blockIdx.x;
   const int t = cta >= args.t[0].ctas;
   if (t) cta -= args.t[0].ctas;
@@ -93,76 +95,135 @@ __global__ void __launch_bounds__(kThreads) block_means_kernel(const MeansArgs a
   }
 }
 
-// 64-bit keys in the order of the scores: 0 for a block that may not be
-// chosen, above every number for NaN (a block with NaN in it is attended, so
-// that NaN is not hidden by the selection).
+// Whole numbers in the order of the scores; 0 is a block that may not be chosen.
+// Of 64-bit scores, NaN is above every number (a block with NaN in it is
+// attended, so that NaN is not hidden by the selection); of 32-bit ones it only
+// says that the 64-bit score is needed, and ~0u is left free.
 __device__ __forceinline__ unsigned long long order_key(double s) {
   if (s != s) return ~0ull;
   const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(s + 0.0));  // -0 is 0
   return (u >> 63) ? ~u : (u | (1ull << 63));
 }
+__device__ __forceinline__ uint32_t order_key(float s) {
+  if (s != s) return ~0u - 1;
+  const uint32_t u = __float_as_uint(s + 0.f);
+  return (u >> 31) ? ~u : (u | (1u << 31));
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
+}
 
-// Sums and prefixes over the threads that share a row: a warp, or the CTA.
-template <int kGroup>
-struct Group {
-  int* scratch;  // [2][kWarps], for the CTA
-  int phase = 0;
-  __device__ __forceinline__ int sum(int v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    if constexpr (kGroup == 32) return v;
-    int* s = scratch + kWarps * phase;  // the other half may still be read
-    phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) total += s[w];
-    return total;
-  }
-  // Threads of the group ahead of this one with `p` set; `total`: all of them.
-  __device__ __forceinline__ int rank(bool p, int& total) {
-    const unsigned m = __ballot_sync(0xffffffffu, p);
-    int before = __popc(m & ((1u << (threadIdx.x & 31)) - 1));
-    total = __popc(m);
-    if constexpr (kGroup == 32) return before;
-    int* s = scratch + kWarps * phase;
-    phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = total;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < static_cast<int>(threadIdx.x >> 5)) before += s[w];
-      total += s[w];
+// x = hi + lo: the upper 10 bits of the mantissa, and the rest, of which the
+// product drops what is below its own 10 (both by truncation, without a
+// conversion: those run at 16 a clock and SM).
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The keep-th largest of n keys (of those above 0, more than keep), by
+// bisection of their range: `floor` and how many that equal floor + 1 belong
+// to it are returned so that chosen = above floor + 1, plus the first `ties`
+// equal to it; ties 0: all above floor.  It ends as soon as exactly `keep` lie
+// above the middle (10 to 20 counts for scores that differ).
+template <typename Key>
+__device__ __forceinline__ void kth_largest(const Key* key, int n, int keep, Key lo, Key hi, int lane, Key& floor,
+                                            int& ties) {
+  int above = 0;  // keys above hi
+  ties = 0;
+  while (lo < hi) {
+    const Key mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
+    int c = 0;
+#pragma unroll 8
+    for (int i = lane; i < n; i += 32) c += key[i] >= mid;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c == keep) {
+      floor = mid - 1;
+      return;
     }
-    return before;
+    if (c > keep) {
+      lo = mid;
+    } else {
+      hi = mid - 1;
+      above = c;
+    }
   }
-};
+  floor = lo - 1;
+  ties = keep - above;
+}
 
-// One CTA scores kRows rows (query blocks of the query heads that share a key
-// head) against every key block, then selects: a warp per row, or with one row
-// the whole CTA.
+// Writes a row's chosen indices in ascending order (one warp): keys above
+// floor + 1, and the first `ties` equal to it (ties 0: keys above floor).
+template <typename Key>
+__device__ __forceinline__ void write_list(const Key* key, int n, Key floor, int ties, int keep, int* out, int* count,
+                                           int lane) {
+  const unsigned below = (1u << lane) - 1;
+  const Key equal = floor + 1;
+  const bool tied = ties > 0;
+  int done = 0;
+#pragma unroll 4
+  for (int n0 = 0; n0 < n; n0 += 32) {
+    const int i = n0 + lane;
+    const Key k = i < n ? key[i] : Key(0);
+    bool take = k > floor;
+    if (tied) {
+      const unsigned m = __ballot_sync(0xffffffffu, take && k == equal);
+      if (take && k == equal) take = __popc(m & below) < ties;
+      ties -= min(ties, __popc(m));
+    }
+    const unsigned m = __ballot_sync(0xffffffffu, take);
+    if (take) out[done + __popc(m & below)] = i;
+    done += __popc(m);
+  }
+  for (int i = done + lane; i < keep; i += 32) out[i] = -1;
+  if (lane == 0) *count = done;
+}
+
+// One CTA scores up to eight rows (query blocks of the query heads that share a
+// key head) against every key block, then a warp selects for each row.
 //
-// The k-th largest key is found by bisection of the 64-bit key range between
-// the row's least and greatest key; it ends as soon as exactly `keep` keys lie
-// above the middle (about log2 of a score's spacing: 10 to 20 counts of the
-// row in shared memory).
-template <int kRows>
-__global__ void __launch_bounds__(kThreads) block_select_kernel(const SelectArgs a) {
-  constexpr int kGroup = kRows == 1 ? kThreads : 32;
+// The scores are first taken on the tensor cores: each mean is split into two
+// tf32 terms and the three larger products are summed in 32 bits, which is off
+// by less than E = 2^-16 |q| max |k| (the dropped terms are 3 * 2^-20 |q||k|, 16
+// sums of the main products, nine terms each, keep 24 bits of their largest:
+// 2^-16.8; the sums of the small products are 2^-10 of that) plus what may
+// underflow.  With T the keep-th largest of these, a block above
+// T + 2E is chosen and one below T - 2E is not, in 64 bits too; only the blocks
+// between (the T block alone, in all but every few rows) are scored in 64 bits.
+// Measured at 75600 tokens, 5 heads, 1182 key blocks, 118 kept: all scores in
+// 64-bit FMAs 120 us (bound by their operands' shared-memory reads).
+//
+// Tiles are 16 key blocks x 8 rows.  The order of the 128 products is free, so
+// a thread loads 16 bytes of a mean and uses them in two products' k-steps: the
+// key means go from L2 to registers once per CTA, without shared memory.
+__global__ void __launch_bounds__(kThreads, 2) block_select_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  double* qs = reinterpret_cast<double*>(smem);                                             // [128][kRows]
-  unsigned long long* keys = reinterpret_cast<unsigned long long*>(qs + kHeadDim * kRows);  // [kRows][k_blocks]
-  __shared__ int scratch[2 * kWarps];
+  unsigned long long* exact = reinterpret_cast<unsigned long long*>(smem);  // [k_blocks], for rows with many ties
+  uint32_t* keys = reinterpret_cast<uint32_t*>(exact + a.k_blocks);         // [rows_per_cta][k_blocks]
+  __shared__ __align__(16) float means[8][kHeadDim];  // of the queries
+  __shared__ uint32_t longest;      // bits of max |k|^2
+  __shared__ uint32_t redo[8];      // rows whose undecided blocks are many: lo key, or 0
+  __shared__ uint32_t redo_hi[8];
 
+  launch_dependents();
+  wait_for_previous();  // the means
   const int rows = a.group * a.q_blocks;  // of one key head
-  const int chunks = (rows + kRows - 1) / kRows;
+  const int chunks = (rows + a.rows_per_cta - 1) / a.rows_per_cta;
   const int chunk = blockIdx.x % chunks;
   const int kv = (blockIdx.x / chunks) % a.kv_heads;
   const int batch = blockIdx.x / chunks / a.kv_heads;
   const int heads = a.kv_heads * a.group;
-  const int row0 = chunk * kRows;
-  const int tid = threadIdx.x;
+  const int row0 = chunk * a.rows_per_cta;
+  const int rows_here = min(a.rows_per_cta, rows - row0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tig = lane & 3;
 
   int k_blocks = a.k_blocks;
   if (a.k_len) {
@@ -174,191 +235,253 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(const SelectArgs
     const int64_t len = max(a.q_len[batch], 0);
     q_blocks = static_cast<int>(min(int64_t(q_blocks), (len + a.query_block - 1) / a.query_block));
   }
-
-  for (int i = tid; i < kHeadDim * kRows; i += kThreads) {
-    const int r = i / kHeadDim, d = i % kHeadDim;
-    const int row = row0 + r;
-    double v = 0;
-    if (row < rows) {
-      const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
-      v = a.q_means[((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * kHeadDim + d];
+  if (threadIdx.x == 0) longest = 0;
+  if (threadIdx.x < 8) redo[threadIdx.x] = 0;
+  if (warp < rows_here) {
+    const int row = row0 + warp;
+    const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
+    float4 m = make_float4(0, 0, 0, 0);
+    if (a.q) {  // few query rows: their mean is taken here
+      const int len = a.q_len ? min(max(a.q_len[batch], 0), a.len_q) : a.len_q;
+      const int n = min(max(len - qb * a.query_block, 0), a.query_block);
+      const uint16_t* x = static_cast<const uint16_t*>(a.q) + batch * a.q_st[0] +
+                          static_cast<int64_t>(qb) * a.query_block * a.q_st[1] + h * a.q_st[2] + 4 * lane;
+      double sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(x + i * a.q_st[1]));
+        const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = a.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
+                                  : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+          sum[2 * e] += static_cast<double>(f.x);
+          sum[2 * e + 1] += static_cast<double>(f.y);
+        }
+      }
+      if (n) m = make_float4(float(sum[0] / n), float(sum[1] / n), float(sum[2] / n), float(sum[3] / n));
+    } else {
+      m = __ldg(reinterpret_cast<const float4*>(a.q_means) +
+                ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
     }
-    qs[d * kRows + r] = v;
+    reinterpret_cast<float4*>(means[warp])[lane] = m;
   }
   __syncthreads();
 
+  auto q_mean = [&](int r) { return reinterpret_cast<const float4*>(means[r]); };  // of row r of this CTA
   const float4* km = reinterpret_cast<const float4*>(a.k_means) +
                      (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4);
   const int64_t kstep = static_cast<int64_t>(a.kv_heads) * (kHeadDim / 4);
-  auto put = [&](int r, int n, double s) {
-    const int row = row0 + r;
-    if (row >= rows) return;
-    const int qb = row % a.q_blocks;
-    bool may = n < k_blocks && qb < q_blocks;
-    if (may && a.allowed)
-      may = a.allowed[batch * a.allowed_st[0] + (kv * a.group + row / a.q_blocks) * a.allowed_st[1] +
-                      qb * a.allowed_st[2] + n * a.allowed_st[3]] != 0;
-    keys[static_cast<int64_t>(r) * a.k_blocks + n] = may ? order_key(s) : 0ull;
-  };
-  if constexpr (kRows == 1) {
-    // Four lanes share a key block, 16 bytes of its mean each in turn.
-    const int sub = tid & 3;
-    for (int n0 = 0; n0 < a.k_blocks; n0 += kThreads / 4) {
-      const int n = n0 + (tid >> 2);
-      double s0 = 0, s1 = 0;
-      if (n < k_blocks) {
-        const float4* p = km + n * kstep;
+
+  float q_sq = 0;  // |q|^2 of row g, after the sum over the four lanes that share it
+  {
+    float4 q[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float4 v = __ldg(p + 4 * u + sub);
-          const double* q = qs + (4 * u + sub) * 4;
-          s0 = fma(static_cast<double>(v.x), q[0], s0);
-          s1 = fma(static_cast<double>(v.y), q[1], s1);
-          s0 = fma(static_cast<double>(v.z), q[2], s0);
-          s1 = fma(static_cast<double>(v.w), q[3], s1);
-        }
-      }
-      double s = s0 + s1;
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (sub == 0 && n < a.k_blocks) put(0, n, s);
+    for (int j = 0; j < 8; ++j) {
+      q[j] = g < rows_here ? q_mean(g)[4 * j + tig] : make_float4(0, 0, 0, 0);
+      q_sq = fmaf(q[j].x, q[j].x, fmaf(q[j].y, q[j].y, fmaf(q[j].z, q[j].z, fmaf(q[j].w, q[j].w, q_sq))));
     }
-  } else {
-    // A thread per key block, kRows scores each: the query means come from
-    // shared memory as broadcasts, a key mean's line stays in L1 for its 512 B.
-    for (int n = tid; n < a.k_blocks; n += kThreads) {
-      double s[kRows];
+    // What each of this thread's two result columns (rows 2 tig, 2 tig + 1) may see.
+    const uint8_t* allowed[2] = {nullptr, nullptr};
+    bool in_use[2];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) s[r] = 0;
-      if (n < k_blocks) {
-        const float4* p = km + n * kstep;
-#pragma unroll 4
-        for (int u = 0; u < kHeadDim / 4; ++u) {
-          const float4 v = __ldg(p + u);
-          const double f[4] = {v.x, v.y, v.z, v.w};
+    for (int c = 0; c < 2; ++c) {
+      const int r = 2 * tig + c, row = row0 + r;
+      in_use[c] = r < rows_here && row % a.q_blocks < q_blocks;
+      if (a.allowed && in_use[c])
+        allowed[c] = a.allowed + batch * a.allowed_st[0] + (kv * a.group + row / a.q_blocks) * a.allowed_st[1] +
+                     (row % a.q_blocks) * a.allowed_st[2];
+    }
+    uint32_t most = 0;
+    for (int t = warp * 16; t < a.k_blocks; t += kWarps * 16) {
+      float c[4] = {0, 0, 0, 0}, small[4] = {0, 0, 0, 0};
+      float sq[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const double2* q = reinterpret_cast<const double2*>(qs + (4 * u + e) * kRows);
+      for (int half = 0; half < 2; ++half) {
+        float4 v[2][4];
 #pragma unroll
-            for (int r = 0; r < kRows / 2; ++r) {
-              const double2 w = q[r];
-              s[2 * r] = fma(f[e], w.x, s[2 * r]);
-              s[2 * r + 1] = fma(f[e], w.y, s[2 * r + 1]);
-            }
+        for (int i = 0; i < 2; ++i) {
+          const int n = t + g + 8 * i;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            v[i][j] = n < k_blocks ? __ldg(km + n * kstep + 4 * (4 * half + j) + tig) : make_float4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float f[2][4] = {{v[0][j].x, v[0][j].y, v[0][j].z, v[0][j].w},
+                                 {v[1][j].x, v[1][j].y, v[1][j].z, v[1][j].w}};
+          const float4 qj = q[4 * half + j];
+          const float qf[4] = {qj.x, qj.y, qj.z, qj.w};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t ah[4], al[4], bh[2], bl[2];
+            split_tf32(f[0][2 * u], ah[0], al[0]);
+            split_tf32(f[1][2 * u], ah[1], al[1]);
+            split_tf32(f[0][2 * u + 1], ah[2], al[2]);
+            split_tf32(f[1][2 * u + 1], ah[3], al[3]);
+            split_tf32(qf[2 * u], bh[0], bl[0]);
+            split_tf32(qf[2 * u + 1], bh[1], bl[1]);
+            mma_tf32(c, ah, bh[0], bh[1]);
+            mma_tf32(small, al, bh[0], bh[1]);
+            mma_tf32(small, ah, bl[0], bl[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              sq[i] = fmaf(f[i][2 * u], f[i][2 * u], fmaf(f[i][2 * u + 1], f[i][2 * u + 1], sq[i]));
           }
         }
       }
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) put(r, n, s[r]);
+      for (int i = 0; i < 4; ++i) c[i] += small[i];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 1);
+        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 2);
+        most = max(most, __float_as_uint(fabsf(sq[i])));  // NaN is above inf
+        const int n = t + g + 8 * i;
+        if (n >= a.k_blocks) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (2 * tig + e >= rows_here) continue;
+          const bool may = in_use[e] && n < k_blocks && (!allowed[e] || allowed[e][n * a.allowed_st[3]] != 0);
+          keys[(2 * tig + e) * a.k_blocks + n] = may ? order_key(c[2 * i + e]) : 0u;
+        }
+      }
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) atomicMax(&longest, most);
+    q_sq += __shfl_xor_sync(0xffffffffu, q_sq, 1);
+    q_sq += __shfl_xor_sync(0xffffffffu, q_sq, 2);
   }
   __syncthreads();
 
-  const int r = kRows == 1 ? 0 : tid >> 5;
-  const int me = kRows == 1 ? tid : tid & 31;
-  const int row = row0 + r;
-  if (row >= rows) return;  // a whole warp; with one row it never holds
-  const unsigned long long* key = keys + static_cast<int64_t>(r) * a.k_blocks;
-  Group<kGroup> group{scratch};
-  unsigned long long least = ~0ull, most = 0;
-  int n_may = 0;
-  for (int n = me; n < a.k_blocks; n += kGroup) {
-    const unsigned long long k = key[n];
-    if (k) {
-      ++n_may;
-      least = min(least, k);
+  auto list_of = [&](int r) {
+    const int row = row0 + r;
+    return (static_cast<int64_t>(batch) * heads + kv * a.group + row / a.q_blocks) * a.q_blocks + row % a.q_blocks;
+  };
+  if (warp < rows_here) {
+    const int r = warp;
+    uint32_t* key = keys + r * a.k_blocks;
+    const int64_t list = list_of(r);
+    uint32_t least = ~0u, most = 0;
+    int n_may = 0;
+#pragma unroll 8
+    for (int n = lane; n < a.k_blocks; n += 32) {
+      const uint32_t k = key[n];
+      n_may += k != 0;
+      least = min(least, k - 1);  // 0 becomes the largest
       most = max(most, k);
     }
-  }
-  n_may = group.sum(n_may);
-  // Chosen: every key above `floor`, and the first `ties` that equal it.
-  unsigned long long floor = 0;
-  int ties = 0;
-  if (n_may > a.keep) {
-    // In the CTA form each warp's bounds would differ: the whole key range
-    // costs a few counts more.
-    unsigned long long lo = 1, hi = ~0ull;
-    if constexpr (kGroup == 32) {
+    n_may = __reduce_add_sync(0xffffffffu, n_may);
+    uint32_t floor = 0;
+    bool settled = true;
+    if (n_may > a.keep) {
+      least = __reduce_min_sync(0xffffffffu, least) + 1;
+      most = __reduce_max_sync(0xffffffffu, most);
+      int ties;
+      kth_largest(key, a.k_blocks, a.keep, least, most, lane, floor, ties);
+      // T: the smallest key above floor.
+      uint32_t kth = ~0u;
+#pragma unroll 8
+      for (int n = lane; n < a.k_blocks; n += 32) {
+        const uint32_t k = key[n];
+        if (k > floor) kth = min(kth, k);
+      }
+      kth = __reduce_min_sync(0xffffffffu, kth);
+      const float T = of_key(kth);
+      const float len_q = sqrtf(__shfl_sync(0xffffffffu, q_sq, 4 * r));
+      const float len_k = sqrtf(__uint_as_float(longest));
+      const float E2 = 3.0517578125e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-15, 2^-110
+      uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
+      if (kth < ~0u - 1 && isfinite(T - E2) && isfinite(T + E2)) {
+        lo_key = order_key(T - E2);
+        hi_key = order_key(T + E2);
+      }
+      int sure = 0, open = 0;
+#pragma unroll 8
+      for (int n = lane; n < a.k_blocks; n += 32) {
+        const uint32_t k = key[n];
+        sure += k > hi_key;
+        open += k >= lo_key && k <= hi_key;
+      }
+      sure = __reduce_add_sync(0xffffffffu, sure);
+      open = __reduce_add_sync(0xffffffffu, open);
+      const int wanted = a.keep - sure;
+      if (open == wanted) {
+        floor = lo_key - 1;
+      } else if (open <= 32) {
+        // Lane i takes the i-th undecided block, in the order of their indices.
+        int mine = -1, seen = 0;
+        for (int n0 = 0; n0 < a.k_blocks && seen < open; n0 += 32) {
+          const uint32_t k = n0 + lane < a.k_blocks ? key[n0 + lane] : 0u;
+          unsigned m = __ballot_sync(0xffffffffu, k >= lo_key && k <= hi_key);
+          for (; m; m &= m - 1, ++seen)
+            if (lane == seen) mine = n0 + __ffs(m) - 1;
+        }
+        const float4 qv = q_mean(r)[lane];
+        unsigned long long score = 0;
+        for (int e = 0; e < open; ++e) {
+          const float4 kk = __ldg(km + __shfl_sync(0xffffffffu, mine, e) * kstep + lane);
+          double d = fma(double(qv.x), double(kk.x), double(qv.y) * double(kk.y)) +
+                     fma(double(qv.z), double(kk.z), double(qv.w) * double(kk.w));
 #pragma unroll
-      for (int o = 16; o; o >>= 1) {
-        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      }
-      lo = least;
-      hi = most;
-    }
-    int above = 0;  // keys above hi
-    bool found = false;
-    while (lo < hi) {
-      const unsigned long long mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
-      int c = 0;
-      for (int n = me; n < a.k_blocks; n += kGroup) c += key[n] >= mid;
-      c = group.sum(c);
-      if (c == a.keep) {
-        floor = mid - 1;
-        found = true;
-        break;
-      }
-      if (c > a.keep) {
-        lo = mid;
+          for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if (lane == e) score = order_key(d);
+        }
+        int better = 0;
+        for (int e = 0; e < open; ++e) {
+          const unsigned long long other = __shfl_sync(0xffffffffu, score, e);
+          better += other > score || (other == score && e < lane);
+        }
+        __syncwarp();
+        if (lane < open) key[mine] = better < wanted ? ~0u : 0u;
+        __syncwarp();
+        floor = hi_key;
       } else {
-        hi = mid - 1;
-        above = c;
+        settled = false;
+        if (lane == 0) {
+          redo[r] = lo_key;
+          redo_hi[r] = hi_key;
+        }
       }
     }
-    if (!found) {
-      floor = lo;
-      ties = a.keep - above;
-    }
+    if (settled) write_list(key, a.k_blocks, floor, 0, a.keep, a.blocks + list * a.keep, a.counts + list, lane);
   }
-  const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
-  const int64_t list = (static_cast<int64_t>(batch) * heads + h) * a.q_blocks + qb;
-  int* out = a.blocks + list * a.keep;
-  int done = 0;
-  for (int n0 = 0; n0 < a.k_blocks; n0 += kGroup) {
-    const int n = n0 + me;
-    const unsigned long long k = n < a.k_blocks ? key[n] : 0ull;
-    bool take = k > floor;
-    int all;
-    if (ties > 0) {  // the same for the whole group
-      const int before = group.rank(k == floor && k != 0, all);
-      take |= k == floor && k != 0 && before < ties;
-      ties -= min(ties, all);
+  __syncthreads();
+  // Rows with more than 32 undecided blocks (equal or overflowing scores): the
+  // CTA scores them in 64 bits, one warp selects.
+  for (int r = 0; r < rows_here; ++r) {
+    const uint32_t lo_key = redo[r], hi_key = redo_hi[r];
+    if (!lo_key) continue;
+    const float4* q = q_mean(r);
+    for (int n = threadIdx.x; n < a.k_blocks; n += kThreads) {
+      const uint32_t k = keys[r * a.k_blocks + n];
+      unsigned long long e = k > hi_key ? ~0ull : 0ull;
+      if (k >= lo_key && k <= hi_key) {
+        double d = 0;
+        for (int u = 0; u < kHeadDim / 4; ++u) {
+          const float4 x = q[u], y = __ldg(km + n * kstep + u);
+          d = fma(double(x.x), double(y.x), d);
+          d = fma(double(x.y), double(y.y), d);
+          d = fma(double(x.z), double(y.z), d);
+          d = fma(double(x.w), double(y.w), d);
+        }
+        e = order_key(d);
+      }
+      exact[n] = e;
     }
-    const int at = done + group.rank(take, all);
-    if (take) out[at] = n;
-    done += all;
+    __syncthreads();
+    if (warp == 0) {
+      unsigned long long floor;
+      int ties;
+      kth_largest(exact, a.k_blocks, a.keep, 1ull, ~0ull, lane, floor, ties);
+      const int64_t list = list_of(r);
+      write_list(exact, a.k_blocks, floor, ties, a.keep, a.blocks + list * a.keep, a.counts + list, lane);
+    }
+    __syncthreads();
   }
-  for (int i = done + me; i < a.keep; i += kGroup) out[i] = -1;
-  if (me == 0) a.counts[list] = done;
 }
 
-// Shared memory of one CTA with `rows` rows of k_blocks keys.
-inline size_t select_smem(int rows, int k_blocks) {
-  return size_t(rows) * (kHeadDim + size_t(k_blocks)) * sizeof(double);
-}
-
-template <int kRows>
-int launch_select(const SelectArgs& a, cudaStream_t stream) {
-  static bool done[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (!done[dev]) {
-    const cudaError_t err = cudaFuncSetAttribute(block_select_kernel<kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(kSelectSmemLimit));
-    if (err != cudaSuccess) return set_cuda_error("block_select: cudaFuncSetAttribute", err);
-    done[dev] = true;
-  }
-  const int64_t chunks = (int64_t(a.group) * a.q_blocks + kRows - 1) / kRows;
-  const int64_t ctas = chunks * a.kv_heads * a.batch;
-  if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^31 lists");
-  block_select_kernel<kRows>
-      <<<static_cast<unsigned>(ctas), kThreads, select_smem(kRows, a.k_blocks), stream>>>(a);
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
-  count_launch();
-  return 0;
-}
+inline size_t select_smem(int rows, int k_blocks) { return size_t(k_blocks) * (8 + 4 * size_t(rows)); }
 
 }  // namespace sparse
 
@@ -377,12 +500,27 @@ int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream) {
   return 0;
 }
 
-int launch_block_select(const SelectArgs& a, cudaStream_t stream) {
+int launch_block_select(SelectArgs a, cudaStream_t stream) {
   using namespace sparse;
-  // Eight rows a CTA read each key mean once for eight scores; with fewer
-  // rows than half of that, or rows too long for shared memory, one row a CTA.
-  const bool eight = int64_t(a.group) * a.q_blocks >= 4 && select_smem(8, a.k_blocks) <= kSelectSmemLimit;
-  return eight ? launch_select<8>(a, stream) : launch_select<1>(a, stream);
+  static bool done[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!done[dev]) {
+    const cudaError_t err = cudaFuncSetAttribute(block_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(kSelectSmemLimit));
+    if (err != cudaSuccess) return set_cuda_error("block_select: cudaFuncSetAttribute", err);
+    done[dev] = true;
+  }
+  // Eight rows share a CTA's reads of the key means where their keys fit shared memory.
+  a.rows_per_cta = select_smem(8, a.k_blocks) <= kSelectSmemLimit ? 8 : 1;
+  const int64_t chunks = (int64_t(a.group) * a.q_blocks + a.rows_per_cta - 1) / a.rows_per_cta;
+  const int64_t ctas = chunks * a.kv_heads * a.batch;
+  if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^31 lists");
+  const cudaError_t err = launch_after(block_select_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads),
+                                       select_smem(a.rows_per_cta, a.k_blocks), stream, a.after_means, a);
+  if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
+  count_launch();
+  return 0;
 }
 
 }  // namespace psb

@@ -6,6 +6,9 @@ allocates: callers pass every output buffer.
 """
 from __future__ import annotations
 
+import functools
+import struct
+
 import torch
 
 from . import _lib
@@ -784,40 +787,81 @@ def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: 
         status.arm()
 
 
+# ps_b200_sparse_call: ten addresses, the strides, eleven sizes and the scale.
+_SPARSE_CALL = struct.Struct("@10P16q11qd")
+
+
+@functools.lru_cache(maxsize=256)
+def _sparse_scratch_bytes(device_index: int, *sizes) -> int:
+    with torch.cuda.device(device_index):
+        return _lib.load().ps_b200_sparse_scratch_bytes(*sizes)
+
+
+def sparse_forward(q, k, v, out, keep: int, query_block: int, key_block: int, scale: float, status: DeviceStatus,
+                   key_means=None, allowed=None, query_lengths=None, key_lengths=None):
+    """``block_means``, ``block_select`` and ``sparse_attention`` in one library
+    call, for q/out [B, Lq, Hq, 128], k/v [B, Lk, Hk, 128] of one 16-bit dtype.
+
+    What the steps hand on lives in one scratch buffer from the caching
+    allocator, so concurrent calls and captured graphs each have their own."""
+    lib = _lib.load()
+    device = q.device
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    if allowed is not None and (allowed.dtype != torch.bool or allowed.device != device):
+        raise ValueError(f"sparse attention: allowed must be bool on {device}")
+    n = _sparse_scratch_bytes(device.index, b, hq, hk, lq, lk, keep, query_block, key_block, key_means is not None)
+    scratch = torch.empty(n, dtype=torch.uint8, device=device)
+    call = _SPARSE_CALL.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if key_means is None else key_means.data_ptr(),
+        0 if allowed is None else allowed.data_ptr(),
+        _lengths_arg(query_lengths, b, device, "sparse attention query_lengths") or 0,
+        _lengths_arg(key_lengths, b, device, "sparse attention key_lengths") or 0, scratch.data_ptr(), status.ptr,
+        *_row_strides(q, "sparse attention q"), *_row_strides(k, "sparse attention k"),
+        *_row_strides(v, "sparse attention v"), *_row_strides(out, "sparse attention out"),
+        *((0, 0, 0, 0) if allowed is None else allowed.stride()), _lib.dtype_code(q.dtype), b, hq, hk, d, lq, lk, keep,
+        query_block, key_block, n, scale)
+    rc = lib.ps_b200_sparse_fwd(call, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, "ps_b200_sparse_fwd")
+    status.arm()
+
+
 _CODES = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.INT8}
 
 
+# ps_b200_cache_call: nine addresses, six strides and ten sizes.
+_CACHE_CALL = struct.Struct("@9P6q10q")
+
+
 def _cache_call(name, pages, scales, rows, table, first, count):
-    lib = _lib.load()
-    k = pages[0]
-    device = k.device
+    (k, v), (ks, vs), (x, y) = pages, scales, rows
+    device, shape = k.device, k.shape
     _lib.require_cuda(k, name)
-    if k.dtype not in _CODES:
+    code = _CODES.get(k.dtype)
+    if code is None:
         raise _lib.UnsupportedAttention(f"{name}: pages hold float8_e4m3fn or int8 codes, got {k.dtype}")
-    if k.dim() != 4:
-        raise ValueError(f"{name}: pages must be [pages, page_rows, H, D], got {tuple(k.shape)}")
-    for p, s in zip(pages, scales):
-        if p.shape != k.shape or p.dtype != k.dtype or p.device != device or not p.is_contiguous():
-            raise ValueError(f"{name}: K and V pages must be contiguous and alike")
-        if s.shape != k.shape[:3] or s.dtype != torch.float32 or s.device != device or not s.is_contiguous():
-            raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(k.shape[:3])} on {device}")
-    strides = []
-    x = rows[0]
-    for t in rows:
-        strides += _row_strides(t, name)
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != device or t.shape[2:] != k.shape[2:]:
-            raise ValueError(f"{name}: K and V rows must be alike, [B, n, {k.shape[2]}, {k.shape[3]}] on {device}")
-    batch, n = x.shape[:2]
+    if (len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.device != device
+            or not k.is_contiguous() or not v.is_contiguous()):
+        raise ValueError(f"{name}: K and V pages must be alike, contiguous [pages, page_rows, H, D] on one device")
+    for s in (ks, vs):
+        if s.shape != shape[:3] or s.dtype != torch.float32 or s.device != device or not s.is_contiguous():
+            raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(shape[:3])} on {device}")
+    strides = *_row_strides(x, name), *_row_strides(y, name)
+    if y.shape != x.shape or x.shape[2:] != shape[2:] or y.dtype != x.dtype or x.device != device or y.device != device:
+        raise ValueError(f"{name}: K and V rows must be alike, [B, n, {shape[2]}, {shape[3]}] on {device}")
+    batch, n = x.shape[0], x.shape[1]
     if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.stride(1) != 1
             or table.device != device):
         raise ValueError(f"{name}: the page table must be int32 [{batch}, pages] with unit inner stride on {device}")
-    rc = getattr(lib, name)(
-        _lib.ptrs([t.data_ptr() for t in pages]), _lib.ptrs([t.data_ptr() for t in scales]),
-        _lib.ptrs([t.data_ptr() for t in rows]), _lib.i64(strides), _lib.dtype_code(x.dtype), _CODES[k.dtype], batch, n,
-        k.shape[2], k.shape[3], k.shape[0], k.shape[1], table.data_ptr(), table.stride(0), table.shape[1],
-        _lengths_arg(first, batch, device, f"{name} first"), _lengths_arg(count, batch, device, f"{name} count"),
-        _lib.stream_handle(device))
-    _lib.check(rc, name)
+    call = _CACHE_CALL.pack(
+        k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), x.data_ptr(), y.data_ptr(), table.data_ptr(),
+        _lengths_arg(first, batch, device, f"{name} first") or 0,
+        _lengths_arg(count, batch, device, f"{name} count") or 0, *strides, _lib.dtype_code(x.dtype), code, batch, n,
+        shape[2], shape[3], shape[0], shape[1], table.stride(0), table.shape[1])
+    rc = getattr(_lib.load(), name)(call, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def cache_write(pages, scales, rows, table, first=None, count=None):

@@ -21,6 +21,7 @@ call can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -30,18 +31,32 @@ from .contract import AttentionOptions, UnsupportedAttention
 from .provider import B200Provider, _tma_ok
 
 NAME = "b200_sparse"
+_DEFAULT = AttentionOptions()
 QUERY_BLOCK, KEY_BLOCK = 256, 128
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """t, or a contiguous copy where its strides do not suit the kernels'
     loads (an expanded axis has stride 0, which a tensor map cannot hold)."""
-    return t if _tma_ok(t) and all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape)) else t.contiguous()
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t if _tma_ok(t) and all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape)) else t.clone(
+        memory_format=torch.contiguous_format)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
-    """Context in which `device` is current."""
-    return torch.cuda.device(device)
+    """Context in which `device` is current (nothing to do where it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _broadcast(allowed, shape):
+    if torch.broadcast_shapes(allowed.shape, shape) != shape:
+        raise ValueError(f"allowed {tuple(allowed.shape)} does not broadcast to {shape} "
+                         "(batch, heads, query blocks, key blocks)")
+    return allowed.broadcast_to(shape)
 
 
 def block_means(x, block: int, lengths=None):
@@ -74,9 +89,7 @@ def select_blocks(query_means, key_means, keep: int, *, allowed=None, query_bloc
     if keep < 1:
         raise ValueError(f"select_blocks: keep must be at least 1, got {keep}")
     if allowed is not None:
-        if torch.broadcast_shapes(allowed.shape, (b, h, nq, nk)) != (b, h, nq, nk):
-            raise ValueError(f"select_blocks: allowed {tuple(allowed.shape)} does not broadcast to {(b, h, nq, nk)}")
-        allowed = allowed.broadcast_to(b, h, nq, nk)
+        allowed = _broadcast(allowed, (b, h, nq, nk))
     keep = min(int(keep), nk)
     device = query_means.device
     blocks = torch.empty((b, h, nq, keep), dtype=torch.int32, device=device)
@@ -153,24 +166,25 @@ class SparseProvider(B200Provider):
         key_means: ``block_means(k, key_block, key_lengths)`` kept from an
         earlier call (of a cache that grew, its new blocks' means appended);
         allowed: bool, broadcastable to [B, Hq, query blocks, key blocks]."""
-        o = o or AttentionOptions()
+        o = o or _DEFAULT
         self.check(q, k, v, o)
+        device = q.device
+        status = _status_for(device)
+        status.poll()
         q, k, v = _readable(q), _readable(k), _readable(v)
         b, lq, h, d = q.shape
-        lk, hk = k.shape[1:3]
+        lk, hk = k.shape[1], k.shape[2]
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        if lq == 0:
+            return out
         nq, nk = -(-lq // self.query_block), -(-lk // self.key_block)
-        q_means = torch.empty((b, nq, h, d), dtype=torch.float32, device=q.device)
-        with _on(q.device):
-            if key_means is None:
-                key_means = torch.empty((b, nk, hk, d), dtype=torch.float32, device=q.device)
-                ops.block_means([q, k], [self.query_block, self.key_block], [query_lengths, key_lengths],
-                                [q_means, key_means])
-            else:
-                if tuple(key_means.shape) != (b, nk, hk, d):
-                    raise ValueError(f"key_means: expected {(b, nk, hk, d)}, got {tuple(key_means.shape)}")
-                ops.block_means([q], [self.query_block], [query_lengths], [q_means])
-        blocks, counts = select_blocks(
-            q_means, key_means, self.blocks_kept(nk), allowed=allowed, query_block=self.query_block,
-            key_block=self.key_block, query_lengths=query_lengths, key_lengths=key_lengths)
-        return sparse_attention(q, k, v, blocks, counts, query_block=self.query_block, key_block=self.key_block,
-                                softmax_scale=o.softmax_scale, query_lengths=query_lengths, key_lengths=key_lengths)
+        if allowed is not None:
+            allowed = _broadcast(allowed, (b, h, nq, nk))
+        if key_means is not None and (tuple(key_means.shape) != (b, nk, hk, d) or key_means.dtype != torch.float32
+                                      or not key_means.is_contiguous() or key_means.device != device):
+            raise ValueError(f"key_means: expected contiguous fp32 {(b, nk, hk, d)} on {device}")
+        scale = d ** -0.5 if o.softmax_scale is None else float(o.softmax_scale)
+        with _on(device):
+            ops.sparse_forward(q, k, v, out, self.blocks_kept(nk), self.query_block, self.key_block, scale, status,
+                               key_means, allowed, query_lengths, key_lengths)
+        return out

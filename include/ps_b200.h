@@ -445,7 +445,7 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
  *   behind them are never chosen, query blocks behind them choose none.  A
  *   score of NaN ranks above all numbers.  blocks [batch][heads_q][q_blocks]
  *   [keep]: the chosen in ascending order, -1 behind them; counts
- *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 25472.
+ *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 16384.
  */
 int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv,
                          int head_dim, int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
@@ -474,13 +474,40 @@ int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const voi
                             size_t workspace_bytes, int* status, void* stream);
 
 /*
+ * ps_b200_sparse_fwd: the three steps above in one call, on one scratch buffer
+ *   (device, 256-byte aligned, ps_b200_sparse_scratch_bytes(...) bytes, owned by
+ *   one call at a time).  key_means: the keys' means kept from an earlier call,
+ *   or NULL to take them here (with_key_means says which to the size).  The
+ *   other fields are those of the three entries; every field is 8 bytes.
+ */
+typedef struct ps_b200_sparse_call {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* key_means;
+  const unsigned char* allowed;
+  const int* q_len;
+  const int* k_len;
+  void* scratch;
+  int* status;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3], allowed_strides[4];
+  int64_t dtype, batch, heads_q, heads_kv, head_dim, len_q, len_k, keep, query_block, key_block, scratch_bytes;
+  double softmax_scale;
+} ps_b200_sparse_call;
+size_t ps_b200_sparse_scratch_bytes(int batch, int heads_q, int heads_kv, int len_q, int len_k, int keep,
+                                    int query_block, int key_block, int with_key_means);
+int ps_b200_sparse_fwd(const ps_b200_sparse_call* call, void* stream);
+
+/*
  * 8-bit key/value cache in pages.  pages: K and V codes
  *   [num_pages][page_rows][heads][head_dim] (cache_dtype PS_B200_E4M3 or _INT8),
  *   scales fp32 [num_pages][page_rows][heads].  Position p of sequence b lives
  *   in row p % page_rows of page table[b*table_stride + p / page_rows] (device
- *   ints).  rows: K and V [batch][n][heads][head_dim] bf16/fp16 under strides
- *   (batch, row, head of K, then of V; multiples of 8 elements); head_dim 64,
- *   128 or 256.
+ *   ints, table_len of them a sequence).  rows: K and V
+ *   [batch][n][heads][head_dim] bf16/fp16 under strides (batch, row, head of K,
+ *   then of V; multiples of 8 elements); head_dim 64, 128 or 256.  first and
+ *   count: device int [batch].
  * ps_b200_cache_write stores row i < count[b] (NULL: n) of sequence b at position
  *   first[b] + i (NULL: i): scale = max(max|x|, 2^-100) / M over the head's
  *   values, code = round(x * (M / max(..))), M = 448 or 127.  Rows whose position
@@ -490,14 +517,18 @@ int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const voi
  *   count[b]; the rows behind them stay as they are, a position whose page is
  *   out of range reads as zeros.
  */
-int ps_b200_cache_write(void* const pages[2], float* const scales[2], const void* const rows[2],
-                        const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
-                        int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
-                        int table_len, const int* first, const int* count, void* stream);
-int ps_b200_cache_read(const void* const pages[2], const float* const scales[2], void* const rows[2],
-                       const int64_t strides[6], int dtype, int cache_dtype, int batch, int n, int heads,
-                       int head_dim, int num_pages, int page_rows, const int* table, int64_t table_stride,
-                       int table_len, const int* first, const int* count, void* stream);
+typedef struct ps_b200_cache_call {
+  void* pages[2];
+  float* scales[2];
+  void* rows[2]; /* only read by the write */
+  const int* table;
+  const int* first;
+  const int* count;
+  int64_t strides[6];
+  int64_t dtype, cache_dtype, batch, n, heads, head_dim, num_pages, page_rows, table_stride, table_len;
+} ps_b200_cache_call;
+int ps_b200_cache_write(const ps_b200_cache_call* call, void* stream);
+int ps_b200_cache_read(const ps_b200_cache_call* call, void* stream);
 
 /*
  * Self-test of the bounded waits (no counterpart in the reference): one warp

@@ -63,24 +63,24 @@ def test_refusals_before_any_launch():
 def test_entries_validate_on_the_host():
     from powershard_b200 import _lib
     lib = _lib.load()
-    st = _lib.i64([0, 256, 128] * 2)
+    from powershard_b200.ops import _CACHE_CALL
 
     def call(write=True, dtype=_lib.BF16, stored=_lib.E4M3, n=4, heads=2, dim=128, page_rows=16, pages=16, rows=16,
-             strides=st, table=16, count=16):
+             strides=(0, 256, 128) * 2, table=16, count=16):
         fn = lib.ps_b200_cache_write if write else lib.ps_b200_cache_read
-        return fn(_lib.ptrs([pages, 16]), _lib.ptrs([16, 16]), _lib.ptrs([rows, 16]), strides, dtype, stored, 1, n,
-                  heads, dim, 4, page_rows, table, 4, 4, None, count, None)
+        return fn(_CACHE_CALL.pack(pages, 16, 16, 16, rows, 16, table, 0, count, *strides, dtype, stored, 1, n, heads,
+                                   dim, 4, page_rows, 4, 4), None)
 
     for write in (True, False):
         assert call(write, dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED
         assert call(write, stored=_lib.BF16) == _lib.ERR_UNSUPPORTED
         assert call(write, dim=96) == _lib.ERR_UNSUPPORTED and b"64, 128 or 256" in lib.ps_b200_last_error()
-        assert call(write, page_rows=0) == _lib.ERR_INVALID and call(write, heads=5000) == _lib.ERR_INVALID
+        assert call(write, page_rows=0) == _lib.ERR_INVALID and call(write, n=1 << 32) == _lib.ERR_INVALID and call(write, heads=5000) == _lib.ERR_INVALID
         assert call(write, pages=24) == _lib.ERR_INVALID and call(write, rows=24) == _lib.ERR_INVALID
-        assert call(write, strides=_lib.i64([0, 250, 128] * 2)) == _lib.ERR_INVALID
-        assert call(write, table=None) == _lib.ERR_INVALID and call(write, table=18) == _lib.ERR_INVALID
+        assert call(write, strides=(0, 250, 128) * 2) == _lib.ERR_INVALID
+        assert call(write, table=0) == _lib.ERR_INVALID and call(write, table=18) == _lib.ERR_INVALID
         assert call(write, n=0) == _lib.OK
-    assert call(False, count=None) == _lib.ERR_INVALID and b"lengths" in lib.ps_b200_last_error()
+    assert call(False, count=0) == _lib.ERR_INVALID and b"lengths" in lib.ps_b200_last_error()
     assert lib.ps_b200_kernel_launches() == 0
 
 

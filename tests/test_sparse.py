@@ -143,6 +143,20 @@ def test_entries_validate_on_the_host():
     assert fwd(n=1 << 25) == _lib.ERR_INVALID  # names more than 2^30 rows
     assert fwd(lq=0) == _lib.OK
 
+    from powershard_b200.ops import _SPARSE_CALL
+
+    def whole(batch=1, heads=2, kv=2, dim=128, lq=300, lk=300, keep=2, qb=256, kb=64, scratch=256, nbytes=1 << 30,
+              dtype=_lib.BF16):
+        return lib.ps_b200_sparse_fwd(_SPARSE_CALL.pack(
+            16, 16, 16, 16, 0, 0, 0, 0, scratch, 0, *(0, 256, 128) * 4, 0, 0, 0, 0, dtype, batch, heads, kv, dim, lq, lk,
+            keep, qb, kb, nbytes, 0.1), None)
+
+    assert whole(batch=1 << 31) == _lib.ERR_INVALID and whole(lk=0) == _lib.ERR_INVALID and whole(lq=0) == _lib.OK
+    assert whole(keep=0) == _lib.ERR_INVALID and whole(keep=6) == _lib.ERR_INVALID and whole(heads=3) == _lib.ERR_INVALID
+    assert whole(scratch=0) == _lib.ERR_INVALID and whole(nbytes=100) == _lib.ERR_INVALID and whole(scratch=272) == _lib.ERR_INVALID
+    assert whole(dim=64) == _lib.ERR_UNSUPPORTED and whole(kb=32) == _lib.ERR_UNSUPPORTED
+    assert whole(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED
+
     def select(heads=2, kv=2, dim=128, nq=2, nk=5, keep=3, means=16, lists=16):
         return lib.ps_b200_block_select(means, 16, 1, heads, kv, dim, nq, nk, keep, None, None, None, 256, None, 64,
                                         lists, 16, None)
@@ -222,6 +236,36 @@ def test_select_ties_and_nan(cuda_lib, nq):
         got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
         want = ref_select(qm, km, keep)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nk", [40, 700, 6000])
+def test_select_in_64_bits(cuda_lib, nk):
+    """Scores that 32 bits cannot tell apart, few and many, and scores that overflow 32 bits."""
+    from powershard_b200 import sparse
+    g = torch.Generator().manual_seed(30)
+    for alike in (5, 33, nk):
+        qm, km = torch.randn(1, 5, 1, 128, generator=g), torch.randn(1, nk, 1, 128, generator=g)
+        some = torch.randperm(nk, generator=g)[:alike]
+        near = km[0, 0, 0].expand(len(some), -1).clone()
+        near[torch.arange(len(some)), torch.randint(0, 128, (len(some),), generator=g)] *= 1 + 2.0 ** -22
+        km[0, some, 0] = near
+        order = ref_select(qm, km, nk)  # every rank at which the near ones may be cut
+        for keep in (1, nk // 7, nk // 2, nk - 3):
+            got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
+            want = ref_select(qm, km, keep)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (alike, keep)
+        for t in range(5):  # cut inside the near ones
+            s = (km[0, :, 0].double() @ qm[0, t, 0].double()).sort(descending=True).values
+            mid = float(km[0, some[0], 0].double() @ qm[0, t, 0].double())
+            keep = min(nk, max(1, int((s > mid).sum()) + 1))
+            got = sparse.select_blocks(*cuda(qm, km), keep)[0].cpu()
+            assert torch.equal(got, ref_select(qm, km, keep)[0])
+        assert order[1].eq(nk).all()
+    for size in (1e25, 1e-25, 1e-38):
+        qm, km = torch.randn(1, 2, 1, 128, generator=g) * size, torch.randn(1, nk, 1, 128, generator=g) * size
+        got = sparse.select_blocks(*cuda(qm, km), nk // 3)[0].cpu()
+        assert torch.equal(got, ref_select(qm, km, nk // 3)[0])
 
 
 # ------------------------------------------------------------------ attention over lists
