@@ -296,7 +296,7 @@ int check_blocks(int batch, int heads_q, int heads_kv, int head_dim, int query_b
 // Where one block-sparse call keeps what its three steps hand on, each on a 256-byte boundary.
 struct SparseScratch {
   int64_t q_blocks, k_blocks;
-  size_t q_means, k_means, blocks, counts, workspace, workspace_bytes, total;
+  size_t q_means, k_means, blocks, counts, scores, scores_bytes, workspace, workspace_bytes, total;
 };
 
 SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t len_q, int64_t len_k,
@@ -315,6 +315,9 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   s.k_means = take(key_means ? 0 : size_t(batch * heads_kv * s.k_blocks) * 128 * sizeof(float));
   s.blocks = take(lists * keep * sizeof(int));
   s.counts = take(lists * sizeof(int));
+  s.scores_bytes =
+      size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, s.q_blocks, s.k_blocks)) * sizeof(float);
+  s.scores = take(s.scores_bytes);
   s.workspace_bytes = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count()).workspace_bytes();
   s.workspace = take(s.workspace_bytes);
   s.total = at;
@@ -1034,7 +1037,8 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
 static int block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
                         int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
                         const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
-                        int key_block, int* blocks, int* counts, void* stream, SelectArgs from = {}) {
+                        int key_block, int* blocks, int* counts, void* workspace, size_t workspace_bytes, void* stream,
+                        SelectArgs from = {}) {
   if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
   if (q_blocks < 0 || k_blocks < 0 || keep < 1) return set_error(PS_B200_ERR_INVALID, "keep must be positive, block counts not negative");
   if (keep > k_blocks && k_blocks > 0) return set_error(PS_B200_ERR_INVALID, "keep %d above the %d key blocks", keep, k_blocks);
@@ -1042,14 +1046,18 @@ static int block_select(const float* q_means, const float* k_means, int batch, i
   if (k_blocks == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
   if (k_blocks > kSelectMaxBlocks)
     return set_error(PS_B200_ERR_UNSUPPORTED, "%d key blocks: at most %d, take larger blocks", k_blocks, kSelectMaxBlocks);
-  if ((!q_means && !from.q) || !k_means || !aligned16(q_means) || !aligned16(k_means))
+  if (!q_means || !k_means || !aligned16(q_means) || !aligned16(k_means))
     return set_error(PS_B200_ERR_INVALID, "means null or not 16-byte aligned");
   if (!blocks || !counts || !aligned4(blocks) || !aligned4(counts) || !aligned4(q_len) || !aligned4(k_len))
     return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
   if (allowed && !allowed_strides) return set_error(PS_B200_ERR_INVALID, "allowed needs strides");
+  const size_t need = ps_b200_block_select_workspace_bytes(batch, heads_q, heads_kv, q_blocks, k_blocks);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+    return set_error(PS_B200_ERR_INVALID, "this call needs a 16-byte aligned workspace of %zu bytes (got %zu)", need,
+                     workspace ? workspace_bytes : size_t(0));
   if (int rc = check_device()) return rc;
   SelectArgs a = from;
-  a.q_means = q_means;
+  a.q_means = const_cast<float*>(q_means);  // written only for the queries of `from`
   a.k_means = k_means;
   a.batch = batch;
   a.kv_heads = heads_kv;
@@ -1065,15 +1073,24 @@ static int block_select(const float* q_means, const float* k_means, int batch, i
   for (int i = 0; i < 4; ++i) a.allowed_st[i] = allowed ? allowed_strides[i] : 0;
   a.blocks = blocks;
   a.counts = counts;
+  a.scores = static_cast<float*>(workspace);
+  a.k_sq = a.scores + int64_t(select_units(batch, a.kv_heads, a.group, q_blocks, k_blocks)) * a.group * q_blocks * k_blocks;
   return launch_block_select(a, static_cast<cudaStream_t>(stream));
 }
 
 int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv, int head_dim,
                          int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
                          const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
-                         int key_block, int* blocks, int* counts, void* stream) {
+                         int key_block, int* blocks, int* counts, void* workspace, size_t workspace_bytes,
+                         void* stream) {
   return block_select(q_means, k_means, batch, heads_q, heads_kv, head_dim, q_blocks, k_blocks, keep, allowed,
-                      allowed_strides, q_len, query_block, k_len, key_block, blocks, counts, stream);
+                      allowed_strides, q_len, query_block, k_len, key_block, blocks, counts, workspace, workspace_bytes,
+                      stream);
+}
+
+size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv, int q_blocks, int k_blocks) {
+  if (batch <= 0 || heads_q <= 0 || heads_kv <= 0 || q_blocks <= 0 || k_blocks <= 0) return 0;
+  return size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, q_blocks, k_blocks)) * sizeof(float);
 }
 
 size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block) {
@@ -1234,7 +1251,7 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
   from.after_means = n > 0;
   if (int rc = block_select(q_means, c->key_means ? c->key_means : k_means, batch, hq, hk, dim, int(s.q_blocks),
                             int(s.k_blocks), keep, c->allowed, c->allowed_strides, c->q_len, qb, c->k_len, kb, blocks,
-                            counts, stream, from))
+                            counts, base + s.scores, s.scores_bytes, stream, from))
     return rc;
   return sparse_attn(c->q, c->q_strides, c->k, c->k_strides, c->v, c->v_strides, c->out, c->out_strides, dtype, batch,
                      hq, hk, dim, lq, lk, blocks, counts, keep, qb, kb, c->q_len, c->k_len,

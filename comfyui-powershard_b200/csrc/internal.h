@@ -183,10 +183,20 @@ struct MeansArgs {
 };
 int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream);
 
-constexpr size_t kSelectSmemLimit = 200 * 1024;
 constexpr int kSelectMaxBlocks = 16384;  // 12 bytes of shared memory each
+// Pairs of batch row and key head whose scores are held at a time, in at most 64 MB where one fits in that.
+inline int select_units(int64_t batch, int64_t kv_heads, int64_t group, int64_t q_blocks, int64_t k_blocks) {
+  const int64_t one = group * q_blocks * k_blocks * 4;
+  int64_t n = (int64_t(64) << 20) / (one > 0 ? one : 1);
+  n = n < 1 ? 1 : (n > 65535 ? 65535 : n);
+  return static_cast<int>(n < batch * kv_heads ? n : batch * kv_heads);
+}
+// Workspace of launch_block_select: the scores of those pairs, and the key means' squared lengths.
+inline int64_t select_score_floats(int64_t batch, int64_t kv_heads, int64_t group, int64_t q_blocks, int64_t k_blocks) {
+  return select_units(batch, kv_heads, group, q_blocks, k_blocks) * (group * q_blocks + 1) * k_blocks;
+}
 struct SelectArgs {
-  const float* q_means;    // [batch][q_blocks][kv_heads * group][128]
+  float* q_means;          // [batch][q_blocks][kv_heads * group][128]
   const float* k_means;    // [batch][k_blocks][kv_heads][128]
   int batch, kv_heads, group, q_blocks, k_blocks, keep;
   int query_block, key_block;
@@ -196,9 +206,11 @@ struct SelectArgs {
   int64_t allowed_st[4];
   int* blocks;             // [batch][heads][q_blocks][keep]
   int* counts;             // [batch][heads][q_blocks]
-  int rows_per_cta;        // set by the launch
-  // Queries [batch][len_q][kv_heads * group][128] (16-bit) whose means the kernel takes itself, in the
-  // place of q_means, or null.
+  float* scores;           // workspace: [units at a time][group * q_blocks][k_blocks]
+  float* k_sq;             // ... and behind it [units at a time][k_blocks]
+  int first_unit;          // set by the launch
+  // Queries [batch][len_q][kv_heads * group][128] (16-bit) whose means the kernel takes itself and writes
+  // to q_means, or null.
   const void* q;
   int64_t q_st[3];         // batch, row, head strides in elements
   int len_q;

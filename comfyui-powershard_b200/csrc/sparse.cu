@@ -23,6 +23,8 @@ namespace sparse {
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kScoreRows = 64, kScoreKeys = 16 * kWarps;  // of one CTA of score_kernel
+constexpr int kPickThreads = 128, kPickWarps = kPickThreads / 32;
 
 template <bool kFp16>
 __device__ __forceinline__ void add8(float (&a)[8], const uint4& v) {
@@ -128,28 +130,183 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The keep-th largest of n keys (of those above 0, more than keep), by
-// bisection of their range: `floor` and how many that equal floor + 1 belong
-// to it are returned so that chosen = above floor + 1, plus the first `ties`
-// equal to it; ties 0: all above floor.  It ends as soon as exactly `keep` lie
-// above the middle (10 to 20 counts for scores that differ).
+__device__ __forceinline__ int blocks_in_use(const int* len, int batch, int block, int blocks) {
+  if (!len) return blocks;
+  const int64_t n = max(len[batch], 0);
+  return static_cast<int>(min(static_cast<int64_t>(blocks), (n + block - 1) / block));
+}
+
+// Scores of 64 rows (query blocks of the query heads that share a key head; one
+// list each) against 128 key blocks, and the squared lengths of the key means.
+//
+// On the tensor cores: each mean is split into two tf32 terms and the three
+// larger products are summed in 32 bits, which is off by less than E = 2^-16
+// |q| max |k| (the dropped terms are 3 * 2^-20 |q||k|, 16 sums of the main
+// products, nine terms each, keep 24 bits of their largest: 2^-16.8; the sums
+// of the small products are 2^-10 of that) plus what may underflow.
+// pick_kernel turns to 64 bits where that decides.
+//
+// A tile is 16 key blocks x 8 rows.  The order of the 128 products is free, so
+// a thread loads 16 bytes of a mean and uses them in two k-steps: a warp's 16
+// key means go from L2 to registers once for all 64 rows.
+__global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) {
+  constexpr int kPad = kHeadDim + 4;
+  __shared__ __align__(16) float qs[kScoreRows * kPad];
+  launch_dependents();
+  wait_for_previous();  // the means
+  const int rows = a.group * a.q_blocks;  // of one key head
+  const int kv = (a.first_unit + blockIdx.z) % a.kv_heads;
+  const int batch = (a.first_unit + blockIdx.z) / a.kv_heads;
+  const int heads = a.kv_heads * a.group;
+  const int row0 = blockIdx.y * kScoreRows;
+  const int rows_here = min(kScoreRows, rows - row0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, tig = lane & 3;
+  const int k_blocks = blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks);
+
+  // The warp's key means, while the queries' are put in shared memory.
+  const int n0 = blockIdx.x * kScoreKeys + warp * 16 + g;
+  const float4* km = reinterpret_cast<const float4*>(a.k_means) +
+                     (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4) + tig;
+  float4 v[2][8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[i][j] = n0 + 8 * i < k_blocks
+                    ? __ldg(km + static_cast<int64_t>(n0 + 8 * i) * a.kv_heads * (kHeadDim / 4) + 4 * j)
+                    : make_float4(0, 0, 0, 0);
+
+  for (int r = warp; r < (rows_here + 7) / 8 * 8; r += kWarps) {
+    const int row = row0 + r;
+    float4 m = make_float4(0, 0, 0, 0);
+    if (r < rows_here) {
+      const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
+      const int64_t at = ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane;
+      if (a.q) {  // few query rows: their mean is taken here
+        const int len = a.q_len ? min(max(a.q_len[batch], 0), a.len_q) : a.len_q;
+        const int n = min(max(len - qb * a.query_block, 0), a.query_block);
+        const uint16_t* x = static_cast<const uint16_t*>(a.q) + batch * a.q_st[0] +
+                            static_cast<int64_t>(qb) * a.query_block * a.q_st[1] + h * a.q_st[2] + 4 * lane;
+        double sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          const uint2 w2 = __ldg(reinterpret_cast<const uint2*>(x + i * a.q_st[1]));
+          const uint32_t w[2] = {w2.x, w2.y};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = a.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
+                                    : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+            sum[2 * e] += static_cast<double>(f.x);
+            sum[2 * e + 1] += static_cast<double>(f.y);
+          }
+        }
+        if (n) m = make_float4(float(sum[0] / n), float(sum[1] / n), float(sum[2] / n), float(sum[3] / n));
+        if (blockIdx.x == 0) reinterpret_cast<float4*>(a.q_means)[at] = m;
+      } else {
+        m = __ldg(reinterpret_cast<const float4*>(a.q_means) + at);
+      }
+    }
+    *reinterpret_cast<float4*>(&qs[r * kPad + 4 * lane]) = m;
+  }
+  __syncthreads();
+
+  const int64_t unit = blockIdx.z;
+  if (blockIdx.y == 0) {
+    float sq[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        sq[i] = fmaf(v[i][j].x, v[i][j].x, fmaf(v[i][j].y, v[i][j].y, fmaf(v[i][j].z, v[i][j].z,
+                fmaf(v[i][j].w, v[i][j].w, sq[i]))));
+      sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 1);
+      sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 2);
+      if (tig == 0 && n0 + 8 * i < a.k_blocks) a.k_sq[unit * a.k_blocks + n0 + 8 * i] = sq[i];
+    }
+  }
+  float* scores = a.scores + (unit * rows + row0) * a.k_blocks;
+#pragma unroll 1
+  for (int t = 0; t < rows_here; t += 8) {
+    float c[4] = {0, 0, 0, 0}, rest[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 qj = *reinterpret_cast<const float4*>(&qs[(t + g) * kPad + 16 * j + 4 * tig]);
+      const float qf[4] = {qj.x, qj.y, qj.z, qj.w};
+      const float f[2][4] = {{v[0][j].x, v[0][j].y, v[0][j].z, v[0][j].w},
+                             {v[1][j].x, v[1][j].y, v[1][j].z, v[1][j].w}};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t ah[4], al[4], bh[2], bl[2];
+        split_tf32(f[0][2 * u], ah[0], al[0]);
+        split_tf32(f[1][2 * u], ah[1], al[1]);
+        split_tf32(f[0][2 * u + 1], ah[2], al[2]);
+        split_tf32(f[1][2 * u + 1], ah[3], al[3]);
+        split_tf32(qf[2 * u], bh[0], bl[0]);
+        split_tf32(qf[2 * u + 1], bh[1], bl[1]);
+        mma_tf32(c, ah, bh[0], bh[1]);
+        mma_tf32(rest, al, bh[0], bh[1]);
+        mma_tf32(rest, ah, bl[0], bl[1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = t + 2 * tig + e;
+        if (r < rows_here && n0 + 8 * i < a.k_blocks)
+          scores[static_cast<int64_t>(r) * a.k_blocks + n0 + 8 * i] = c[2 * i + e] + rest[2 * i + e];
+      }
+  }
+}
+
+// Sums over the CTA; consecutive calls alternate between two halves of `part`.
+struct CtaSum {
+  int (*part)[kPickWarps];
+  int phase;
+  __device__ __forceinline__ int operator()(int v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    int* p = part[phase];
+    phase ^= 1;
+    if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWarps; ++w) total += p[w];
+    return total;
+  }
+};
+
+// The keep-th largest of the keys that are not 0 (more than keep): chosen are
+// those above floor + 1 and the first `ties` that equal it; ties 0: all above
+// floor.  `lo` and `hi` are the least and the greatest key, `n` how many.  The
+// range is cut where the counts at its ends put the keep-th on a straight line
+// (64-bit keys, and every third time: in the middle) until exactly `keep` lie
+// above the cut.
 template <typename Key>
-__device__ __forceinline__ void kth_largest(const Key* key, int n, int keep, Key lo, Key hi, int lane, Key& floor,
-                                            int& ties) {
-  int above = 0;  // keys above hi
+__device__ __forceinline__ void kth_largest(const Key* key, int begin, int end, int keep, Key lo, Key hi, int n,
+                                            CtaSum& sum, Key& floor, int& ties) {
+  const int lane = threadIdx.x & 31;
+  int above = 0;  // keys above hi; n: keys from lo up
   ties = 0;
-  while (lo < hi) {
-    const Key mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
+  for (int round = 1; lo < hi; ++round) {
+    Key mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
+    if constexpr (sizeof(Key) == 4) {
+      const float a = of_key(lo), b = of_key(hi);
+      const float f = a + (b - a) * (static_cast<float>(n - keep) / static_cast<float>(n - above));
+      if (round % 3 && isfinite(f)) mid = min(max(order_key(f), lo + 1), hi);
+    }
     int c = 0;
-#pragma unroll 8
-    for (int i = lane; i < n; i += 32) c += key[i] >= mid;
-    c = __reduce_add_sync(0xffffffffu, c);
+#pragma unroll 4
+    for (int i = begin + lane; i < end; i += 32) c += key[i] >= mid;
+    c = sum(c);
     if (c == keep) {
       floor = mid - 1;
       return;
     }
     if (c > keep) {
       lo = mid;
+      n = c;
     } else {
       hi = mid - 1;
       above = c;
@@ -159,329 +316,207 @@ __device__ __forceinline__ void kth_largest(const Key* key, int n, int keep, Key
   ties = keep - above;
 }
 
-// Writes a row's chosen indices in ascending order (one warp): keys above
-// floor + 1, and the first `ties` equal to it (ties 0: keys above floor).
+// Writes the chosen indices in ascending order; each warp has its range.
 template <typename Key>
-__device__ __forceinline__ void write_list(const Key* key, int n, Key floor, int ties, int keep, int* out, int* count,
-                                           int lane) {
+__device__ __forceinline__ void write_list(const Key* key, int begin, int end, Key floor, int ties, int keep, int* out,
+                                           int* count, int (*part)[kPickWarps]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned below = (1u << lane) - 1;
   const Key equal = floor + 1;
-  const bool tied = ties > 0;
-  int done = 0;
+  // Ahead of this warp's range: keys above the tied one, and tied ones.
+  int more = 0, same = 0;
 #pragma unroll 4
-  for (int n0 = 0; n0 < n; n0 += 32) {
-    const int i = n0 + lane;
-    const Key k = i < n ? key[i] : Key(0);
+  for (int i = begin + lane; i < end; i += 32) {
+    const Key k = key[i];
+    const bool tied = ties > 0 && k == equal;
+    same += tied;
+    more += k > floor && !tied;
+  }
+  more = __reduce_add_sync(0xffffffffu, more);
+  same = __reduce_add_sync(0xffffffffu, same);
+  __syncthreads();  // `part` may still be read
+  if (lane == 0) {
+    part[0][warp] = more;
+    part[1][warp] = same;
+  }
+  __syncthreads();
+  int done = 0, left = ties, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPickWarps; ++w) {
+    if (w == warp) {
+      done = total;
+      left = ties;
+    }
+    const int s = min(ties, part[1][w]);
+    total += part[0][w] + s;
+    ties -= s;
+  }
+  for (int i0 = begin; i0 < end; i0 += 32) {
+    const int i = i0 + lane;
+    const Key k = i < end ? key[i] : Key(0);
     bool take = k > floor;
-    if (tied) {
-      const unsigned m = __ballot_sync(0xffffffffu, take && k == equal);
-      if (take && k == equal) take = __popc(m & below) < ties;
-      ties -= min(ties, __popc(m));
+    if (same > 0) {  // of this warp's range
+      const bool tied = k == equal;
+      const unsigned m = __ballot_sync(0xffffffffu, tied);
+      if (tied) take = __popc(m & below) < left;
+      left -= min(left, __popc(m));
     }
     const unsigned m = __ballot_sync(0xffffffffu, take);
     if (take) out[done + __popc(m & below)] = i;
     done += __popc(m);
   }
-  for (int i = done + lane; i < keep; i += 32) out[i] = -1;
-  if (lane == 0) *count = done;
+  for (int i = total + threadIdx.x; i < keep; i += kPickThreads) out[i] = -1;
+  if (threadIdx.x == 0) *count = total;
 }
 
-// One CTA scores up to eight rows (query blocks of the query heads that share a
-// key head) against every key block, then a warp selects for each row.
-//
-// The scores are first taken on the tensor cores: each mean is split into two
-// tf32 terms and the three larger products are summed in 32 bits, which is off
-// by less than E = 2^-16 |q| max |k| (the dropped terms are 3 * 2^-20 |q||k|, 16
-// sums of the main products, nine terms each, keep 24 bits of their largest:
-// 2^-16.8; the sums of the small products are 2^-10 of that) plus what may
-// underflow.  With T the keep-th largest of these, a block above
-// T + 2E is chosen and one below T - 2E is not, in 64 bits too; only the blocks
-// between (the T block alone, in all but every few rows) are scored in 64 bits.
-// Measured at 75600 tokens, 5 heads, 1182 key blocks, 118 kept: all scores in
-// 64-bit FMAs 120 us (bound by their operands' shared-memory reads).
-//
-// Tiles are 16 key blocks x 8 rows.  The order of the 128 products is free, so
-// a thread loads 16 bytes of a mean and uses them in two products' k-steps: the
-// key means go from L2 to registers once per CTA, without shared memory.
-__global__ void __launch_bounds__(kThreads, 2) block_select_kernel(const SelectArgs a) {
+// One CTA picks one list.  With T the keep-th largest of the scores, a block
+// above T + 2E is chosen and one below T - 2E is not, in 64 bits too; only the
+// blocks between (the T block alone, in seven lists of eight) are scored again
+// in 64 bits.
+__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  unsigned long long* exact = reinterpret_cast<unsigned long long*>(smem);  // [k_blocks], for rows with many ties
-  uint32_t* keys = reinterpret_cast<uint32_t*>(exact + a.k_blocks);         // [rows_per_cta][k_blocks]
-  __shared__ __align__(16) float means[8][kHeadDim];  // of the queries
-  __shared__ uint32_t longest;      // bits of max |k|^2
-  __shared__ uint32_t redo[8];      // rows whose undecided blocks are many: lo key, or 0
-  __shared__ uint32_t redo_hi[8];
-
+  unsigned long long* exact = reinterpret_cast<unsigned long long*>(smem);  // [k_blocks], with many ties only
+  uint32_t* key = reinterpret_cast<uint32_t*>(exact + a.k_blocks);          // [k_blocks]
+  __shared__ int part[2][kPickWarps];
+  __shared__ uint32_t ends[3][kPickWarps];
+  __shared__ int open_at[32];
+  __shared__ unsigned long long open_key[32];
+  __shared__ int n_open;
   launch_dependents();
-  wait_for_previous();  // the means
-  const int rows = a.group * a.q_blocks;  // of one key head
-  const int chunks = (rows + a.rows_per_cta - 1) / a.rows_per_cta;
-  const int chunk = blockIdx.x % chunks;
-  const int kv = (blockIdx.x / chunks) % a.kv_heads;
-  const int batch = blockIdx.x / chunks / a.kv_heads;
+  wait_for_previous();  // the scores
+  const int rows = a.group * a.q_blocks;
+  const int unit = blockIdx.x / rows, row = blockIdx.x % rows;
+  const int kv = (a.first_unit + unit) % a.kv_heads, batch = (a.first_unit + unit) / a.kv_heads;
   const int heads = a.kv_heads * a.group;
-  const int row0 = chunk * a.rows_per_cta;
-  const int rows_here = min(a.rows_per_cta, rows - row0);
+  const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
+  const int64_t list = (static_cast<int64_t>(batch) * heads + h) * a.q_blocks + qb;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, tig = lane & 3;
+  const bool in_use = qb < blocks_in_use(a.q_len, batch, a.query_block, a.q_blocks);
+  const int n_used = in_use ? blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks) : 0;
+  // Each warp owns a quarter of the blocks, in whole 32s.
+  const int quarter = ((a.k_blocks + 31) / 32 + kPickWarps - 1) / kPickWarps * 32;
+  const int begin = min(warp * quarter, a.k_blocks), end = min(begin + quarter, a.k_blocks);
 
-  int k_blocks = a.k_blocks;
-  if (a.k_len) {
-    const int64_t len = max(a.k_len[batch], 0);
-    k_blocks = static_cast<int>(min(int64_t(k_blocks), (len + a.key_block - 1) / a.key_block));
-  }
-  int q_blocks = a.q_blocks;
-  if (a.q_len) {
-    const int64_t len = max(a.q_len[batch], 0);
-    q_blocks = static_cast<int>(min(int64_t(q_blocks), (len + a.query_block - 1) / a.query_block));
-  }
-  if (threadIdx.x == 0) longest = 0;
-  if (threadIdx.x < 8) redo[threadIdx.x] = 0;
-  if (warp < rows_here) {
-    const int row = row0 + warp;
-    const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
-    float4 m = make_float4(0, 0, 0, 0);
-    if (a.q) {  // few query rows: their mean is taken here
-      const int len = a.q_len ? min(max(a.q_len[batch], 0), a.len_q) : a.len_q;
-      const int n = min(max(len - qb * a.query_block, 0), a.query_block);
-      const uint16_t* x = static_cast<const uint16_t*>(a.q) + batch * a.q_st[0] +
-                          static_cast<int64_t>(qb) * a.query_block * a.q_st[1] + h * a.q_st[2] + 4 * lane;
-      double sum[4] = {0, 0, 0, 0};
+  const float4 q = __ldg(reinterpret_cast<const float4*>(a.q_means) +
+                         ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
+  const float* score = a.scores + (static_cast<int64_t>(unit) * rows + row) * a.k_blocks;
+  const float* k_sq = a.k_sq + static_cast<int64_t>(unit) * a.k_blocks;
+  const uint8_t* allowed = a.allowed ? a.allowed + batch * a.allowed_st[0] + h * a.allowed_st[1] + qb * a.allowed_st[2]
+                                     : nullptr;
+  uint32_t least = ~0u, most = 0, longest = 0;
+  int n_may = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(x + i * a.q_st[1]));
-        const uint32_t w[2] = {v.x, v.y};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 f = a.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
-                                  : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
-          sum[2 * e] += static_cast<double>(f.x);
-          sum[2 * e + 1] += static_cast<double>(f.y);
-        }
-      }
-      if (n) m = make_float4(float(sum[0] / n), float(sum[1] / n), float(sum[2] / n), float(sum[3] / n));
-    } else {
-      m = __ldg(reinterpret_cast<const float4*>(a.q_means) +
-                ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
+  for (int i = begin + lane; i < end; i += 32) {
+    uint32_t k = 0;
+    if (i < n_used && (!allowed || allowed[i * a.allowed_st[3]] != 0)) {
+      k = order_key(__ldg(score + i));
+      longest = max(longest, __float_as_uint(fabsf(__ldg(k_sq + i))));  // NaN is above inf
     }
-    reinterpret_cast<float4*>(means[warp])[lane] = m;
+    key[i] = k;
+    n_may += k != 0;
+    least = min(least, k - 1);  // 0 becomes the largest
+    most = max(most, k);
   }
-  __syncthreads();
-
-  auto q_mean = [&](int r) { return reinterpret_cast<const float4*>(means[r]); };  // of row r of this CTA
-  const float4* km = reinterpret_cast<const float4*>(a.k_means) +
-                     (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4);
-  const int64_t kstep = static_cast<int64_t>(a.kv_heads) * (kHeadDim / 4);
-
-  float q_sq = 0;  // |q|^2 of row g, after the sum over the four lanes that share it
-  {
-    float4 q[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      q[j] = g < rows_here ? q_mean(g)[4 * j + tig] : make_float4(0, 0, 0, 0);
-      q_sq = fmaf(q[j].x, q[j].x, fmaf(q[j].y, q[j].y, fmaf(q[j].z, q[j].z, fmaf(q[j].w, q[j].w, q_sq))));
-    }
-    // What each of this thread's two result columns (rows 2 tig, 2 tig + 1) may see.
-    const uint8_t* allowed[2] = {nullptr, nullptr};
-    bool in_use[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int r = 2 * tig + c, row = row0 + r;
-      in_use[c] = r < rows_here && row % a.q_blocks < q_blocks;
-      if (a.allowed && in_use[c])
-        allowed[c] = a.allowed + batch * a.allowed_st[0] + (kv * a.group + row / a.q_blocks) * a.allowed_st[1] +
-                     (row % a.q_blocks) * a.allowed_st[2];
-    }
-    uint32_t most = 0;
-    for (int t = warp * 16; t < a.k_blocks; t += kWarps * 16) {
-      float c[4] = {0, 0, 0, 0}, small[4] = {0, 0, 0, 0};
-      float sq[2] = {0, 0};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float4 v[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = t + g + 8 * i;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[i][j] = n < k_blocks ? __ldg(km + n * kstep + 4 * (4 * half + j) + tig) : make_float4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float f[2][4] = {{v[0][j].x, v[0][j].y, v[0][j].z, v[0][j].w},
-                                 {v[1][j].x, v[1][j].y, v[1][j].z, v[1][j].w}};
-          const float4 qj = q[4 * half + j];
-          const float qf[4] = {qj.x, qj.y, qj.z, qj.w};
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t ah[4], al[4], bh[2], bl[2];
-            split_tf32(f[0][2 * u], ah[0], al[0]);
-            split_tf32(f[1][2 * u], ah[1], al[1]);
-            split_tf32(f[0][2 * u + 1], ah[2], al[2]);
-            split_tf32(f[1][2 * u + 1], ah[3], al[3]);
-            split_tf32(qf[2 * u], bh[0], bl[0]);
-            split_tf32(qf[2 * u + 1], bh[1], bl[1]);
-            mma_tf32(c, ah, bh[0], bh[1]);
-            mma_tf32(small, al, bh[0], bh[1]);
-            mma_tf32(small, ah, bl[0], bl[1]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              sq[i] = fmaf(f[i][2 * u], f[i][2 * u], fmaf(f[i][2 * u + 1], f[i][2 * u + 1], sq[i]));
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] += small[i];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 1);
-        sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 2);
-        most = max(most, __float_as_uint(fabsf(sq[i])));  // NaN is above inf
-        const int n = t + g + 8 * i;
-        if (n >= a.k_blocks) continue;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (2 * tig + e >= rows_here) continue;
-          const bool may = in_use[e] && n < k_blocks && (!allowed[e] || allowed[e][n * a.allowed_st[3]] != 0);
-          keys[(2 * tig + e) * a.k_blocks + n] = may ? order_key(c[2 * i + e]) : 0u;
-        }
-      }
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) atomicMax(&longest, most);
-    q_sq += __shfl_xor_sync(0xffffffffu, q_sq, 1);
-    q_sq += __shfl_xor_sync(0xffffffffu, q_sq, 2);
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0) {
+    ends[0][warp] = least;
+    ends[1][warp] = most;
+    ends[2][warp] = longest;
   }
-  __syncthreads();
-
-  auto list_of = [&](int r) {
-    const int row = row0 + r;
-    return (static_cast<int64_t>(batch) * heads + kv * a.group + row / a.q_blocks) * a.q_blocks + row % a.q_blocks;
-  };
-  if (warp < rows_here) {
-    const int r = warp;
-    uint32_t* key = keys + r * a.k_blocks;
-    const int64_t list = list_of(r);
-    uint32_t least = ~0u, most = 0;
-    int n_may = 0;
-#pragma unroll 8
-    for (int n = lane; n < a.k_blocks; n += 32) {
-      const uint32_t k = key[n];
-      n_may += k != 0;
-      least = min(least, k - 1);  // 0 becomes the largest
-      most = max(most, k);
-    }
-    n_may = __reduce_add_sync(0xffffffffu, n_may);
-    uint32_t floor = 0;
-    bool settled = true;
-    if (n_may > a.keep) {
-      least = __reduce_min_sync(0xffffffffu, least) + 1;
-      most = __reduce_max_sync(0xffffffffu, most);
-      int ties;
-      kth_largest(key, a.k_blocks, a.keep, least, most, lane, floor, ties);
-      // T: the smallest key above floor.
-      uint32_t kth = ~0u;
-#pragma unroll 8
-      for (int n = lane; n < a.k_blocks; n += 32) {
-        const uint32_t k = key[n];
-        if (k > floor) kth = min(kth, k);
-      }
-      kth = __reduce_min_sync(0xffffffffu, kth);
-      const float T = of_key(kth);
-      const float len_q = sqrtf(__shfl_sync(0xffffffffu, q_sq, 4 * r));
-      const float len_k = sqrtf(__uint_as_float(longest));
-      const float E2 = 3.0517578125e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-15, 2^-110
-      uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
-      if (kth < ~0u - 1 && isfinite(T - E2) && isfinite(T + E2)) {
-        lo_key = order_key(T - E2);
-        hi_key = order_key(T + E2);
-      }
-      int sure = 0, open = 0;
-#pragma unroll 8
-      for (int n = lane; n < a.k_blocks; n += 32) {
-        const uint32_t k = key[n];
-        sure += k > hi_key;
-        open += k >= lo_key && k <= hi_key;
-      }
-      sure = __reduce_add_sync(0xffffffffu, sure);
-      open = __reduce_add_sync(0xffffffffu, open);
-      const int wanted = a.keep - sure;
-      if (open == wanted) {
-        floor = lo_key - 1;
-      } else if (open <= 32) {
-        // Lane i takes the i-th undecided block, in the order of their indices.
-        int mine = -1, seen = 0;
-        for (int n0 = 0; n0 < a.k_blocks && seen < open; n0 += 32) {
-          const uint32_t k = n0 + lane < a.k_blocks ? key[n0 + lane] : 0u;
-          unsigned m = __ballot_sync(0xffffffffu, k >= lo_key && k <= hi_key);
-          for (; m; m &= m - 1, ++seen)
-            if (lane == seen) mine = n0 + __ffs(m) - 1;
-        }
-        const float4 qv = q_mean(r)[lane];
-        unsigned long long score = 0;
-        for (int e = 0; e < open; ++e) {
-          const float4 kk = __ldg(km + __shfl_sync(0xffffffffu, mine, e) * kstep + lane);
-          double d = fma(double(qv.x), double(kk.x), double(qv.y) * double(kk.y)) +
-                     fma(double(qv.z), double(kk.z), double(qv.w) * double(kk.w));
+  if (threadIdx.x == 0) n_open = 0;
+  CtaSum sum{part, 0};
+  n_may = sum(n_may);  // and a barrier
 #pragma unroll
-          for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-          if (lane == e) score = order_key(d);
-        }
-        int better = 0;
-        for (int e = 0; e < open; ++e) {
-          const unsigned long long other = __shfl_sync(0xffffffffu, score, e);
-          better += other > score || (other == score && e < lane);
-        }
-        __syncwarp();
-        if (lane < open) key[mine] = better < wanted ? ~0u : 0u;
-        __syncwarp();
-        floor = hi_key;
-      } else {
-        settled = false;
-        if (lane == 0) {
-          redo[r] = lo_key;
-          redo_hi[r] = hi_key;
-        }
-      }
-    }
-    if (settled) write_list(key, a.k_blocks, floor, 0, a.keep, a.blocks + list * a.keep, a.counts + list, lane);
+  for (int w = 0; w < kPickWarps; ++w) {
+    least = min(least, ends[0][w]);
+    most = max(most, ends[1][w]);
+    longest = max(longest, ends[2][w]);
   }
-  __syncthreads();
-  // Rows with more than 32 undecided blocks (equal or overflowing scores): the
-  // CTA scores them in 64 bits, one warp selects.
-  for (int r = 0; r < rows_here; ++r) {
-    const uint32_t lo_key = redo[r], hi_key = redo_hi[r];
-    if (!lo_key) continue;
-    const float4* q = q_mean(r);
-    for (int n = threadIdx.x; n < a.k_blocks; n += kThreads) {
-      const uint32_t k = keys[r * a.k_blocks + n];
-      unsigned long long e = k > hi_key ? ~0ull : 0ull;
+  ++least;
+
+  int* out = a.blocks + list * a.keep;
+  uint32_t floor = 0;
+  if (n_may > a.keep) {
+    int ties;
+    kth_largest(key, begin, end, a.keep, least, most, n_may, sum, floor, ties);
+    uint32_t kth = ~0u;  // T: the smallest key above floor
+#pragma unroll 4
+    for (int i = begin + lane; i < end; i += 32) kth = key[i] > floor ? min(kth, key[i]) : kth;
+    kth = __reduce_min_sync(0xffffffffu, kth);
+    float q_sq = fmaf(q.x, q.x, fmaf(q.y, q.y, fmaf(q.z, q.z, q.w * q.w)));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) q_sq += __shfl_xor_sync(0xffffffffu, q_sq, o);
+    if (lane == 0) ends[0][warp] = kth;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPickWarps; ++w) kth = min(kth, ends[0][w]);
+    const float T = of_key(kth);
+    const float len_q = sqrtf(q_sq), len_k = sqrtf(__uint_as_float(longest));
+    const float E2 = 3.0517578125e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-15, 2^-110
+    uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
+    if (kth < ~0u - 1 && isfinite(T - E2) && isfinite(T + E2)) {
+      lo_key = order_key(T - E2);
+      hi_key = order_key(T + E2);
+    }
+    int sure = 0;
+#pragma unroll 4
+    for (int i = begin + lane; i < end; i += 32) {
+      const uint32_t k = key[i];
+      sure += k > hi_key;
       if (k >= lo_key && k <= hi_key) {
-        double d = 0;
-        for (int u = 0; u < kHeadDim / 4; ++u) {
-          const float4 x = q[u], y = __ldg(km + n * kstep + u);
-          d = fma(double(x.x), double(y.x), d);
-          d = fma(double(x.y), double(y.y), d);
-          d = fma(double(x.z), double(y.z), d);
-          d = fma(double(x.w), double(y.w), d);
-        }
-        e = order_key(d);
+        const int at = atomicAdd(&n_open, 1);  // in any order: they are ranked below
+        if (at < 32) open_at[at] = i;
       }
-      exact[n] = e;
     }
-    __syncthreads();
-    if (warp == 0) {
-      unsigned long long floor;
-      int ties;
-      kth_largest(exact, a.k_blocks, a.keep, 1ull, ~0ull, lane, floor, ties);
-      const int64_t list = list_of(r);
-      write_list(exact, a.k_blocks, floor, ties, a.keep, a.blocks + list * a.keep, a.counts + list, lane);
+    const int wanted = a.keep - sum(sure);
+    const int open = n_open;
+    const float4* km = reinterpret_cast<const float4*>(a.k_means) +
+                       (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4);
+    const int64_t kstep = static_cast<int64_t>(a.kv_heads) * (kHeadDim / 4);
+    auto score64 = [&](int i) {  // by one warp
+      const float4 k = __ldg(km + i * kstep + lane);
+      double d = fma(double(q.x), double(k.x), double(q.y) * double(k.y)) +
+                 fma(double(q.z), double(k.z), double(q.w) * double(k.w));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      return order_key(d);
+    };
+    if (open == wanted) {
+      floor = lo_key - 1;
+    } else if (open <= 32) {
+      for (int e = warp; e < open; e += kPickWarps) {
+        const unsigned long long k = score64(open_at[e]);
+        if (lane == 0) open_key[e] = k;
+      }
+      __syncthreads();
+      if (threadIdx.x < open) {
+        const int at = open_at[threadIdx.x];
+        const unsigned long long mine = open_key[threadIdx.x];
+        int better = 0;
+        for (int e = 0; e < open; ++e) better += open_key[e] > mine || (open_key[e] == mine && open_at[e] < at);
+        key[at] = better < wanted ? ~0u : 0u;
+      }
+      __syncthreads();
+      floor = hi_key;
+    } else {
+      // Many equal or overflowing scores: all of them in 64 bits.
+      for (int i = begin; i < end; ++i) {
+        const uint32_t k = key[i];
+        unsigned long long e = k > hi_key ? ~0ull : 0ull;
+        if (k >= lo_key && k <= hi_key) e = score64(i);
+        if (lane == 0) exact[i] = e;
+      }
+      __syncthreads();
+      unsigned long long floor64;
+      kth_largest(exact, begin, end, a.keep, 1ull, ~0ull, n_may, sum, floor64, ties);
+      write_list(exact, begin, end, floor64, ties, a.keep, out, a.counts + list, part);
+      return;
     }
-    __syncthreads();
   }
+  write_list(key, begin, end, floor, 0, a.keep, out, a.counts + list, part);
 }
-
-inline size_t select_smem(int rows, int k_blocks) { return size_t(k_blocks) * (8 + 4 * size_t(rows)); }
 
 }  // namespace sparse
 
@@ -502,24 +537,32 @@ int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream) {
 
 int launch_block_select(SelectArgs a, cudaStream_t stream) {
   using namespace sparse;
+  const size_t smem = size_t(a.k_blocks) * 12;
   static bool done[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!done[dev]) {
-    const cudaError_t err = cudaFuncSetAttribute(block_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(kSelectSmemLimit));
+    const cudaError_t err = cudaFuncSetAttribute(pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSelectMaxBlocks * 12);
     if (err != cudaSuccess) return set_cuda_error("block_select: cudaFuncSetAttribute", err);
     done[dev] = true;
   }
-  // Eight rows share a CTA's reads of the key means where their keys fit shared memory.
-  a.rows_per_cta = select_smem(8, a.k_blocks) <= kSelectSmemLimit ? 8 : 1;
-  const int64_t chunks = (int64_t(a.group) * a.q_blocks + a.rows_per_cta - 1) / a.rows_per_cta;
-  const int64_t ctas = chunks * a.kv_heads * a.batch;
-  if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^31 lists");
-  const cudaError_t err = launch_after(block_select_kernel, dim3(static_cast<unsigned>(ctas)), dim3(kThreads),
-                                       select_smem(a.rows_per_cta, a.k_blocks), stream, a.after_means, a);
-  if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
-  count_launch();
+  const int64_t rows = int64_t(a.group) * a.q_blocks;
+  const int64_t row_chunks = (rows + kScoreRows - 1) / kScoreRows;
+  if (row_chunks > 65535) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^22 lists a key head");
+  const int units = a.batch * a.kv_heads;
+  const int step = select_units(a.batch, a.kv_heads, a.group, a.q_blocks, a.k_blocks);
+  for (a.first_unit = 0; a.first_unit < units; a.first_unit += step) {
+    const int n = units - a.first_unit < step ? units - a.first_unit : step;
+    const dim3 grid(static_cast<unsigned>((a.k_blocks + kScoreKeys - 1) / kScoreKeys), static_cast<unsigned>(row_chunks),
+                    static_cast<unsigned>(n));
+    cudaError_t err = launch_after(score_kernel, grid, dim3(kThreads), 0, stream, a.after_means && a.first_unit == 0, a);
+    if (err != cudaSuccess) return set_cuda_error("block_select scores launch", err);
+    count_launch();
+    err = launch_after(pick_kernel, dim3(static_cast<unsigned>(n * rows)), dim3(kPickThreads), smem, stream, true, a);
+    if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
+    count_launch();
+  }
   return 0;
 }
 

@@ -736,11 +736,13 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
         if allowed.dtype != torch.bool or tuple(allowed.shape) != (batch, hq, nq, nk) or allowed.device != device:
             raise ValueError(f"block_select: allowed must be bool {(batch, hq, nq, nk)} on {device}")
         mask, strides = allowed.data_ptr(), _lib.i64(allowed.stride())
+    n = lib.ps_b200_block_select_workspace_bytes(batch, hq, hk, nq, nk) if hk else 0
+    workspace = torch.empty(n, dtype=torch.uint8, device=device)
     rc = lib.ps_b200_block_select(
         q_means.data_ptr(), k_means.data_ptr(), batch, hq, hk, dim, nq, nk, keep, mask, strides,
         _lengths_arg(query_lengths, batch, device, "block_select query_lengths"), query_block,
         _lengths_arg(key_lengths, batch, device, "block_select key_lengths"), key_block, blocks.data_ptr(),
-        counts.data_ptr(), _lib.stream_handle(device))
+        counts.data_ptr(), workspace.data_ptr(), n, _lib.stream_handle(device))
     _lib.check(rc, "ps_b200_block_select")
 
 

@@ -445,12 +445,16 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
  *   behind them are never chosen, query blocks behind them choose none.  A
  *   score of NaN ranks above all numbers.  blocks [batch][heads_q][q_blocks]
  *   [keep]: the chosen in ascending order, -1 behind them; counts
- *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 16384.
+ *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 16384.  workspace: device
+ *   scratch (16-byte aligned) of ps_b200_block_select_workspace_bytes(...) bytes,
+ *   owned by one call at a time.
  */
 int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv,
                          int head_dim, int q_blocks, int k_blocks, int keep, const unsigned char* allowed,
                          const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
-                         int key_block, int* blocks, int* counts, void* stream);
+                         int key_block, int* blocks, int* counts, void* workspace, size_t workspace_bytes,
+                         void* stream);
+size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv, int q_blocks, int k_blocks);
 
 /*
  * ps_b200_sparse_attn_fwd: softmax attention of each block of query_block rows

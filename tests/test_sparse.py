@@ -157,15 +157,16 @@ def test_entries_validate_on_the_host():
     assert whole(dim=64) == _lib.ERR_UNSUPPORTED and whole(kb=32) == _lib.ERR_UNSUPPORTED
     assert whole(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED
 
-    def select(heads=2, kv=2, dim=128, nq=2, nk=5, keep=3, means=16, lists=16):
+    def select(heads=2, kv=2, dim=128, nq=2, nk=5, keep=3, means=16, lists=16, ws=16, nbytes=1 << 20):
         return lib.ps_b200_block_select(means, 16, 1, heads, kv, dim, nq, nk, keep, None, None, None, 256, None, 64,
-                                        lists, 16, None)
+                                        lists, 16, ws, nbytes, None)
 
     assert select(keep=0) == _lib.ERR_INVALID and select(keep=6) == _lib.ERR_INVALID
     assert select(heads=3) == _lib.ERR_INVALID and select(dim=64) == _lib.ERR_UNSUPPORTED
     assert select(nk=30000) == _lib.ERR_UNSUPPORTED and b"larger blocks" in lib.ps_b200_last_error()
     assert select(means=20) == _lib.ERR_INVALID and select(lists=None) == _lib.ERR_INVALID
     assert select(nq=0) == _lib.OK
+    assert select(ws=None) == _lib.ERR_INVALID and select(nbytes=8) == _lib.ERR_INVALID
 
     def means(n=1, dtype=_lib.BF16, dim=128, block=64, length=100, x=16, stride=128):
         return lib.ps_b200_block_means(n, _lib.ptrs([x]), _lib.i64([0, stride, 128]), dtype, 1, _lib.i32([length]),
