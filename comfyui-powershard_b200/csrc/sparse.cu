@@ -23,8 +23,8 @@ namespace sparse {
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kFewBlocks = 4096;  // up to which two warps pick a list, eight beyond
 constexpr int kScoreRows = 64, kScoreKeys = 16 * kWarps;  // of one CTA of score_kernel
-constexpr int kPickThreads = 128, kPickWarps = kPickThreads / 32;
 
 template <bool kFp16>
 __device__ __forceinline__ void add8(float (&a)[8], const uint4& v) {
@@ -115,17 +115,15 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
-// x = hi + lo: the upper 10 bits of the mantissa, and the rest, of which the
-// product drops what is below its own 10 (both by truncation, without a
-// conversion: those run at 16 a clock and SM).
-__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  hi = __float_as_uint(x) & 0xffffe000u;
-  lo = __float_as_uint(x - __uint_as_float(hi));
+// x = hi + lo + at most 2^-18 x, two bf16 numbers; pairs of them packed for the tensor cores.
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16x2(x, y);
+  lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -139,19 +137,22 @@ __device__ __forceinline__ int blocks_in_use(const int* len, int batch, int bloc
 // Scores of 64 rows (query blocks of the query heads that share a key head; one
 // list each) against 128 key blocks, and the squared lengths of the key means.
 //
-// On the tensor cores: each mean is split into two tf32 terms and the three
-// larger products are summed in 32 bits, which is off by less than E = 2^-16
-// |q| max |k| (the dropped terms are 3 * 2^-20 |q||k|, 16 sums of the main
-// products, nine terms each, keep 24 bits of their largest: 2^-16.8; the sums
-// of the small products are 2^-10 of that) plus what may underflow.
-// pick_kernel turns to 64 bits where that decides.
+// On the tensor cores: each mean is split into two bf16 terms and the three
+// larger products are summed in 32 bits, which is off by less than E = 2^-15
+// |q| max |k| (the terms leave 2 * 2^-18, the dropped product 2^-18; 8 sums of
+// the main products, 17 terms each, keep 24 bits of their largest: 2^-16.9; the
+// sums of the small products are 2^-8 of that) plus what may underflow.
+// pick_kernel turns to 64 bits where that decides.  (Two tf32 terms are closer,
+// but take twice the products and, split between them, six times the other
+// arithmetic: 24 against MEASURED_SCORE us for 1182 key blocks and 296 query
+// blocks of 5 heads.)
 //
 // A tile is 16 key blocks x 8 rows.  The order of the 128 products is free, so
-// a thread loads 16 bytes of a mean and uses them in two k-steps: a warp's 16
-// key means go from L2 to registers once for all 64 rows.
+// a thread loads 16 bytes of a mean for one k-step of 16; a warp's 16 key means
+// go from L2 to registers once, split, for all 64 rows.
 __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) {
-  constexpr int kPad = kHeadDim + 4;
-  __shared__ __align__(16) float qs[kScoreRows * kPad];
+  constexpr int kPad = 32 + 4;  // of a row's 32 (hi, hi, lo, lo): 8 lanes' reads fall in different banks
+  __shared__ uint4 qs[kScoreRows * kPad];
   launch_dependents();
   wait_for_previous();  // the means
   const int rows = a.group * a.q_blocks;  // of one key head
@@ -168,14 +169,28 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
   const int n0 = blockIdx.x * kScoreKeys + warp * 16 + g;
   const float4* km = reinterpret_cast<const float4*>(a.k_means) +
                      (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4) + tig;
-  float4 v[2][8];
+  uint32_t kh[8][4], kl[8][4];
+  float sq[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int half = 0; half < 2; ++half) {
+    float4 v[2][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[i][j] = n0 + 8 * i < k_blocks
-                    ? __ldg(km + static_cast<int64_t>(n0 + 8 * i) * a.kv_heads * (kHeadDim / 4) + 4 * j)
-                    : make_float4(0, 0, 0, 0);
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        v[i][j] = n0 + 8 * i < k_blocks ? __ldg(km + static_cast<int64_t>(n0 + 8 * i) * a.kv_heads * (kHeadDim / 4) +
+                                                4 * (4 * half + j))
+                                        : make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 x = v[i][j];
+        sq[i] = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, fmaf(x.w, x.w, sq[i]))));
+        split_bf16(x.x, x.y, kh[4 * half + j][i], kl[4 * half + j][i]);
+        split_bf16(x.z, x.w, kh[4 * half + j][2 + i], kl[4 * half + j][2 + i]);
+      }
+  }
 
   for (int r = warp; r < (rows_here + 7) / 8 * 8; r += kWarps) {
     const int row = row0 + r;
@@ -207,47 +222,32 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
         m = __ldg(reinterpret_cast<const float4*>(a.q_means) + at);
       }
     }
-    *reinterpret_cast<float4*>(&qs[r * kPad + 4 * lane]) = m;
+    uint4 t;
+    split_bf16(m.x, m.y, t.x, t.z);
+    split_bf16(m.z, m.w, t.y, t.w);
+    qs[r * kPad + lane] = t;
   }
   __syncthreads();
 
   const int64_t unit = blockIdx.z;
   if (blockIdx.y == 0) {
-    float sq[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        sq[i] = fmaf(v[i][j].x, v[i][j].x, fmaf(v[i][j].y, v[i][j].y, fmaf(v[i][j].z, v[i][j].z,
-                fmaf(v[i][j].w, v[i][j].w, sq[i]))));
       sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 1);
       sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 2);
       if (tig == 0 && n0 + 8 * i < a.k_blocks) a.k_sq[unit * a.k_blocks + n0 + 8 * i] = sq[i];
     }
   }
   float* scores = a.scores + (unit * rows + row0) * a.k_blocks;
-#pragma unroll 1
+#pragma unroll 2
   for (int t = 0; t < rows_here; t += 8) {
     float c[4] = {0, 0, 0, 0}, rest[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float4 qj = *reinterpret_cast<const float4*>(&qs[(t + g) * kPad + 16 * j + 4 * tig]);
-      const float qf[4] = {qj.x, qj.y, qj.z, qj.w};
-      const float f[2][4] = {{v[0][j].x, v[0][j].y, v[0][j].z, v[0][j].w},
-                             {v[1][j].x, v[1][j].y, v[1][j].z, v[1][j].w}};
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t ah[4], al[4], bh[2], bl[2];
-        split_tf32(f[0][2 * u], ah[0], al[0]);
-        split_tf32(f[1][2 * u], ah[1], al[1]);
-        split_tf32(f[0][2 * u + 1], ah[2], al[2]);
-        split_tf32(f[1][2 * u + 1], ah[3], al[3]);
-        split_tf32(qf[2 * u], bh[0], bl[0]);
-        split_tf32(qf[2 * u + 1], bh[1], bl[1]);
-        mma_tf32(c, ah, bh[0], bh[1]);
-        mma_tf32(rest, al, bh[0], bh[1]);
-        mma_tf32(rest, ah, bl[0], bl[1]);
-      }
+      const uint4 b = qs[(t + g) * kPad + 4 * j + tig];
+      mma_bf16(c, kh[j], b.x, b.y);
+      mma_bf16(rest, kl[j], b.x, b.y);
+      mma_bf16(rest, kh[j], b.z, b.w);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -261,8 +261,9 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
 }
 
 // Sums over the CTA; consecutive calls alternate between two halves of `part`.
+template <int kWarps>
 struct CtaSum {
-  int (*part)[kPickWarps];
+  int (*part)[kWarps];
   int phase;
   __device__ __forceinline__ int operator()(int v) {
     v = __reduce_add_sync(0xffffffffu, v);
@@ -272,7 +273,7 @@ struct CtaSum {
     __syncthreads();
     int total = 0;
 #pragma unroll
-    for (int w = 0; w < kPickWarps; ++w) total += p[w];
+    for (int w = 0; w < kWarps; ++w) total += p[w];
     return total;
   }
 };
@@ -280,12 +281,13 @@ struct CtaSum {
 // The keep-th largest of the keys that are not 0 (more than keep): chosen are
 // those above floor + 1 and the first `ties` that equal it; ties 0: all above
 // floor.  `lo` and `hi` are the least and the greatest key, `n` how many.  The
-// range is cut where the counts at its ends put the keep-th on a straight line
-// (64-bit keys, and every third time: in the middle) until exactly `keep` lie
-// above the cut.
-template <typename Key>
+// range is cut first at `guess`, then where the counts at its ends put the
+// keep-th on a straight line, every fourth time (and for 64-bit keys) in the
+// middle, until exactly `keep` lie above the cut: 4.3 counts of 1182 normal
+// scores, against 15 with bisection of the keys alone.
+template <typename Key, int kWarps>
 __device__ __forceinline__ void kth_largest(const Key* key, int begin, int end, int keep, Key lo, Key hi, int n,
-                                            CtaSum& sum, Key& floor, int& ties) {
+                                            float guess, CtaSum<kWarps>& sum, Key& floor, int& ties) {
   const int lane = threadIdx.x & 31;
   int above = 0;  // keys above hi; n: keys from lo up
   ties = 0;
@@ -293,8 +295,9 @@ __device__ __forceinline__ void kth_largest(const Key* key, int begin, int end, 
     Key mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
     if constexpr (sizeof(Key) == 4) {
       const float a = of_key(lo), b = of_key(hi);
-      const float f = a + (b - a) * (static_cast<float>(n - keep) / static_cast<float>(n - above));
-      if (round % 3 && isfinite(f)) mid = min(max(order_key(f), lo + 1), hi);
+      const float f = round == 1 ? guess
+                                 : a + (b - a) * __fdividef(static_cast<float>(n - keep), static_cast<float>(n - above));
+      if ((round & 3) && isfinite(f)) mid = min(max(order_key(f), lo + 1), hi);
     }
     int c = 0;
 #pragma unroll 4
@@ -317,9 +320,9 @@ __device__ __forceinline__ void kth_largest(const Key* key, int begin, int end, 
 }
 
 // Writes the chosen indices in ascending order; each warp has its range.
-template <typename Key>
+template <typename Key, int kWarps>
 __device__ __forceinline__ void write_list(const Key* key, int begin, int end, Key floor, int ties, int keep, int* out,
-                                           int* count, int (*part)[kPickWarps]) {
+                                           int* count, int (*part)[kWarps]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned below = (1u << lane) - 1;
   const Key equal = floor + 1;
@@ -342,7 +345,7 @@ __device__ __forceinline__ void write_list(const Key* key, int begin, int end, K
   __syncthreads();
   int done = 0, left = ties, total = 0;
 #pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w == warp) {
       done = total;
       left = ties;
@@ -365,20 +368,22 @@ __device__ __forceinline__ void write_list(const Key* key, int begin, int end, K
     if (take) out[done + __popc(m & below)] = i;
     done += __popc(m);
   }
-  for (int i = total + threadIdx.x; i < keep; i += kPickThreads) out[i] = -1;
+  for (int i = total + threadIdx.x; i < keep; i += 32 * kWarps) out[i] = -1;
   if (threadIdx.x == 0) *count = total;
 }
 
 // One CTA picks one list.  With T the keep-th largest of the scores, a block
 // above T + 2E is chosen and one below T - 2E is not, in 64 bits too; only the
-// blocks between (the T block alone, in seven lists of eight) are scored again
-// in 64 bits.
-__global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) {
+// blocks between (the T block alone, in three lists of four) are scored again in
+// 64 bits.
+template <int kWarps>
+__global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned long long* exact = reinterpret_cast<unsigned long long*>(smem);  // [k_blocks], with many ties only
   uint32_t* key = reinterpret_cast<uint32_t*>(exact + a.k_blocks);          // [k_blocks]
-  __shared__ int part[2][kPickWarps];
-  __shared__ uint32_t ends[3][kPickWarps];
+  __shared__ int part[2][kWarps];
+  __shared__ uint32_t ends[3][kWarps];
+  __shared__ float sums[2][kWarps];
   __shared__ int open_at[32];
   __shared__ unsigned long long open_key[32];
   __shared__ int n_open;
@@ -393,9 +398,9 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool in_use = qb < blocks_in_use(a.q_len, batch, a.query_block, a.q_blocks);
   const int n_used = in_use ? blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks) : 0;
-  // Each warp owns a quarter of the blocks, in whole 32s.
-  const int quarter = ((a.k_blocks + 31) / 32 + kPickWarps - 1) / kPickWarps * 32;
-  const int begin = min(warp * quarter, a.k_blocks), end = min(begin + quarter, a.k_blocks);
+  // Each warp owns a range of the blocks, in whole 32s.
+  const int range = ((a.k_blocks + 31) / 32 + kWarps - 1) / kWarps * 32;
+  const int begin = min(warp * range, a.k_blocks), end = min(begin + range, a.k_blocks);
 
   const float4 q = __ldg(reinterpret_cast<const float4*>(a.q_means) +
                          ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
@@ -405,11 +410,15 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
                                      : nullptr;
   uint32_t least = ~0u, most = 0, longest = 0;
   int n_may = 0;
+  float s1 = 0, s2 = 0;  // sums of the scores and their squares
 #pragma unroll 4
   for (int i = begin + lane; i < end; i += 32) {
     uint32_t k = 0;
     if (i < n_used && (!allowed || allowed[i * a.allowed_st[3]] != 0)) {
-      k = order_key(__ldg(score + i));
+      const float x = __ldg(score + i);
+      k = order_key(x);
+      s1 += x;
+      s2 = fmaf(x, x, s2);
       longest = max(longest, __float_as_uint(fabsf(__ldg(k_sq + i))));  // NaN is above inf
     }
     key[i] = k;
@@ -420,16 +429,23 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
   longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+    s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+  }
   if (lane == 0) {
+    sums[0][warp] = s1;
+    sums[1][warp] = s2;
     ends[0][warp] = least;
     ends[1][warp] = most;
     ends[2][warp] = longest;
   }
   if (threadIdx.x == 0) n_open = 0;
-  CtaSum sum{part, 0};
+  CtaSum<kWarps> sum{part, 0};
   n_may = sum(n_may);  // and a barrier
 #pragma unroll
-  for (int w = 0; w < kPickWarps; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     least = min(least, ends[0][w]);
     most = max(most, ends[1][w]);
     longest = max(longest, ends[2][w]);
@@ -440,7 +456,17 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
   uint32_t floor = 0;
   if (n_may > a.keep) {
     int ties;
-    kth_largest(key, begin, end, a.keep, least, most, n_may, sum, floor, ties);
+    // Where the keep-th would lie if the scores were normal.
+    s1 = s2 = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      s1 += sums[0][w];
+      s2 += sums[1][w];
+    }
+    const float part_kept = __fdividef(static_cast<float>(a.keep), static_cast<float>(n_may));
+    s1 = __fdividef(s1, static_cast<float>(n_may));
+    const float spread = sqrtf(fmaxf(__fdividef(s2, static_cast<float>(n_may)) - s1 * s1, 0.f));
+    kth_largest(key, begin, end, a.keep, least, most, n_may, s1 - spread * normcdfinvf(part_kept), sum, floor, ties);
     uint32_t kth = ~0u;  // T: the smallest key above floor
 #pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) kth = key[i] > floor ? min(kth, key[i]) : kth;
@@ -451,10 +477,10 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
     if (lane == 0) ends[0][warp] = kth;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kPickWarps; ++w) kth = min(kth, ends[0][w]);
+    for (int w = 0; w < kWarps; ++w) kth = min(kth, ends[0][w]);
     const float T = of_key(kth);
     const float len_q = sqrtf(q_sq), len_k = sqrtf(__uint_as_float(longest));
-    const float E2 = 3.0517578125e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-15, 2^-110
+    const float E2 = 6.103515625e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-14, 2^-110
     uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
     if (kth < ~0u - 1 && isfinite(T - E2) && isfinite(T + E2)) {
       lo_key = order_key(T - E2);
@@ -486,7 +512,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
     if (open == wanted) {
       floor = lo_key - 1;
     } else if (open <= 32) {
-      for (int e = warp; e < open; e += kPickWarps) {
+      for (int e = warp; e < open; e += kWarps) {
         const unsigned long long k = score64(open_at[e]);
         if (lane == 0) open_key[e] = k;
       }
@@ -510,7 +536,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const SelectArgs a) 
       }
       __syncthreads();
       unsigned long long floor64;
-      kth_largest(exact, begin, end, a.keep, 1ull, ~0ull, n_may, sum, floor64, ties);
+      kth_largest(exact, begin, end, a.keep, 1ull, ~0ull, n_may, 0.f, sum, floor64, ties);
       write_list(exact, begin, end, floor64, ties, a.keep, out, a.counts + list, part);
       return;
     }
@@ -542,8 +568,10 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!done[dev]) {
-    const cudaError_t err = cudaFuncSetAttribute(pick_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kSelectMaxBlocks * 12);
+    cudaError_t err = cudaFuncSetAttribute(pick_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           kSelectMaxBlocks * 12);
+    if (err == cudaSuccess)
+      err = cudaFuncSetAttribute(pick_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewBlocks * 12);
     if (err != cudaSuccess) return set_cuda_error("block_select: cudaFuncSetAttribute", err);
     done[dev] = true;
   }
@@ -559,7 +587,9 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
     cudaError_t err = launch_after(score_kernel, grid, dim3(kThreads), 0, stream, a.after_means && a.first_unit == 0, a);
     if (err != cudaSuccess) return set_cuda_error("block_select scores launch", err);
     count_launch();
-    err = launch_after(pick_kernel, dim3(static_cast<unsigned>(n * rows)), dim3(kPickThreads), smem, stream, true, a);
+    const dim3 lists(static_cast<unsigned>(n * rows));
+    err = a.k_blocks <= kFewBlocks ? launch_after(pick_kernel<2>, lists, dim3(64), smem, stream, true, a)
+                                   : launch_after(pick_kernel<8>, lists, dim3(256), smem, stream, true, a);
     if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
     count_launch();
   }
