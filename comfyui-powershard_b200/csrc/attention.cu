@@ -451,31 +451,11 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const AttnArgs args) 
   void* const obase = pre ? args.pre_out : args.seg_out[seg];
   const int64_t* ost = pre ? args.pre_o_stride : args.o_stride;
   const int64_t otile = batch * ost[0] + static_cast<int64_t>(row0) * ost[2] + head * ost[3];
-  const int S = args.split;
   const int r = (blockIdx.x & 7) * 16 + (threadIdx.x >> 4);
   const int c = (threadIdx.x & 15) * 8;
   if (r < valid) {
-    float mx = -INFINITY;
-    for (int p = 0; p < S; ++p) mx = fmaxf(mx, args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r]);
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    float wsum = 0.f;
-    for (int p = 0; p < S; ++p) {
-      const float lse = args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r];
-      const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - mx);
-      wsum += w;
-      const float4* src = reinterpret_cast<const float4*>(
-          args.ws_o + ((static_cast<int64_t>(u * S + p) * 2 + t) * kBlockM + r) * kHeadDim + c);
-      const float4 a0 = src[0], a1 = src[1];
-      acc[0] = fmaf(w, a0.x, acc[0]);
-      acc[1] = fmaf(w, a0.y, acc[1]);
-      acc[2] = fmaf(w, a0.z, acc[2]);
-      acc[3] = fmaf(w, a0.w, acc[3]);
-      acc[4] = fmaf(w, a1.x, acc[4]);
-      acc[5] = fmaf(w, a1.y, acc[5]);
-      acc[6] = fmaf(w, a1.z, acc[6]);
-      acc[7] = fmaf(w, a1.w, acc[7]);
-    }
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+    float acc[8];
+    const float inv = merge_parts(args, u, t, r, c, acc);
     const int64_t oidx = otile + static_cast<int64_t>(r) * ost[2] + c;
     if (args.out_fp32) {
       float4* dst = reinterpret_cast<float4*>(static_cast<float*>(obase) + oidx);

@@ -187,5 +187,33 @@ __device__ __forceinline__ void softmax_row(const float (&s)[128], bool first, f
   mbar_arrive(bar_p);
 }
 
+// Merges the parts of split unit u for 8 columns from c of row r of its query
+// tile t: acc = sum_p w_p o_p with w_p = 2^(lse_p - max lse); returns 1 / sum_p w_p.
+__device__ __forceinline__ float merge_parts(const AttnArgs& args, int u, int t, int r, int c, float (&acc)[8]) {
+  const int S = args.split;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  float mx = -INFINITY;
+  for (int p = 0; p < S; ++p) mx = fmaxf(mx, args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r]);
+  float wsum = 0.f;
+  for (int p = 0; p < S; ++p) {
+    const float lse = args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r];
+    const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - mx);
+    wsum += w;
+    const float4* src = reinterpret_cast<const float4*>(
+        args.ws_o + ((static_cast<int64_t>(u * S + p) * 2 + t) * kBlockM + r) * kHeadDim + c);
+    const float4 a0 = src[0], a1 = src[1];
+    acc[0] = fmaf(w, a0.x, acc[0]);
+    acc[1] = fmaf(w, a0.y, acc[1]);
+    acc[2] = fmaf(w, a0.z, acc[2]);
+    acc[3] = fmaf(w, a0.w, acc[3]);
+    acc[4] = fmaf(w, a1.x, acc[4]);
+    acc[5] = fmaf(w, a1.y, acc[5]);
+    acc[6] = fmaf(w, a1.z, acc[6]);
+    acc[7] = fmaf(w, a1.w, acc[7]);
+  }
+  return wsum > 0.f ? 1.f / wsum : 0.f;
+}
+
 }  // namespace attn
 }  // namespace psb

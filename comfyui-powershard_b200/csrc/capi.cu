@@ -257,7 +257,8 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
 
 // How block-sparse attention is cut into CTAs: the last, partial wave's units
 // (query tile pair, head, batch) run as `split` CTAs each over parts of their
-// lists, at least two key tiles a part by the lists' full length.
+// lists, at least two key tiles a part by the lists' full length (one for few
+// queries, where a part is mostly waiting for its tiles).
 struct SparsePlan {
   int64_t units, rem;
   int split;
@@ -272,7 +273,8 @@ SparsePlan sparse_plan(int64_t batch, int64_t heads, int64_t len_q, int64_t list
   if (p.rem > 0) {
     const int64_t tiles = (list_len * key_block + 127) / 128;
     int64_t split = sms / p.rem;
-    split = split < tiles / 2 ? split : tiles / 2;
+    const int64_t most = len_q <= kMergeRows ? tiles : tiles / 2;
+    split = split < most ? split : most;
     split = split < kMaxSparseSplit ? split : kMaxSparseSplit;
     if (split >= 2) p.split = static_cast<int>(split);
   }
@@ -296,7 +298,8 @@ int check_blocks(int batch, int heads_q, int heads_kv, int head_dim, int query_b
 // Where one block-sparse call keeps what its three steps hand on, each on a 256-byte boundary.
 struct SparseScratch {
   int64_t q_blocks, k_blocks;
-  size_t q_means, k_means, blocks, counts, scores, scores_bytes, workspace, workspace_bytes, total;
+  size_t q_means, k_means, blocks, counts, scores, scores_bytes, workspace, workspace_bytes, tickets, total;
+  int64_t n_tickets;  // 0: the parts of split units are merged by a kernel of their own
 };
 
 SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t len_q, int64_t len_k,
@@ -318,8 +321,11 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   s.scores_bytes =
       size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, s.q_blocks, s.k_blocks)) * sizeof(float);
   s.scores = take(s.scores_bytes);
-  s.workspace_bytes = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count()).workspace_bytes();
+  const SparsePlan plan = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count());
+  s.workspace_bytes = plan.workspace_bytes();
   s.workspace = take(s.workspace_bytes);
+  s.n_tickets = plan.split > 1 && len_q <= kMergeRows ? 2 * plan.rem : 0;
+  s.tickets = take(s.n_tickets * sizeof(int));
   s.total = at;
   return s;
 }
@@ -1103,7 +1109,7 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
                        int batch, int heads_q, int heads_kv, int head_dim, int len_q, int len_k, const int* blocks,
                        const int* counts, int list_len, int query_block, int key_block, const int* q_len,
                        const int* k_len, float softmax_scale, void* workspace, size_t workspace_bytes, int* status,
-                       void* stream, bool after_select) {
+                       void* stream, bool after_select, int* tickets = nullptr) {
   if (!q_strides || !k_strides || !v_strides || !out_strides) return set_error(PS_B200_ERR_INVALID, "null strides");
   if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
   if (int rc = check_blocks(batch, heads_q, heads_kv, head_dim, query_block, key_block)) return rc;
@@ -1169,6 +1175,7 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
     a.full_units = static_cast<int>(plan.units - plan.rem);
     a.ws_o = static_cast<float*>(workspace);
     a.ws_lse = a.ws_o + plan.rem * plan.split * 2 * 128 * 128;
+    a.tickets = tickets;
   }
   return launch_sparse_attention(tq, tk, tv, a, plan.units, fp16, after_select, static_cast<cudaStream_t>(stream));
 }
@@ -1249,6 +1256,10 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
   if (n)
     if (int rc = ps_b200_block_means(n, x, st, dtype, batch, len, heads, dim, block, lens, means, stream)) return rc;
   from.after_means = n > 0;
+  if (s.n_tickets) {
+    from.zeros = reinterpret_cast<int*>(base + s.tickets);
+    from.n_zeros = int(s.n_tickets);
+  }
   if (int rc = block_select(q_means, c->key_means ? c->key_means : k_means, batch, hq, hk, dim, int(s.q_blocks),
                             int(s.k_blocks), keep, c->allowed, c->allowed_strides, c->q_len, qb, c->k_len, kb, blocks,
                             counts, base + s.scores, s.scores_bytes, stream, from))
@@ -1256,7 +1267,7 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
   return sparse_attn(c->q, c->q_strides, c->k, c->k_strides, c->v, c->v_strides, c->out, c->out_strides, dtype, batch,
                      hq, hk, dim, lq, lk, blocks, counts, keep, qb, kb, c->q_len, c->k_len,
                      static_cast<float>(c->softmax_scale), s.workspace_bytes ? base + s.workspace : nullptr,
-                     s.workspace_bytes, c->status, stream, true);
+                     s.workspace_bytes, c->status, stream, true, from.zeros);
 }
 
 static int cache_common(bool write, const ps_b200_cache_call* c, void* stream) {

@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, tig = lane & 3;
   const int k_blocks = blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks);
+  if (a.zeros && blockIdx.x + blockIdx.y + blockIdx.z == 0)
+    for (int i = threadIdx.x; i < a.n_zeros; i += kThreads) a.zeros[i] = 0;
 
   // The warp's key means, while the queries' are put in shared memory.
   const int n0 = blockIdx.x * kScoreKeys + warp * 16 + g;

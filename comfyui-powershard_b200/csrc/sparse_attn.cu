@@ -68,6 +68,7 @@ struct Work {
 struct Small {  // behind the barriers
   Work work[2];
   int meta[kRing];  // rows in use of a tile's lower 64 | upper 64 << 8
+  int last[2];      // whether this CTA wrote the last part of its unit's query tile t
   uint32_t tmem;
   int abort;
   __align__(16) int answer[4];
@@ -450,6 +451,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (row < rows) args.ws_lse[at] = live && l > 0.f ? m + __log2f(l) : -INFINITY;
         }
+        if (args.tickets) {
+          // Few rows: whichever part is written last merges them, in the order
+          // of the parts (a launch less: 3 us of a 25 us call).
+          const int split_unit = w.slot / args.split;
+          const int sub = threadIdx.x & 127;
+          __threadfence();
+          named_bar_sync(1 + t, 128);
+          if (sub == 0) small->last[t] = atomicAdd(&args.tickets[2 * split_unit + t], 1) == args.split - 1;
+          named_bar_sync(1 + t, 128);
+          if (small->last[t]) {
+            __threadfence();
+            uint16_t* out = static_cast<uint16_t*>(args.seg_out[0]) + c.batch * args.o_stride[0] +
+                            static_cast<int64_t>(row0) * args.o_stride[2] + c.head * args.o_stride[3];
+            const int col = (sub & 15) * 8;
+            for (int r = sub >> 4; r < rows; r += 8) {
+              float acc[8];
+              const float inv = merge_parts(args, split_unit, t, r, col, acc);
+              uint4 v;
+              v.x = pack2<kFp16>(acc[0] * inv, acc[1] * inv);
+              v.y = pack2<kFp16>(acc[2] * inv, acc[3] * inv);
+              v.z = pack2<kFp16>(acc[4] * inv, acc[5] * inv);
+              v.w = pack2<kFp16>(acc[6] * inv, acc[7] * inv);
+              *reinterpret_cast<uint4*>(out + r * args.o_stride[2] + col) = v;
+            }
+          }
+        }
       } else {
         // Each warp stages 64 columns of its 32 rows (row r, 16-byte chunk k at
         // r*128 + ((k ^ (r & 7)) << 4)), then 8 threads store 128 bytes of a row.
@@ -519,7 +546,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
                                        kSmem, stream, after_select, tq, tk, tv, args);
   if (err != cudaSuccess) return set_cuda_error("sparse attention launch", err);
   count_launch();
-  if (split_units > 0) return launch_combine(args, split_units, kFp16, true, stream);
+  if (split_units > 0 && !args.tickets) return launch_combine(args, split_units, kFp16, true, stream);
   return 0;
 }
 

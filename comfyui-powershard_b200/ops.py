@@ -791,6 +791,7 @@ def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: 
 
 # ps_b200_sparse_call: ten addresses, the strides, eleven sizes and the scale.
 _SPARSE_CALL = struct.Struct("@10P16q11qd")
+_NO_STRIDES = (0, 0, 0, 0)
 
 
 @functools.lru_cache(maxsize=256)
@@ -807,22 +808,27 @@ def sparse_forward(q, k, v, out, keep: int, query_block: int, key_block: int, sc
     What the steps hand on lives in one scratch buffer from the caching
     allocator, so concurrent calls and captured graphs each have their own."""
     lib = _lib.load()
-    device = q.device
+    device, dtype = q.device, q.dtype
     b, lq, hq, d = q.shape
-    lk, hk = k.shape[1], k.shape[2]
-    if allowed is not None and (allowed.dtype != torch.bool or allowed.device != device):
-        raise ValueError(f"sparse attention: allowed must be bool on {device}")
+    _, lk, hk, _ = k_shape = k.shape
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if (v.shape != k_shape or out.shape != q.shape or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype
+            or sq[3] != 1 or sk[3] != 1 or sv[3] != 1 or so[3] != 1):
+        raise ValueError("sparse attention: q/out [B, Lq, Hq, 128] and k/v [B, Lk, Hk, 128] need one dtype and a unit "
+                         f"inner stride, got {tuple(q.shape)}, {tuple(k_shape)}, {tuple(v.shape)}, {tuple(out.shape)}")
+    mask, sm = 0, _NO_STRIDES
+    if allowed is not None:
+        if allowed.dtype != torch.bool or allowed.device != device:
+            raise ValueError(f"sparse attention: allowed must be bool on {device}")
+        mask, sm = allowed.data_ptr(), allowed.stride()
     n = _sparse_scratch_bytes(device.index, b, hq, hk, lq, lk, keep, query_block, key_block, key_means is not None)
     scratch = torch.empty(n, dtype=torch.uint8, device=device)
     call = _SPARSE_CALL.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if key_means is None else key_means.data_ptr(),
-        0 if allowed is None else allowed.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if key_means is None else key_means.data_ptr(), mask,
         _lengths_arg(query_lengths, b, device, "sparse attention query_lengths") or 0,
         _lengths_arg(key_lengths, b, device, "sparse attention key_lengths") or 0, scratch.data_ptr(), status.ptr,
-        *_row_strides(q, "sparse attention q"), *_row_strides(k, "sparse attention k"),
-        *_row_strides(v, "sparse attention v"), *_row_strides(out, "sparse attention out"),
-        *((0, 0, 0, 0) if allowed is None else allowed.stride()), _lib.dtype_code(q.dtype), b, hq, hk, d, lq, lk, keep,
-        query_block, key_block, n, scale)
+        sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], so[0], so[1], so[2], *sm, _lib.dtype_code(dtype),
+        b, hq, hk, d, lq, lk, keep, query_block, key_block, n, scale)
     rc = lib.ps_b200_sparse_fwd(call, _lib.stream_handle(device))
     if rc:
         _lib.check(rc, "ps_b200_sparse_fwd")
