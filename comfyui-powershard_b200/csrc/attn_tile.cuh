@@ -99,9 +99,10 @@ struct TileMma {
     m.dv = sdesc_sw128(smem_u32(sV), kHalfTile, 1024);
     return m;
   }
-  // S_t = Q_t K^T with the K tile of stage st.
-  __device__ __forceinline__ void s(int t, int st) const {
-    const uint64_t dq = t ? dq1 : dq0;
+  // S_t = Q_q K^T with the K tile of stage st.
+  __device__ __forceinline__ void s(int t, int st) const { s(t, t, st); }
+  __device__ __forceinline__ void s(int t, int q, int st) const {
+    const uint64_t dq = q ? dq1 : dq0;
     const uint64_t dks = dk + static_cast<uint64_t>(st * (kTileBytes >> 4));
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
@@ -194,8 +195,10 @@ __device__ __forceinline__ float merge_parts(const AttnArgs& args, int u, int t,
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
   float mx = -INFINITY;
+#pragma unroll 4
   for (int p = 0; p < S; ++p) mx = fmaxf(mx, args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r]);
   float wsum = 0.f;
+#pragma unroll 4
   for (int p = 0; p < S; ++p) {
     const float lse = args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r];
     const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - mx);

@@ -324,7 +324,7 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   const SparsePlan plan = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count());
   s.workspace_bytes = plan.workspace_bytes();
   s.workspace = take(s.workspace_bytes);
-  s.n_tickets = plan.split > 1 && len_q <= kMergeRows ? 2 * plan.rem : 0;
+  s.n_tickets = plan.split > 1 && len_q <= kMergeRows ? plan.rem : 0;
   s.tickets = take(s.n_tickets * sizeof(int));
   s.total = at;
   return s;

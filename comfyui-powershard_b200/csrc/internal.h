@@ -56,12 +56,12 @@ struct AttnArgs {
   int piece;             // rows of one K/V load: 128, or 64 when key_block is not a multiple of 128
   const int* q_len;      // [batch] query rows in use, or null: all; output rows behind them are zero
   const int* k_len;      // [batch] key rows in use, or null: all; what lies behind them is not used
-  int* tickets;          // [split units][2] zeros: the last part of a unit merges it, or null: a kernel of its own does
+  int* tickets;          // few queries: [split units] zeros, the last part of a unit merges it; or null: a kernel of its own does
 };
 
 constexpr int kMaxSplit = 8;
 constexpr int kMaxSparseSplit = 32;
-constexpr int kMergeRows = 16;  // query rows up to which the attention kernel itself can merge a unit's parts
+constexpr int kMergeRows = 16;  // query rows up to which sparse attention runs in its form for few queries
 // Workspace bytes for up to 160 SMs: one partial (O, lse) per CTA of a wave.
 constexpr int64_t kAttnWorkspaceBytes = int64_t(160) * 2 * 128 * (128 + 1) * 4;
 

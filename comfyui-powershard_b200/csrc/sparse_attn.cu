@@ -24,7 +24,16 @@
 // Warp roles (320 threads) as in the dense kernel: 0-3 / 4-7 softmax and
 // epilogue of query tile 0 / 1, 8 producer (the whole warp: it also zeroes V
 // rows), 9 UMMA issuer.  Where a unit has one query tile (the last pair of an
-// odd count, or few queries), group 1 sits it out.
+// odd count), group 1 sits it out.
+//
+// The form for few queries (kFew: at most 16 rows, one tile of which one warp's
+// rows hold them) is bound by the keys it reads and, per CTA, by the latency of
+// load, scores, softmax and output product in turn.  So warps 0 and 4 take the
+// key tiles by turns, each with its own S, P and O; the issue order S_n,
+// PV_{n-1}, S_{n+1} keeps two tiles under way, and the memory of the second
+// query tile is a third V stage.  At a unit's end warp 0 adds the two up.
+// Measured, 48 tiles a list, 120 lists: 2.0 us a tile with one group alone,
+// MEASURED_FEW in turns.
 #include "attn_tile.cuh"
 
 namespace psb {
@@ -38,7 +47,7 @@ enum SparseBar : int {
   kQ = 0,
   kKFull = 1,
   kVFull = kKFull + kKStages,
-  kS = kVFull + kVStages,  // [2] S_t computed
+  kS = kVFull + 3,         // [2] S_t computed
   kFree = kS + 2,          // [2] FREE[n%2]: every S of tile n observed complete -> K_n, V_{n-1} free
   kP = kFree + 2,          // [2] P_t written
   kPH = kP + 2,            // [2][kPParts-1]
@@ -47,11 +56,17 @@ enum SparseBar : int {
   kTail = kDrain + 1,      // V rows of a partly used tile loaded
   kMeta = kTail + 1,       // [kRing] rows in use of a tile published
   kWork = kMeta + kRing,   // [2] a unit published
-  kTaken = kWork + 2,      // [2] ... and read by the other nine warps
+  kTaken = kWork + 2,      // [2] ... and read by the issuer and the softmax warps
   kNext = kTaken + 2,      // the grid's answer
-  kCount = kNext + 1
+  kOther = kNext + 1,      // few queries: group 1's rows of a unit staged
+  kOtherRead = kOther + 1, // ... and read
+  kCount = kOtherRead + 1
 };
+constexpr int kFewVStages = 3;
 constexpr int kStageOff = kSmemQ + kSmemK + kSmemV;
+static_assert(kTileBytes + kSmemK + kFewVStages * kTileBytes == kStageOff, "few queries: one Q tile, three V stages");
+constexpr int kMergePad = kHeadDim + 4;  // floats of a staged row of O
+static_assert(kMergeRows * (kMergePad + 2) * 4 <= 8 * kStageBytes && kMergeRows <= 32, "staged rows");
 constexpr int kBarOff = kStageOff + 8 * kStageBytes;
 constexpr int kSmem = kBarOff + 512 + 1024;  // barriers and small words, 1 KiB align slack
 static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
@@ -68,7 +83,6 @@ struct Work {
 struct Small {  // behind the barriers
   Work work[2];
   int meta[kRing];  // rows in use of a tile's lower 64 | upper 64 << 8
-  int last[2];      // whether this CTA wrote the last part of its unit's query tile t
   uint32_t tmem;
   int abort;
   __align__(16) int answer[4];
@@ -132,15 +146,16 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int x, BlockList& b
   return w;
 }
 
-template <bool kFp16>
+template <bool kFp16, bool kFew>
 __global__ void __launch_bounds__(kThreads, 1)
     sparse_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const AttnArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = smem + kSmemQ;
+  uint8_t* sK = smem + (kFew ? kTileBytes : kSmemQ);
   uint8_t* sV = sK + kSmemK;
+  constexpr int kVSt = kFew ? kFewVStages : kVStages;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
   Small* small = reinterpret_cast<Small*>(bars + kCount + (kCount & 1));
   volatile int* abort_flag = &small->abort;
@@ -155,19 +170,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bar(kQ), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(kKFull + i), 1);
-      mbar_init(bar(kVFull + i), 1);
       mbar_init(bar(kS + i), 1);
       mbar_init(bar(kFree + i), 1);
-      mbar_init(bar(kP + i), 128);
-      for (int q = 0; q + 1 < kPParts; ++q) mbar_init(bar(kPH + i * (kPParts - 1) + q), 128);
+      mbar_init(bar(kP + i), kFew ? 32 : 128);
+      for (int q = 0; q + 1 < kPParts; ++q) mbar_init(bar(kPH + i * (kPParts - 1) + q), kFew ? 32 : 128);
       mbar_init(bar(kWork + i), 1);
-      mbar_init(bar(kTaken + i), 9);
+      mbar_init(bar(kTaken + i), kFew ? 3 : 9);
     }
+    for (int i = 0; i < kVSt; ++i) mbar_init(bar(kVFull + i), 1);
     for (int i = 0; i < kRing; ++i) mbar_init(bar(kMeta + i), 1);
     mbar_init(bar(kO), 1);
     mbar_init(bar(kDrain), 1);
     mbar_init(bar(kTail), 1);
     mbar_init(bar(kNext), 1);
+    mbar_init(bar(kOther), 1);
+    mbar_init(bar(kOtherRead), 1);
     fence_mbar_init();
   }
   if (warp == 9) {
@@ -245,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         };
         for (int i = 0; i < w.tiles; ++i, ++n) {
-          const int st = n & 1;
+          const int st = n & 1, vst = n % kVSt;
           // The rows are looked up before the wait for the stage.
           int row[2] = {0, 0}, valid[2] = {0, 0};
           bool tail = false;  // rows of the tensor that are not in use reach the tile
@@ -264,13 +281,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           load(sK + st * kTileBytes, &tm_k, kKFull + st, row);
           issued = 2 * n + 1;
-          if (n >= kVStages)
+          // V_{n-kVSt} is read: S_{n-1} is complete, and every PV issued before it.
+          if (n >= kVSt)
             ok = warp_wait(bar(kFree + ((n - 1) & 1)), ((n - 1) >> 1) & 1u, abort_flag, status, kErrEmpty);
           if (!ok) break;
           if (!tail) {
-            load(sV + st * kTileBytes, &tm_v, kVFull + st, row);
+            load(sV + vst * kTileBytes, &tm_v, kVFull + vst, row);
           } else {
-            uint8_t* stage = sV + st * kTileBytes;
+            uint8_t* stage = sV + vst * kTileBytes;
             load(stage, &tm_v, kTail, row);
             drain_wait(bar(kTail), tail_phase, status);
             tail_phase ^= 1u;
@@ -286,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kVFull + st));
+            if (lane == 0) mbar_arrive(bar(kVFull + vst));
           }
           issued = 2 * n + 2;
         }
@@ -303,11 +321,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (open_request >= 0) drain_wait(bar(kNext), static_cast<uint32_t>(open_request), status);
     if (loaded) drain_wait(bar(kQ), (loaded - 1) & 1u, status);
     const int tiles = (issued + 1) / 2;  // with at least the K copy issued
-    for (int i = max(0, tiles - kKStages); i < tiles; ++i) {
-      const uint32_t ph = (i >> 1) & 1u;
-      drain_wait(bar(kKFull + (i & 1)), ph, status);
-      if (2 * i + 2 <= issued) drain_wait(bar(kVFull + (i & 1)), ph, status);
-    }
+    for (int i = max(0, tiles - kKStages); i < tiles; ++i) drain_wait(bar(kKFull + (i & 1)), (i >> 1) & 1u, status);
+    for (int i = max(0, tiles - kVSt); i < tiles; ++i)
+      if (2 * i + 2 <= issued) drain_wait(bar(kVFull + i % kVSt), (i / kVSt) & 1u, status);
   } else if (warp == 9) {
     // ------------------------------------------------------------ UMMA issuer (one lane)
     if (lane == 0) {
@@ -335,32 +351,199 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool two = (w.unit % args.npairs) * 2 + 1 < args.num_q_tiles;
         ok = mbar_wait(bar(kQ), loaded & 1u, abort_flag, status, kErrQ);
         ++loaded;
-        // Issue order per key tile: S0_i, PV1_{i-1}, S1_i, PV0_i.  The first S
-        // of a unit follow the last PV of the one before on the tensor pipe.
-        for (int i = 0; i < w.tiles && ok; ++i, ++n) {
-          const int st = n & 1;
-          ok = mbar_wait(bar(kKFull + st), (n >> 1) & 1u, abort_flag, status, kErrFull);
-          if (!ok) break;
-          tc_fence_after();
-          mma.s(0, st);
-          umma_commit(bar(kS + 0));
-          if (two) {
-            if (i > 0) ok = pv(1, (n - 1) & 1, (n1 - 1) & 1u, i > 1);
-            if (!ok) break;
-            mma.s(1, st);
-            umma_commit(bar(kS + 1));
-            ++n1;
+        if constexpr (kFew) {
+          // Tile j belongs to group j & 1: PV_{j-2}, S_j, PV_{j-1}, S_{j+1}, ...
+          const int n0 = n;
+          for (int j = n0; j < n0 + w.tiles + 2 && ok; ++j) {
+            const int d = j - 2;
+            if (d >= n0) {
+              ok = mbar_wait(bar(kVFull + d % kVSt), (d / kVSt) & 1u, abort_flag, status, kErrFull);
+              if (ok) ok = pv(d & 1, d % kVSt, (d >> 1) & 1u, d - n0 >= 2);
+              if (!ok) break;
+            }
+            if (j < n0 + w.tiles) {
+              ok = mbar_wait(bar(kKFull + (j & 1)), (j >> 1) & 1u, abort_flag, status, kErrFull);
+              if (!ok) break;
+              tc_fence_after();
+              mma.s(j & 1, 0, j & 1);
+              umma_commit(bar(kS + (j & 1)));
+            }
           }
-          ok = mbar_wait(bar(kVFull + st), (n >> 1) & 1u, abort_flag, status, kErrFull);
-          if (ok) ok = pv(0, st, n & 1u, i > 0);
+          n = n0 + w.tiles;
+        } else {
+          // Issue order per key tile: S0_i, PV1_{i-1}, S1_i, PV0_i.  The first S
+          // of a unit follow the last PV of the one before on the tensor pipe.
+          for (int i = 0; i < w.tiles && ok; ++i, ++n) {
+            const int st = n & 1;
+            ok = mbar_wait(bar(kKFull + st), (n >> 1) & 1u, abort_flag, status, kErrFull);
+            if (!ok) break;
+            tc_fence_after();
+            mma.s(0, st);
+            umma_commit(bar(kS + 0));
+            if (two) {
+              if (i > 0) ok = pv(1, (n - 1) & 1, (n1 - 1) & 1u, i > 1);
+              if (!ok) break;
+              mma.s(1, st);
+              umma_commit(bar(kS + 1));
+              ++n1;
+            }
+            ok = mbar_wait(bar(kVFull + st), (n >> 1) & 1u, abort_flag, status, kErrFull);
+            if (ok) ok = pv(0, st, n & 1u, i > 0);
+          }
+          if (ok && two) ok = pv(1, (n - 1) & 1, (n1 - 1) & 1u, w.tiles > 1);
         }
-        if (!ok) break;
-        if (two) ok = pv(1, (n - 1) & 1, (n1 - 1) & 1u, w.tiles > 1);
         if (ok) umma_commit(bar(kO));
       }
       // All issued UMMAs complete before TMEM is released.
       umma_commit(bar(kDrain));
       drain_wait(bar(kDrain), 0, status);
+    }
+  } else if (kFew) {
+    // ------------------------------------------------------------ softmax, few queries
+    const int t = warp >> 2;
+    const uint32_t s_addr = tmem + 128 * t, o_addr = tmem + 256 + 128 * t;
+    float* rows_o = reinterpret_cast<float*>(smem + kStageOff);  // of group 1: [kMergeRows][kMergePad], then m, l
+    float* rows_ml = rows_o + kMergeRows * kMergePad;
+    int n = 0, loaded = 0;  // tiles; units with tiles
+    for (int u = 0; (warp & 3) == 0; ++u) {
+      const int b = u & 1;
+      if (!warp_wait(bar(kWork + b), (u >> 1) & 1u, abort_flag, status, kErrWork)) break;
+      const int tiles = small->work[b].tiles;
+      if (small->work[b].unit < 0) break;
+      float m = -1e30f, l = 0.f;
+      bool ok = true, any = false;
+      const int end = n + tiles;
+      for (int j = n + ((n ^ t) & 1); j < end; j += 2) {
+        const int slot = j & (kRing - 1);
+        ok = warp_wait(bar(kMeta + slot), (j / kRing) & 1u, abort_flag, status, kErrMeta);
+        if (!ok) break;
+        const int used = small->meta[slot];
+        ok = warp_wait(bar(kS + t), (j >> 1) & 1u, abort_flag, status, kErrS);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(bar(kFree + t));
+        tc_fence_after();
+        uint32_t sr[128];
+        tmem_ld32_at<0>(s_addr + 0, sr);
+        tmem_ld32_at<32>(s_addr + 32, sr);
+        tmem_ld32_at<64>(s_addr + 64, sr);
+        tmem_ld32_at<96>(s_addr + 96, sr);
+        tmem_wait_ld();
+        float s[128];
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(sr[i]);
+        if (used != (64 | (64 << 8))) {
+          const int lo = used & 0xff, hi = used >> 8;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if ((i & 63) >= (i < 64 ? lo : hi)) s[i] = -INFINITY;
+        }
+        softmax_row<kFp16, true>(s, !any, args.scale_log2, s_addr, o_addr, bar(kPH + t * (kPParts - 1)), bar(kP + t), m, l);
+        any = true;
+      }
+      n = end;
+      if (tiles > 0) {
+        if (ok) ok = warp_wait(bar(kO), loaded & 1u, abort_flag, status, kErrO);
+        // Group 1's staged rows: free to write, or written.
+        if (ok && t == 0) ok = warp_wait(bar(kOther), loaded & 1u, abort_flag, status, kErrO);
+        if (ok && t == 1 && loaded > 0) ok = warp_wait(bar(kOtherRead), (loaded - 1) & 1u, abort_flag, status, kErrO);
+        ++loaded;
+      }
+      if (!ok) break;
+      const Work w = small->work[b];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kTaken + b));
+      tc_fence_after();
+      const Coord c(args, w.unit);
+      const int rows = args.seg_rows_q;
+      // out = (w0 O_0 + w1 O_1) / (w0 l_0 + w1 l_1), w_t = 2^(m_t - max); a group
+      // without a tile never wrote its O.
+      if (t == 1) {
+        if (tiles == 0) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + 32 * q, o);
+          tmem_wait_ld();
+          if (lane < rows) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(rows_o + lane * kMergePad + 32 * q + 4 * i) =
+                  any ? make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                    __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]))
+                      : make_float4(0, 0, 0, 0);
+          }
+        }
+        if (lane < rows) {
+          rows_ml[2 * lane] = m;
+          rows_ml[2 * lane + 1] = l;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kOther));
+      } else {
+        const bool live = tiles > 0 && lane < w.rows;
+        const float m1 = lane < rows ? rows_ml[2 * lane] : -1e30f, l1 = lane < rows ? rows_ml[2 * lane + 1] : 0.f;
+        const float top = fmaxf(m, m1);
+        const float w0 = ex2_approx(m - top), w1 = ex2_approx(m1 - top);
+        const float total = fmaf(w0, l, w1 * l1);
+        const float inv_l = total > 0.f ? 1.f / total : 0.f;
+        const float f0 = w0 * inv_l, f1 = w1 * inv_l;
+        const int64_t at = static_cast<int64_t>(w.slot) * 2 * kBlockM + lane;  // of the split workspace
+        uint16_t* out = static_cast<uint16_t*>(args.seg_out[0]) + c.batch * args.o_stride[0] + c.head * args.o_stride[3];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + 32 * q, o);
+          tmem_wait_ld();
+          if (lane < rows) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 a = *reinterpret_cast<const float4*>(rows_o + lane * kMergePad + 32 * q + 8 * i);
+              const float4 e = *reinterpret_cast<const float4*>(rows_o + lane * kMergePad + 32 * q + 8 * i + 4);
+              const float other[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+              float v[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const float own = any ? __uint_as_float(o[8 * i + x]) : 0.f;
+                v[x] = live ? fmaf(own, f0, other[x] * f1) : 0.f;
+              }
+              if (w.slot >= 0) {
+                float4* dst = reinterpret_cast<float4*>(args.ws_o + at * kHeadDim + 32 * q + 8 * i);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+              } else {
+                *reinterpret_cast<uint4*>(out + lane * args.o_stride[2] + 32 * q + 8 * i) =
+                    make_uint4(pack2<kFp16>(v[0], v[1]), pack2<kFp16>(v[2], v[3]), pack2<kFp16>(v[4], v[5]),
+                               pack2<kFp16>(v[6], v[7]));
+              }
+            }
+          }
+        }
+        if (w.slot >= 0 && lane < rows) args.ws_lse[at] = live && total > 0.f ? top + __log2f(total) : -INFINITY;
+        __syncwarp();
+        if (lane == 0 && tiles > 0) mbar_arrive(bar(kOtherRead));
+        if (w.slot >= 0 && args.tickets) {
+          // Whichever part is written last merges them, in the order of the
+          // parts (a launch less: 3 us of a 25 us call).
+          const int split_unit = w.slot / args.split;
+          __threadfence();
+          __syncwarp();
+          int done = 0;
+          if (lane == 0) done = atomicAdd(&args.tickets[split_unit], 1);
+          done = __shfl_sync(0xffffffffu, done, 0);
+          if (done == args.split - 1) {
+            __threadfence();
+            const int col = (lane & 15) * 8;
+            for (int r = lane >> 4; r < rows; r += 2) {
+              float acc[8];
+              const float inv = merge_parts(args, split_unit, 0, r, col, acc);
+              *reinterpret_cast<uint4*>(out + r * args.o_stride[2] + col) =
+                  make_uint4(pack2<kFp16>(acc[0] * inv, acc[1] * inv), pack2<kFp16>(acc[2] * inv, acc[3] * inv),
+                             pack2<kFp16>(acc[4] * inv, acc[5] * inv), pack2<kFp16>(acc[6] * inv, acc[7] * inv));
+            }
+          }
+        }
+      }
+      tc_fence_before();  // O is read before the next unit's P is released
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -451,32 +634,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (row < rows) args.ws_lse[at] = live && l > 0.f ? m + __log2f(l) : -INFINITY;
         }
-        if (args.tickets) {
-          // Few rows: whichever part is written last merges them, in the order
-          // of the parts (a launch less: 3 us of a 25 us call).
-          const int split_unit = w.slot / args.split;
-          const int sub = threadIdx.x & 127;
-          __threadfence();
-          named_bar_sync(1 + t, 128);
-          if (sub == 0) small->last[t] = atomicAdd(&args.tickets[2 * split_unit + t], 1) == args.split - 1;
-          named_bar_sync(1 + t, 128);
-          if (small->last[t]) {
-            __threadfence();
-            uint16_t* out = static_cast<uint16_t*>(args.seg_out[0]) + c.batch * args.o_stride[0] +
-                            static_cast<int64_t>(row0) * args.o_stride[2] + c.head * args.o_stride[3];
-            const int col = (sub & 15) * 8;
-            for (int r = sub >> 4; r < rows; r += 8) {
-              float acc[8];
-              const float inv = merge_parts(args, split_unit, t, r, col, acc);
-              uint4 v;
-              v.x = pack2<kFp16>(acc[0] * inv, acc[1] * inv);
-              v.y = pack2<kFp16>(acc[2] * inv, acc[3] * inv);
-              v.z = pack2<kFp16>(acc[4] * inv, acc[5] * inv);
-              v.w = pack2<kFp16>(acc[6] * inv, acc[7] * inv);
-              *reinterpret_cast<uint4*>(out + r * args.o_stride[2] + col) = v;
-            }
-          }
-        }
       } else {
         // Each warp stages 64 columns of its 32 rows (row r, 16-byte chunk k at
         // r*128 + ((k ^ (r & 7)) << 4)), then 8 threads store 128 bytes of a row.
@@ -526,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool kFp16>
+template <bool kFp16, bool kFew>
 int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args, int64_t units,
            bool after_select, cudaStream_t stream) {
   static bool done[64] = {false};
@@ -534,7 +691,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (!done[dev]) {
     const cudaError_t err =
-        cudaFuncSetAttribute(sparse_attn_kernel<kFp16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        cudaFuncSetAttribute(sparse_attn_kernel<kFp16, kFew>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (err != cudaSuccess) return set_cuda_error("sparse attention: cudaFuncSetAttribute", err);
     done[dev] = true;
   }
@@ -542,7 +699,7 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
   const int64_t ctas = args.full_units + (split_units > 0 ? split_units * args.split : units - args.full_units);
   if (ctas <= 0) return 0;
   if (ctas > 0x7fffffff) return set_error(PS_B200_ERR_UNSUPPORTED, "attention grid above 2^31 CTAs");
-  const cudaError_t err = launch_after(sparse_attn_kernel<kFp16>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads),
+  const cudaError_t err = launch_after(sparse_attn_kernel<kFp16, kFew>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads),
                                        kSmem, stream, after_select, tq, tk, tv, args);
   if (err != cudaSuccess) return set_cuda_error("sparse attention launch", err);
   count_launch();
@@ -555,8 +712,10 @@ int launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, 
 
 int launch_sparse_attention(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnArgs& args,
                             int64_t total_units, bool fp16, bool after_select, cudaStream_t stream) {
-  return fp16 ? attn::launch<true>(tq, tk, tv, args, total_units, after_select, stream)
-              : attn::launch<false>(tq, tk, tv, args, total_units, after_select, stream);
+  const bool few = args.seg_rows_q <= kMergeRows;
+  auto launch = fp16 ? (few ? attn::launch<true, true> : attn::launch<true, false>)
+                     : (few ? attn::launch<false, true> : attn::launch<false, false>);
+  return launch(tq, tk, tv, args, total_units, after_select, stream);
 }
 
 }  // namespace psb

@@ -279,7 +279,7 @@ def random_lists(seed, b, h, nq, nk, n):
 @pytest.mark.parametrize("lq,lk,heads,kv,key_block,n", [
     (256, 256, 1, 1, 128, 1), (256, 512, 2, 2, 64, 3), (300, 1000, 2, 1, 128, 5), (1, 1, 1, 1, 64, 1),
     (1, 700, 4, 2, 64, 9), (513, 257, 2, 2, 64, 5), (130, 2000, 3, 1, 192, 10), (257, 1300, 2, 2, 256, 4),
-    (70, 5000, 2, 2, 64, 70)])
+    (70, 5000, 2, 2, 64, 70), (16, 3000, 4, 1, 128, 20), (17, 3000, 4, 1, 128, 20), (3, 640, 90, 45, 64, 5)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_sparse_attention(cuda_lib, lq, lk, heads, kv, key_block, n, dtype):
     from powershard_b200 import sparse
@@ -298,7 +298,7 @@ def test_sparse_attention_lists_of_any_kind(cuda_lib, key_block):
     """Short and empty lists, entries that name no block, repeated and unordered entries, and what lies behind
     the lengths (NaN and infinities), in the whole and in the split form."""
     from powershard_b200 import sparse
-    for b, heads, lq, lk, n in ((2, 3, 600, 1111, 7), (3, 2, 40, 3000, 20)):
+    for b, heads, lq, lk, n in ((2, 3, 600, 1111, 7), (3, 2, 40, 3000, 20), (2, 3, 16, 3000, 20), (3, 60, 2, 900, 6)):
         q, k, v = (rows(s, b, m, heads, 128) for s, m in ((9, lq), (10, lk), (11, lk)))
         nq, nk = -(-lq // 256), -(-lk // key_block)
         blocks = random_lists(12, b, heads, nq, nk, n)
@@ -308,7 +308,7 @@ def test_sparse_attention_lists_of_any_kind(cuda_lib, key_block):
         blocks[1, 1, 0, 0] = nk - 1                   # the block that ends inside the tensor
         counts = torch.full((b, heads, nq), n, dtype=torch.int32)
         counts[0, 0, -1], counts[1, 1, -1], counts[1, 0, 0] = 1, 0, n + 9  # clamped to the list
-        q_len, k_len = lens(lq, lq - 7, 0)[:b], lens(lk - 70, lk, 33)[:b]
+        q_len, k_len = lens(lq, max(lq - 7, 1), 0)[:b], lens(lk - 70, lk, 33)[:b]
         for i in range(b):
             q[i, int(q_len[i]):] = float("nan")
             k[i, int(k_len[i]):] = float("inf")
@@ -381,7 +381,7 @@ def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,lq,lk,heads,kv,qb,kb,keep,ragged", [
     (1, 1000, 1000, 2, 2, 256, 128, 3, False), (2, 777, 777, 4, 2, 256, 64, 5, True), (1, 1, 4096, 3, 1, 256, 128, 8, False),
-    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (5, 1, 1, 2, 2, 256, 64, 1, True)])
+    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (2, 7, 9000, 6, 3, 256, 64, 50, True), (4, 16, 2000, 50, 10, 256, 128, 9, True), (5, 1, 1, 2, 2, 256, 64, 1, True)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_provider(cuda_lib, b, lq, lk, heads, kv, qb, kb, keep, ragged, dtype):
     from powershard_b200 import sparse
