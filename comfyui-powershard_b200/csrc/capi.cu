@@ -1138,7 +1138,8 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
   const int64_t qs[4] = {q_strides[0], 0, q_strides[1], q_strides[2]};
   const int64_t ks[4] = {k_strides[0], 0, k_strides[1], k_strides[2]};
   const int64_t vs[4] = {v_strides[0], 0, v_strides[1], v_strides[2]};
-  if (int rc = make_map(&tq, q, fp16, head_dim, heads_q, len_q, 1, batch, qs)) return rc;
+  const int q_box = len_q <= kMergeRows ? 32 : 128;  // few queries: a quarter of a tile
+  if (int rc = make_map(&tq, q, fp16, head_dim, heads_q, len_q, 1, batch, qs, q_box)) return rc;
   if (int rc = make_map(&tk, k, fp16, head_dim, heads_kv, len_k, 1, batch, ks, a.piece)) return rc;
   if (int rc = make_map(&tv, v, fp16, head_dim, heads_kv, len_k, 1, batch, vs, a.piece)) return rc;
   a.seg_out[0] = a.pre_out = out;

@@ -30,8 +30,11 @@
 // rows hold them) is bound by the keys it reads and, per CTA, by the latency of
 // load, scores, softmax and output product in turn.  So warps 0 and 4 take the
 // key tiles by turns, each with its own S, P and O; the issue order S_n,
-// PV_{n-1}, S_{n+1} keeps two tiles under way, and the memory of the second
-// query tile is a third V stage.  At a unit's end warp 0 adds the two up.
+// PV_{n-1}, S_{n+1} keeps two tiles under way, and the shared memory of the
+// second query tile and of the output staging are a third K and V stage (the
+// 1.5 us and more that a load takes under way are then spread over three
+// tiles).  At a unit's end warp 0 adds the two up, through the part of the
+// query tile that holds no query.
 // Measured, 48 tiles a list, 120 lists: 2.0 us a tile with one group alone,
 // MEASURED_FEW in turns.
 #include "attn_tile.cuh"
@@ -41,33 +44,39 @@ namespace attn {
 namespace {
 
 constexpr int kStageBytes = 4096;  // output staging of one softmax warp: 32 rows x 64 columns
-constexpr int kRing = 4;           // tiles whose rows in use are published ahead
+constexpr int kRing = 4;           // FREE signals: K_{n+4} is never loaded before FREE(n) is waited for
+constexpr int kMetaRing = 8;       // published rows: tile n+8 is published after FREE(n+5), so n has been read
 
 enum SparseBar : int {
   kQ = 0,
   kKFull = 1,
-  kVFull = kKFull + kKStages,
+  kVFull = kKFull + 3,
   kS = kVFull + 3,         // [2] S_t computed
-  kFree = kS + 2,          // [2] FREE[n%2]: every S of tile n observed complete -> K_n, V_{n-1} free
-  kP = kFree + 2,          // [2] P_t written
+  kFree = kS + 2,          // [kRing] FREE[n%4]: every S of tile n observed complete -> K_n free, and V_{n-1}
+                           // (few queries: V_{n-2}), whose PV was issued before
+  kP = kFree + kRing,      // [2] P_t written
   kPH = kP + 2,            // [2][kPParts-1]
   kO = kPH + 2 * (kPParts - 1),  // O_0 and O_1 of a unit final
   kDrain = kO + 1,
   kTail = kDrain + 1,      // V rows of a partly used tile loaded
-  kMeta = kTail + 1,       // [kRing] rows in use of a tile published
-  kWork = kMeta + kRing,   // [2] a unit published
+  kMeta = kTail + 1,       // [kMetaRing] rows in use of a tile published
+  kWork = kMeta + kMetaRing,  // [2] a unit published
   kTaken = kWork + 2,      // [2] ... and read by the issuer and the softmax warps
   kNext = kTaken + 2,      // the grid's answer
   kOther = kNext + 1,      // few queries: group 1's rows of a unit staged
   kOtherRead = kOther + 1, // ... and read
   kCount = kOtherRead + 1
 };
-constexpr int kFewVStages = 3;
 constexpr int kStageOff = kSmemQ + kSmemK + kSmemV;
-static_assert(kTileBytes + kSmemK + kFewVStages * kTileBytes == kStageOff, "few queries: one Q tile, three V stages");
-constexpr int kMergePad = kHeadDim + 4;  // floats of a staged row of O
-static_assert(kMergeRows * (kMergePad + 2) * 4 <= 8 * kStageBytes && kMergeRows <= 32, "staged rows");
 constexpr int kBarOff = kStageOff + 8 * kStageBytes;
+// Few queries: one Q tile, of which the first 32 rows are loaded (the others
+// give rows of S and O that nothing reads), and three K and V stages.
+constexpr int kFewStages = 3;
+constexpr int kFewQRows = 32;
+constexpr int kMergePad = kHeadDim + 4;     // floats of a staged row of O
+constexpr int kMergeOff = kFewQRows * 128;  // behind those rows of the tile's first 64 columns
+static_assert(kMergeOff + kMergeRows * (kMergePad + 2) * 4 <= kHalfTile && kMergeRows <= kFewQRows, "staged rows");
+static_assert(kTileBytes + 2 * kFewStages * kTileBytes == kBarOff, "both forms end at the barriers");
 constexpr int kSmem = kBarOff + 512 + 1024;  // barriers and small words, 1 KiB align slack
 static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
 
@@ -82,7 +91,7 @@ struct Work {
 
 struct Small {  // behind the barriers
   Work work[2];
-  int meta[kRing];  // rows in use of a tile's lower 64 | upper 64 << 8
+  int meta[kMetaRing];  // rows in use of a tile's lower 64 | upper 64 << 8
   uint32_t tmem;
   int abort;
   __align__(16) int answer[4];
@@ -99,33 +108,42 @@ struct Coord {
   }
 };
 
-// Key tiles of one unit's list.  A block is cut into pieces of `piece` rows and
-// a 128-row tile holds 128 / piece consecutive pieces of the list.
+// The pieces of one unit's list, in order: a block is cut into pieces of
+// args.piece rows, a 128-row tile holds 128 / piece consecutive ones.
 struct BlockList {
   const int* list;
-  int count;  // entries in use
-  int len_k;  // key rows in use
-  int ppb;    // pieces of one block
+  int count;     // entries in use
+  int len_k;     // key rows in use
+  int per;       // pieces of one block
+  int entry, sub;  // of the next piece
 
-  // First row of piece p of key tile t, and in `valid` its rows in use.  A
-  // piece without any starts behind the tensor: its load fills with zeros.
-  __device__ __forceinline__ int row(const AttnArgs& a, int t, int p, int& valid) const {
-    const int g = t * (kBlockN / a.piece) + p;
-    const int e = g / ppb;
+  struct Piece {
+    int block, sub;
+  };
+  // The load of the block's number is under way until the piece is used.
+  __device__ __forceinline__ Piece next() {
+    const Piece p{entry < count ? __ldg(list + entry) : -1, sub};
+    if (++sub == per) {
+      sub = 0;
+      ++entry;
+    }
+    return p;
+  }
+  // First row of a piece, and in `valid` its rows in use.  A piece without any
+  // starts behind the tensor: its load fills with zeros.
+  __device__ __forceinline__ int row(const AttnArgs& a, const Piece& p, int& valid) const {
     valid = 0;
-    if (e >= count) return a.seg_rows_k;
-    const int blk = list[e];
-    if (blk < 0 || blk >= a.key_blocks) return a.seg_rows_k;
-    const int64_t r = static_cast<int64_t>(blk) * a.key_block + (g - e * ppb) * a.piece;
+    if (p.block < 0 || p.block >= a.key_blocks) return a.seg_rows_k;
+    const int64_t r = static_cast<int64_t>(p.block) * a.key_block + p.sub * a.piece;
     if (r >= len_k) return a.seg_rows_k;
     valid = min(a.piece, len_k - static_cast<int>(r));
     return static_cast<int>(r);
   }
 };
 
-// The unit (or part of one) that grid index x stands for: its list, and in
-// `begin` its first tile of the list.
-__device__ __forceinline__ Work find_work(const AttnArgs& a, int x, BlockList& b, int& begin) {
+// The unit (or part of one) that grid index x stands for, and its list from
+// the first tile on.
+__device__ __forceinline__ Work find_work(const AttnArgs& a, int x, BlockList& b) {
   Work w;
   const bool partial = x >= a.full_units;
   w.slot = partial ? x - a.full_units : -1;
@@ -139,10 +157,13 @@ __device__ __forceinline__ Work find_work(const AttnArgs& a, int x, BlockList& b
   b.list = a.blocks + at * a.list_len;
   b.count = a.counts ? min(max(a.counts[at], 0), a.list_len) : a.list_len;
   if (c.pair * 2 * kBlockM >= w.rows || b.len_k == 0) b.count = 0;
-  b.ppb = a.key_block / a.piece;
+  b.per = a.key_block / a.piece;
   const int64_t tiles = (static_cast<int64_t>(b.count) * a.key_block + kBlockN - 1) / kBlockN;
-  begin = static_cast<int>(part * tiles / parts);
+  const int begin = static_cast<int>(part * tiles / parts);
   w.tiles = static_cast<int>((part + 1) * tiles / parts) - begin;
+  const int first = begin * (kBlockN / a.piece);
+  b.entry = first / b.per;
+  b.sub = first - b.entry * b.per;
   return w;
 }
 
@@ -153,9 +174,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
+  constexpr int kKSt = kFew ? kFewStages : kKStages, kVSt = kFew ? kFewStages : kVStages;
   uint8_t* sK = smem + (kFew ? kTileBytes : kSmemQ);
-  uint8_t* sV = sK + kSmemK;
-  constexpr int kVSt = kFew ? kFewVStages : kVStages;
+  uint8_t* sV = sK + kKSt * kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBarOff);
   Small* small = reinterpret_cast<Small*>(bars + kCount + (kCount & 1));
   volatile int* abort_flag = &small->abort;
@@ -169,16 +190,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     small->abort = 0;
     mbar_init(bar(kQ), 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kKFull + i), 1);
       mbar_init(bar(kS + i), 1);
-      mbar_init(bar(kFree + i), 1);
       mbar_init(bar(kP + i), kFew ? 32 : 128);
       for (int q = 0; q + 1 < kPParts; ++q) mbar_init(bar(kPH + i * (kPParts - 1) + q), kFew ? 32 : 128);
       mbar_init(bar(kWork + i), 1);
       mbar_init(bar(kTaken + i), kFew ? 3 : 9);
     }
+    for (int i = 0; i < kKSt; ++i) mbar_init(bar(kKFull + i), 1);
     for (int i = 0; i < kVSt; ++i) mbar_init(bar(kVFull + i), 1);
-    for (int i = 0; i < kRing; ++i) mbar_init(bar(kMeta + i), 1);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(bar(kFree + i), 1);
+    }
+    for (int i = 0; i < kMetaRing; ++i) mbar_init(bar(kMeta + i), 1);
     mbar_init(bar(kO), 1);
     mbar_init(bar(kDrain), 1);
     mbar_init(bar(kTail), 1);
@@ -210,16 +233,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int piece_bytes = args.piece * 128;  // of one 64-column half
     int x = blockIdx.x;
     int n = 0, loaded = 0;  // tiles; units with tiles
-    int issued = 0;         // K and V loads
+    int k_loads = 0, v_loads = 0;
     uint32_t tail_phase = 0;
     int open_request = -1;  // phase of an answer not yet read
     bool ok = true;
     for (int u = 0;; ++u) {
       const int b = u & 1;
       BlockList list;
-      int begin = 0;
       Work w{-1, -1, 0, 0};
-      if (x >= 0) w = find_work(args, x, list, begin);
+      if (x >= 0) w = find_work(args, x, list);
       if (u >= 2) ok = warp_wait(bar(kTaken + b), ((u >> 1) - 1) & 1u, abort_flag, status, kErrWork);
       if (!ok) break;
       if (lane == 0) {
@@ -236,12 +258,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Coord c(args, w.unit);
         const int kv_head = c.head / args.group;
         // The last unit's scores are all computed once its last tile is free.
-        if (n > 0) ok = warp_wait(bar(kFree + ((n - 1) & 1)), ((n - 1) >> 1) & 1u, abort_flag, status, kErrEmpty);
+        auto free_wait = [&](int tile) {
+          return warp_wait(bar(kFree + tile % kRing), (tile / kRing) & 1u, abort_flag, status, kErrEmpty);
+        };
+        if (n > 0) ok = free_wait(n - 1);
         if (!ok) break;
         if (lane == 0) {
           const int t0 = c.pair * 2;
           const bool two = t0 + 1 < args.num_q_tiles;
-          mbar_arrive_expect_tx(bar(kQ), two ? 2 * kTileBytes : kTileBytes);
+          mbar_arrive_expect_tx(bar(kQ), kFew ? 2 * kFewQRows * 128 : two ? 2 * kTileBytes : kTileBytes);
           for (int h = 0; h < 2; ++h) {
             tma_load_5d(smem_u32(sQ + h * kHalfTile), &tm_q, bar(kQ), h * 64, c.head, t0 * kBlockM, 0, c.batch);
             if (two)
@@ -261,29 +286,44 @@ __global__ void __launch_bounds__(kThreads, 1)
                               row[p], 0, c.batch);
           }
         };
-        for (int i = 0; i < w.tiles; ++i, ++n) {
-          const int st = n & 1, vst = n % kVSt;
-          // The rows are looked up before the wait for the stage.
-          int row[2] = {0, 0}, valid[2] = {0, 0};
+        // The blocks of a tile are looked up a tile ahead of its K, and K goes a
+        // tile ahead of V.
+        BlockList::Piece ahead[2];
+        auto look = [&] {
+          ahead[0] = list.next();
+          if (pieces == 2) ahead[1] = list.next();
+        };
+        int row[2], valid[2], next_row[2] = {0, 0}, next_valid[2] = {0, 0};
+        auto load_k = [&](int tile) -> bool {  // and looks up the tile after it
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            if (p < pieces) next_row[p] = list.row(args, ahead[p], next_valid[p]);
+          look();
+          if (tile >= kKSt && !free_wait(tile - kKSt)) return false;
+          if (lane == 0) {
+            const int lo = pieces == 1 ? min(next_valid[0], 64) : next_valid[0];
+            const int hi = pieces == 1 ? max(next_valid[0] - 64, 0) : next_valid[1];
+            small->meta[tile % kMetaRing] = lo | (hi << 8);
+            mbar_arrive(bar(kMeta + tile % kMetaRing));
+          }
+          load(sK + tile % kKSt * kTileBytes, &tm_k, kKFull + tile % kKSt, next_row);
+          k_loads = tile + 1;
+          return true;
+        };
+        look();
+        ok = load_k(n);
+        for (int i = 0; i < w.tiles && ok; ++i, ++n) {
+          const int vst = n % kVSt;
           bool tail = false;  // rows of the tensor that are not in use reach the tile
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            if (p < pieces) row[p] = list.row(args, begin + i, p, valid[p]);
+            row[p] = next_row[p];
+            valid[p] = next_valid[p];
             tail |= valid[p] > 0 && valid[p] < args.piece && list.len_k < args.seg_rows_k;
           }
-          if (n >= kKStages) ok = warp_wait(bar(kFree + st), ((n - 2) >> 1) & 1u, abort_flag, status, kErrEmpty);
-          if (!ok) break;
-          if (lane == 0) {
-            const int lo = pieces == 1 ? min(valid[0], 64) : valid[0];
-            const int hi = pieces == 1 ? max(valid[0] - 64, 0) : valid[1];
-            small->meta[n & (kRing - 1)] = lo | (hi << 8);
-            mbar_arrive(bar(kMeta + (n & (kRing - 1))));
-          }
-          load(sK + st * kTileBytes, &tm_k, kKFull + st, row);
-          issued = 2 * n + 1;
+          if (i + 1 < w.tiles) ok = load_k(n + 1);
           // V_{n-kVSt} is read: S_{n-1} is complete, and every PV issued before it.
-          if (n >= kVSt)
-            ok = warp_wait(bar(kFree + ((n - 1) & 1)), ((n - 1) >> 1) & 1u, abort_flag, status, kErrEmpty);
+          if (ok && n >= kVSt) ok = free_wait(n - 1);
           if (!ok) break;
           if (!tail) {
             load(sV + vst * kTileBytes, &tm_v, kVFull + vst, row);
@@ -306,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kVFull + vst));
           }
-          issued = 2 * n + 2;
+          v_loads = n + 1;
         }
         if (!ok) break;
       }
@@ -320,10 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Every copy issued must land before the CTA may exit.
     if (open_request >= 0) drain_wait(bar(kNext), static_cast<uint32_t>(open_request), status);
     if (loaded) drain_wait(bar(kQ), (loaded - 1) & 1u, status);
-    const int tiles = (issued + 1) / 2;  // with at least the K copy issued
-    for (int i = max(0, tiles - kKStages); i < tiles; ++i) drain_wait(bar(kKFull + (i & 1)), (i >> 1) & 1u, status);
-    for (int i = max(0, tiles - kVSt); i < tiles; ++i)
-      if (2 * i + 2 <= issued) drain_wait(bar(kVFull + i % kVSt), (i / kVSt) & 1u, status);
+    for (int i = max(0, k_loads - kKSt); i < k_loads; ++i) drain_wait(bar(kKFull + i % kKSt), (i / kKSt) & 1u, status);
+    for (int i = max(0, v_loads - kVSt); i < v_loads; ++i) drain_wait(bar(kVFull + i % kVSt), (i / kVSt) & 1u, status);
   } else if (warp == 9) {
     // ------------------------------------------------------------ UMMA issuer (one lane)
     if (lane == 0) {
@@ -362,10 +400,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
             }
             if (j < n0 + w.tiles) {
-              ok = mbar_wait(bar(kKFull + (j & 1)), (j >> 1) & 1u, abort_flag, status, kErrFull);
+              ok = mbar_wait(bar(kKFull + j % kKSt), (j / kKSt) & 1u, abort_flag, status, kErrFull);
               if (!ok) break;
               tc_fence_after();
-              mma.s(j & 1, 0, j & 1);
+              mma.s(j & 1, 0, j % kKSt);
               umma_commit(bar(kS + (j & 1)));
             }
           }
@@ -402,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ softmax, few queries
     const int t = warp >> 2;
     const uint32_t s_addr = tmem + 128 * t, o_addr = tmem + 256 + 128 * t;
-    float* rows_o = reinterpret_cast<float*>(smem + kStageOff);  // of group 1: [kMergeRows][kMergePad], then m, l
+    float* rows_o = reinterpret_cast<float*>(smem + kMergeOff);  // of group 1: [kMergeRows][kMergePad], then m, l
     float* rows_ml = rows_o + kMergeRows * kMergePad;
     int n = 0, loaded = 0;  // tiles; units with tiles
     for (int u = 0; (warp & 3) == 0; ++u) {
@@ -414,13 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true, any = false;
       const int end = n + tiles;
       for (int j = n + ((n ^ t) & 1); j < end; j += 2) {
-        const int slot = j & (kRing - 1);
-        ok = warp_wait(bar(kMeta + slot), (j / kRing) & 1u, abort_flag, status, kErrMeta);
+        const int slot = j % kMetaRing;
+        ok = warp_wait(bar(kMeta + slot), (j / kMetaRing) & 1u, abort_flag, status, kErrMeta);
         if (!ok) break;
         const int used = small->meta[slot];
         ok = warp_wait(bar(kS + t), (j >> 1) & 1u, abort_flag, status, kErrS);
         if (!ok) break;
-        if (lane == 0) mbar_arrive(bar(kFree + t));
+        if (lane == 0) mbar_arrive(bar(kFree + j % kRing));
         tc_fence_after();
         uint32_t sr[128];
         tmem_ld32_at<0>(s_addr + 0, sr);
@@ -566,14 +604,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       if (mine) {
         for (int i = 0; i < tiles; ++i, ++nt) {
-          const int slot = (n + i) & (kRing - 1);
-          ok = warp_wait(bar(kMeta + slot), ((n + i) / kRing) & 1u, abort_flag, status, kErrMeta);
+          const int slot = (n + i) % kMetaRing;
+          ok = warp_wait(bar(kMeta + slot), ((n + i) / kMetaRing) & 1u, abort_flag, status, kErrMeta);
           if (!ok) break;
           const int used = small->meta[slot];
           ok = warp_wait(bar(kS + t), nt & 1u, abort_flag, status, kErrS);
           if (!ok) break;
           // The group whose S comes last says that the tile's K is free.
-          if (quarter == 0 && lane == 0 && t == (two ? 1 : 0)) mbar_arrive(bar(kFree + ((n + i) & 1)));
+          if (quarter == 0 && lane == 0 && t == (two ? 1 : 0)) mbar_arrive(bar(kFree + (n + i) % kRing));
           tc_fence_after();
           uint32_t sr[128];
           tmem_ld32_at<0>(s_addr + 0, sr);
