@@ -1020,7 +1020,10 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
     m.block = block[t];
     m.blocks = static_cast<int>((int64_t(len[t]) + block[t] - 1) / block[t]);
     m.head_pairs = (heads[t] + 1) / 2;
-    m.ctas = int64_t(batch) * m.blocks * m.head_pairs;
+    m.warps = 1;
+    while (m.warps < 8 && m.warps * 32 < block[t]) m.warps *= 2;
+    m.items = int64_t(batch) * m.blocks * m.head_pairs;
+    m.ctas = (m.items * m.warps + 7) / 8;
     if (m.ctas == 0) continue;
     if (!x[t] || !aligned16(x[t])) return set_error(PS_B200_ERR_INVALID, "tensor %d null or not 16-byte aligned", t);
     if (!out[t] || !aligned4(out[t])) return set_error(PS_B200_ERR_INVALID, "means %d null or not 4-byte aligned", t);

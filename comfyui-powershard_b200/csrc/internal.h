@@ -176,7 +176,9 @@ struct MeansTensor {
   int len, heads, block;
   int blocks;              // ceil(len / block)
   int head_pairs;          // ceil(heads / 2)
-  int64_t ctas;            // batch * blocks * head_pairs
+  int warps;               // that share a block (1, 2, 4 or 8), about 32 rows each
+  int64_t items;           // batch * blocks * head_pairs
+  int64_t ctas;            // of eight warps
   const int* lens;         // [batch] rows in use, or null: len
   float* out;              // [batch][blocks][heads][128]
 };
