@@ -1083,7 +1083,8 @@ static int block_select(const float* q_means, const float* k_means, int batch, i
   a.blocks = blocks;
   a.counts = counts;
   a.scores = static_cast<float*>(workspace);
-  a.k_sq = a.scores + int64_t(select_units(batch, a.kv_heads, a.group, q_blocks, k_blocks)) * a.group * q_blocks * k_blocks;
+  a.k_sq = reinterpret_cast<uint32_t*>(a.scores + int64_t(select_units(batch, a.kv_heads, a.group, q_blocks, k_blocks)) *
+                                                      a.group * q_blocks * k_blocks);
   return launch_block_select(a, static_cast<cudaStream_t>(stream));
 }
 

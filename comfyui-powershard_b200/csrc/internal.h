@@ -187,7 +187,7 @@ struct MeansArgs {
 };
 int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream);
 
-constexpr int kSelectMaxBlocks = 16384;  // 12 bytes of shared memory each
+constexpr int kSelectMaxBlocks = 16384;  // 8 bytes of shared memory each
 // Pairs of batch row and key head whose scores are held at a time, in at most 64 MB where one fits in that.
 inline int select_units(int64_t batch, int64_t kv_heads, int64_t group, int64_t q_blocks, int64_t k_blocks) {
   const int64_t one = group * q_blocks * k_blocks * 4;
@@ -195,7 +195,7 @@ inline int select_units(int64_t batch, int64_t kv_heads, int64_t group, int64_t 
   n = n < 1 ? 1 : (n > 65535 ? 65535 : n);
   return static_cast<int>(n < batch * kv_heads ? n : batch * kv_heads);
 }
-// Workspace of launch_block_select: the scores of those pairs, and the key means' squared lengths.
+// Workspace of launch_block_select: the scores of those pairs, and the largest of the key means' squared lengths.
 inline int64_t select_score_floats(int64_t batch, int64_t kv_heads, int64_t group, int64_t q_blocks, int64_t k_blocks) {
   return select_units(batch, kv_heads, group, q_blocks, k_blocks) * (group * q_blocks + 1) * k_blocks;
 }
@@ -211,7 +211,7 @@ struct SelectArgs {
   int* blocks;             // [batch][heads][q_blocks][keep]
   int* counts;             // [batch][heads][q_blocks]
   float* scores;           // workspace: [units at a time][group * q_blocks][k_blocks]
-  float* k_sq;             // ... and behind it [units at a time][k_blocks]
+  uint32_t* k_sq;          // ... and behind it, bits of the largest |k|^2 of every 128 key blocks [units][chunks]
   int first_unit;          // set by the launch
   // Queries [batch][len_q][kv_heads * group][128] (16-bit) whose means the kernel takes itself and writes
   // to q_means, or null.

@@ -23,7 +23,6 @@ namespace sparse {
 constexpr int kHeadDim = 128;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kFewBlocks = 4096;  // up to which two warps pick a list, eight beyond
 constexpr int kScoreRows = 64, kScoreKeys = 16 * kWarps;  // of one CTA of score_kernel
 
 template <bool kFp16>
@@ -147,7 +146,7 @@ __device__ __forceinline__ int blocks_in_use(const int* len, int batch, int bloc
 }
 
 // Scores of 64 rows (query blocks of the query heads that share a key head; one
-// list each) against 128 key blocks, and the squared lengths of the key means.
+// list each) against 128 key blocks, and the largest squared length of their means.
 //
 // On the tensor cores: each mean is split into two bf16 terms and the three
 // larger products are summed in 32 bits, which is off by less than E = 2^-15
@@ -165,6 +164,7 @@ __device__ __forceinline__ int blocks_in_use(const int* len, int batch, int bloc
 __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) {
   constexpr int kPad = 32 + 4;  // of a row's 32 (hi, hi, lo, lo): 8 lanes' reads fall in different banks
   __shared__ uint4 qs[kScoreRows * kPad];
+  __shared__ uint32_t longest;  // bits of the largest |k|^2 of this CTA's key blocks
   launch_dependents();
   wait_for_previous();  // the means
   const int rows = a.group * a.q_blocks;  // of one key head
@@ -178,6 +178,8 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
   const int k_blocks = blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks);
   if (a.zeros && blockIdx.x + blockIdx.y + blockIdx.z == 0)
     for (int i = threadIdx.x; i < a.n_zeros; i += kThreads) a.zeros[i] = 0;
+
+  if (threadIdx.x == 0) longest = 0;
 
   // The warp's key means, while the queries' are put in shared memory.
   const int n0 = blockIdx.x * kScoreKeys + warp * 16 + g;
@@ -245,12 +247,17 @@ __global__ void __launch_bounds__(kThreads, 2) score_kernel(const SelectArgs a) 
 
   const int64_t unit = blockIdx.z;
   if (blockIdx.y == 0) {
+    uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 1);
       sq[i] += __shfl_xor_sync(0xffffffffu, sq[i], 2);
-      if (tig == 0 && n0 + 8 * i < a.k_blocks) a.k_sq[unit * a.k_blocks + n0 + 8 * i] = sq[i];
+      most = max(most, __float_as_uint(fabsf(sq[i])));  // NaN is above inf
     }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) atomicMax(&longest, most);
+    __syncthreads();
+    if (threadIdx.x == 0) a.k_sq[unit * gridDim.x + blockIdx.x] = longest;
   }
   float* scores = a.scores + (unit * rows + row0) * a.k_blocks;
 #pragma unroll 2
@@ -292,109 +299,21 @@ struct CtaSum {
   }
 };
 
-// The keep-th largest of the keys that are not 0 (more than keep): chosen are
-// those above floor + 1 and the first `ties` that equal it; ties 0: all above
-// floor.  `lo` and `hi` are the least and the greatest key, `n` how many.  The
-// range is cut first at `guess`, then where the counts at its ends put the
-// keep-th on a straight line, every fourth time (and for 64-bit keys) in the
-// middle, until exactly `keep` lie above the cut: 4.3 counts of 1182 normal
-// scores, against 15 with bisection of the keys alone.
-template <typename Key, int kWarps>
-__device__ __forceinline__ void kth_largest(const Key* key, int begin, int end, int keep, Key lo, Key hi, int n,
-                                            float guess, CtaSum<kWarps>& sum, Key& floor, int& ties) {
-  const int lane = threadIdx.x & 31;
-  int above = 0;  // keys above hi; n: keys from lo up
-  ties = 0;
-  for (int round = 1; lo < hi; ++round) {
-    Key mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
-    if constexpr (sizeof(Key) == 4) {
-      const float a = of_key(lo), b = of_key(hi);
-      const float f = round == 1 ? guess
-                                 : a + (b - a) * __fdividef(static_cast<float>(n - keep), static_cast<float>(n - above));
-      if ((round & 3) && isfinite(f)) mid = min(max(order_key(f), lo + 1), hi);
-    }
-    int c = 0;
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) c += key[i] >= mid;
-    c = sum(c);
-    if (c == keep) {
-      floor = mid - 1;
-      return;
-    }
-    if (c > keep) {
-      lo = mid;
-      n = c;
-    } else {
-      hi = mid - 1;
-      above = c;
-    }
-  }
-  floor = lo - 1;
-  ties = keep - above;
-}
-
-// Writes the chosen indices in ascending order; each warp has its range.
-template <typename Key, int kWarps>
-__device__ __forceinline__ void write_list(const Key* key, int begin, int end, Key floor, int ties, int keep, int* out,
-                                           int* count, int (*part)[kWarps]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned below = (1u << lane) - 1;
-  const Key equal = floor + 1;
-  // Ahead of this warp's range: keys above the tied one, and tied ones.
-  int more = 0, same = 0;
-#pragma unroll 4
-  for (int i = begin + lane; i < end; i += 32) {
-    const Key k = key[i];
-    const bool tied = ties > 0 && k == equal;
-    same += tied;
-    more += k > floor && !tied;
-  }
-  more = __reduce_add_sync(0xffffffffu, more);
-  same = __reduce_add_sync(0xffffffffu, same);
-  __syncthreads();  // `part` may still be read
-  if (lane == 0) {
-    part[0][warp] = more;
-    part[1][warp] = same;
-  }
-  __syncthreads();
-  int done = 0, left = ties, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) {
-      done = total;
-      left = ties;
-    }
-    const int s = min(ties, part[1][w]);
-    total += part[0][w] + s;
-    ties -= s;
-  }
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const Key k = i < end ? key[i] : Key(0);
-    bool take = k > floor;
-    if (same > 0) {  // of this warp's range
-      const bool tied = k == equal;
-      const unsigned m = __ballot_sync(0xffffffffu, tied);
-      if (tied) take = __popc(m & below) < left;
-      left -= min(left, __popc(m));
-    }
-    const unsigned m = __ballot_sync(0xffffffffu, take);
-    if (take) out[done + __popc(m & below)] = i;
-    done += __popc(m);
-  }
-  for (int i = total + threadIdx.x; i < keep; i += 32 * kWarps) out[i] = -1;
-  if (threadIdx.x == 0) *count = total;
-}
-
-// One CTA picks one list.  With T the keep-th largest of the scores, a block
-// above T + 2E is chosen and one below T - 2E is not, in 64 bits too; only the
-// blocks between (the T block alone, in three lists of four) are scored again in
-// 64 bits.
-template <int kWarps>
+// One CTA picks one list; a thread holds kPer of the scores, as keys in their
+// order (block (warp * kPer + j) * 32 + lane).
+//
+// With T the keep-th largest score, a block above T + 2E is chosen and one
+// below T - 2E is not, in 64 bits too; only the blocks between (the T block
+// alone, in two lists of three) are scored again in 64 bits.
+//
+// T is found by counting the keys above a cut, first where the keep-th of as
+// many normal scores lies, then where the counts at the ends put it on a
+// straight line, every fourth time in the middle of the key range, until
+// exactly `keep` lie above: 4.3 counts of 1182 normal scores, against 15 with
+// bisection alone.
+template <int kWarps, int kPer>
 __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned long long* exact = reinterpret_cast<unsigned long long*>(smem);  // [k_blocks], with many ties only
-  uint32_t* key = reinterpret_cast<uint32_t*>(exact + a.k_blocks);          // [k_blocks]
+  extern __shared__ __align__(16) unsigned long long exact[];  // [k_blocks], used with many ties only
   __shared__ int part[2][kWarps];
   __shared__ uint32_t ends[3][kWarps];
   __shared__ float sums[2][kWarps];
@@ -404,94 +323,117 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
   launch_dependents();
   wait_for_previous();  // the scores
   const int rows = a.group * a.q_blocks;
-  const int unit = blockIdx.x / rows, row = blockIdx.x % rows;
-  const int kv = (a.first_unit + unit) % a.kv_heads, batch = (a.first_unit + unit) / a.kv_heads;
+  const int unit = blockIdx.x / rows, row = blockIdx.x - unit * rows;
+  const int batch = (a.first_unit + unit) / a.kv_heads, kv = a.first_unit + unit - batch * a.kv_heads;
   const int heads = a.kv_heads * a.group;
   const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
   const int64_t list = (static_cast<int64_t>(batch) * heads + h) * a.q_blocks + qb;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool in_use = qb < blocks_in_use(a.q_len, batch, a.query_block, a.q_blocks);
   const int n_used = in_use ? blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks) : 0;
-  // Each warp owns a range of the blocks, in whole 32s.
-  const int range = ((a.k_blocks + 31) / 32 + kWarps - 1) / kWarps * 32;
-  const int begin = min(warp * range, a.k_blocks), end = min(begin + range, a.k_blocks);
+  const int first = warp * kPer * 32 + lane;  // block of the thread's first key
 
-  const float4 q = __ldg(reinterpret_cast<const float4*>(a.q_means) +
-                         ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
   const float* score = a.scores + (static_cast<int64_t>(unit) * rows + row) * a.k_blocks;
-  const float* k_sq = a.k_sq + static_cast<int64_t>(unit) * a.k_blocks;
   const uint8_t* allowed = a.allowed ? a.allowed + batch * a.allowed_st[0] + h * a.allowed_st[1] + qb * a.allowed_st[2]
                                      : nullptr;
-  uint32_t least = ~0u, most = 0, longest = 0;
+  uint32_t key[kPer];
+  uint32_t least = ~0u, most = 0;
   int n_may = 0;
   float s1 = 0, s2 = 0;  // sums of the scores and their squares
-#pragma unroll 4
-  for (int i = begin + lane; i < end; i += 32) {
-    uint32_t k = 0;
-    if (i < n_used && (!allowed || allowed[i * a.allowed_st[3]] != 0)) {
-      const float x = __ldg(score + i);
-      k = order_key(x);
-      s1 += x;
-      s2 = fmaf(x, x, s2);
-      longest = max(longest, __float_as_uint(fabsf(__ldg(k_sq + i))));  // NaN is above inf
+  {
+    float x[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = first + 32 * j < n_used ? __ldg(score + first + 32 * j) : 0.f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = first + 32 * j;
+      const bool may = i < n_used && (!allowed || allowed[i * a.allowed_st[3]] != 0);
+      key[j] = may ? order_key(x[j]) : 0u;
+      n_may += may;
+      s1 += may ? x[j] : 0.f;
+      s2 += may ? x[j] * x[j] : 0.f;
+      least = min(least, key[j] - 1);  // 0 becomes the largest
+      most = max(most, key[j]);
     }
-    key[i] = k;
-    n_may += k != 0;
-    least = min(least, k - 1);  // 0 becomes the largest
-    most = max(most, k);
   }
   least = __reduce_min_sync(0xffffffffu, least);
   most = __reduce_max_sync(0xffffffffu, most);
-  longest = __reduce_max_sync(0xffffffffu, longest);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     s1 += __shfl_xor_sync(0xffffffffu, s1, o);
     s2 += __shfl_xor_sync(0xffffffffu, s2, o);
   }
   if (lane == 0) {
-    sums[0][warp] = s1;
-    sums[1][warp] = s2;
     ends[0][warp] = least;
     ends[1][warp] = most;
-    ends[2][warp] = longest;
+    sums[0][warp] = s1;
+    sums[1][warp] = s2;
   }
   if (threadIdx.x == 0) n_open = 0;
   CtaSum<kWarps> sum{part, 0};
   n_may = sum(n_may);  // and a barrier
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    least = min(least, ends[0][w]);
-    most = max(most, ends[1][w]);
-    longest = max(longest, ends[2][w]);
-  }
-  ++least;
 
-  int* out = a.blocks + list * a.keep;
-  uint32_t floor = 0;
-  if (n_may > a.keep) {
-    int ties;
-    // Where the keep-th would lie if the scores were normal.
+  unsigned long long chosen = 0;  // bit j: key j
+  if (n_may <= a.keep) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) chosen |= static_cast<unsigned long long>(key[j] != 0) << j;
+  } else {
+    // T, the smallest key above `floor`.
     s1 = s2 = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
+      least = min(least, ends[0][w]);
+      most = max(most, ends[1][w]);
       s1 += sums[0][w];
       s2 += sums[1][w];
     }
-    const float part_kept = __fdividef(static_cast<float>(a.keep), static_cast<float>(n_may));
     s1 = __fdividef(s1, static_cast<float>(n_may));
     const float spread = sqrtf(fmaxf(__fdividef(s2, static_cast<float>(n_may)) - s1 * s1, 0.f));
-    kth_largest(key, begin, end, a.keep, least, most, n_may, s1 - spread * normcdfinvf(part_kept), sum, floor, ties);
-    uint32_t kth = ~0u;  // T: the smallest key above floor
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) kth = key[i] > floor ? min(kth, key[i]) : kth;
+    float f = s1 - spread * normcdfinvf(__fdividef(static_cast<float>(a.keep), static_cast<float>(n_may)));
+    uint32_t lo = least + 1, hi = most, floor = 0;
+    int from_lo = n_may, above = 0;  // keys from lo up, keys above hi
+    for (int round = 1;; ++round) {
+      if (lo >= hi) {
+        floor = lo - 1;
+        break;
+      }
+      uint32_t mid = lo + ((hi - lo) >> 1) + 1;  // lo < mid <= hi
+      if ((round & 3) && isfinite(f)) mid = min(max(order_key(f), lo + 1), hi);
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) c += key[j] >= mid;
+      c = sum(c);
+      if (c == a.keep) {
+        floor = mid - 1;
+        break;
+      }
+      if (c > a.keep) {
+        lo = mid;
+        from_lo = c;
+      } else {
+        hi = mid - 1;
+        above = c;
+      }
+      const float u = of_key(lo), v = of_key(hi);
+      f = u + (v - u) * __fdividef(static_cast<float>(from_lo - a.keep), static_cast<float>(from_lo - above));
+    }
+    uint32_t kth = ~0u;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) kth = key[j] > floor ? min(kth, key[j]) : kth;
     kth = __reduce_min_sync(0xffffffffu, kth);
+    if (lane == 0) ends[2][warp] = kth;
+    const float4 q = __ldg(reinterpret_cast<const float4*>(a.q_means) +
+                           ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * (kHeadDim / 4) + lane);
     float q_sq = fmaf(q.x, q.x, fmaf(q.y, q.y, fmaf(q.z, q.z, q.w * q.w)));
 #pragma unroll
     for (int o = 16; o; o >>= 1) q_sq += __shfl_xor_sync(0xffffffffu, q_sq, o);
-    if (lane == 0) ends[0][warp] = kth;
+    uint32_t longest = 0;
+    const int k_chunks = (a.k_blocks + kScoreKeys - 1) / kScoreKeys;
+    for (int i = lane; i < k_chunks; i += 32) longest = max(longest, __ldg(a.k_sq + static_cast<int64_t>(unit) * k_chunks + i));
+    longest = __reduce_max_sync(0xffffffffu, longest);
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) kth = min(kth, ends[0][w]);
+    for (int w = 0; w < kWarps; ++w) kth = min(kth, ends[2][w]);
     const float T = of_key(kth);
     const float len_q = sqrtf(q_sq), len_k = sqrtf(__uint_as_float(longest));
     const float E2 = 6.103515625e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-14, 2^-110
@@ -501,22 +443,21 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
       hi_key = order_key(T + E2);
     }
     int sure = 0;
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) {
-      const uint32_t k = key[i];
-      sure += k > hi_key;
-      if (k >= lo_key && k <= hi_key) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      sure += key[j] > hi_key;
+      chosen |= static_cast<unsigned long long>(key[j] > hi_key) << j;
+      if (key[j] >= lo_key && key[j] <= hi_key) {
         const int at = atomicAdd(&n_open, 1);  // in any order: they are ranked below
-        if (at < 32) open_at[at] = i;
+        if (at < 32) open_at[at] = first + 32 * j;
       }
     }
     const int wanted = a.keep - sum(sure);
     const int open = n_open;
     const float4* km = reinterpret_cast<const float4*>(a.k_means) +
                        (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4);
-    const int64_t kstep = static_cast<int64_t>(a.kv_heads) * (kHeadDim / 4);
     auto score64 = [&](int i) {  // by one warp
-      const float4 k = __ldg(km + i * kstep + lane);
+      const float4 k = __ldg(km + static_cast<int64_t>(i) * a.kv_heads * (kHeadDim / 4) + lane);
       double d = fma(double(q.x), double(k.x), double(q.y) * double(k.y)) +
                  fma(double(q.z), double(k.z), double(q.w) * double(k.w));
 #pragma unroll
@@ -524,38 +465,99 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
       return order_key(d);
     };
     if (open == wanted) {
-      floor = lo_key - 1;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) chosen |= static_cast<unsigned long long>(key[j] >= lo_key) << j;
     } else if (open <= 32) {
       for (int e = warp; e < open; e += kWarps) {
         const unsigned long long k = score64(open_at[e]);
         if (lane == 0) open_key[e] = k;
       }
       __syncthreads();
-      if (threadIdx.x < open) {
-        const int at = open_at[threadIdx.x];
-        const unsigned long long mine = open_key[threadIdx.x];
+      for (int e = 0; e < open; ++e) {
+        // Every thread ranks every open block and keeps its own.
+        const int at = open_at[e];
         int better = 0;
-        for (int e = 0; e < open; ++e) better += open_key[e] > mine || (open_key[e] == mine && open_at[e] < at);
-        key[at] = better < wanted ? ~0u : 0u;
+        for (int o = lane; o < open; o += 32)
+          better += open_key[o] > open_key[e] || (open_key[o] == open_key[e] && open_at[o] < at);
+        better = __reduce_add_sync(0xffffffffu, better);
+        const int j = (at - first) >> 5;
+        if (better < wanted && ((at ^ first) & 31) == 0 && j >= 0 && j < kPer) chosen |= 1ull << j;
       }
-      __syncthreads();
-      floor = hi_key;
     } else {
-      // Many equal or overflowing scores: all of them in 64 bits.
-      for (int i = begin; i < end; ++i) {
-        const uint32_t k = key[i];
-        unsigned long long e = k > hi_key ? ~0ull : 0ull;
-        if (k >= lo_key && k <= hi_key) e = score64(i);
-        if (lane == 0) exact[i] = e;
+      // Many equal or overflowing scores: all that are open in 64 bits, and
+      // the bisection of 64-bit keys (0: not open) for the wanted-th of them.
+      for (int j = 0; j < kPer; ++j) {
+        const int i0 = warp * kPer * 32 + 32 * j;
+        for (int l = 0; l < 32 && i0 + l < a.k_blocks; ++l) {
+          const uint32_t k = __shfl_sync(0xffffffffu, key[j], l);
+          unsigned long long e = 0;
+          if (k >= lo_key && k <= hi_key) e = score64(i0 + l);
+          if (lane == 0) exact[i0 + l] = e;
+        }
       }
+      __syncwarp();
+      const int begin = min(warp * kPer * 32, a.k_blocks), end = min(begin + kPer * 32, a.k_blocks);
+      unsigned long long lo64 = 1, hi64 = ~0ull;
+      int left = 0, over = 0;  // ties to be chosen; keys above hi64
+      bool found = false;
+      while (lo64 < hi64) {
+        const unsigned long long mid = lo64 + ((hi64 - lo64) >> 1) + 1;
+        int c = 0;
+        for (int i = begin + lane; i < end; i += 32) c += exact[i] >= mid;
+        c = sum(c);
+        if (c == wanted) {
+          lo64 = mid;
+          found = true;
+          break;
+        }
+        if (c > wanted) {
+          lo64 = mid;
+        } else {
+          hi64 = mid - 1;
+          over = c;
+        }
+      }
+      // Chosen: keys above lo64, and as many that equal it as are still wanted
+      // (all of them where the cut was exact), by index across the warps.
+      int same = 0;
+      for (int i = begin + lane; i < end; i += 32) same += exact[i] == lo64;
+      same = __reduce_add_sync(0xffffffffu, same);
+      __syncthreads();  // `part` may still be read
+      if (lane == 0) part[0][warp] = same;
       __syncthreads();
-      unsigned long long floor64;
-      kth_largest(exact, begin, end, a.keep, 1ull, ~0ull, n_may, 0.f, sum, floor64, ties);
-      write_list(exact, begin, end, floor64, ties, a.keep, out, a.counts + list, part);
-      return;
+      left = found ? a.k_blocks : wanted - over;
+      for (int w = 0; w < warp; ++w) left = max(left - part[0][w], 0);
+      for (int j = 0; j < kPer; ++j) {
+        const int i = first + 32 * j;
+        const unsigned long long e = i < end ? exact[i] : 0ull;
+        const unsigned m = __ballot_sync(0xffffffffu, e == lo64);
+        if (e > lo64 || (e == lo64 && __popc(m & ((1u << lane) - 1)) < left)) chosen |= 1ull << j;
+        left = max(left - __popc(m), 0);
+      }
     }
   }
-  write_list(key, begin, end, floor, 0, a.keep, out, a.counts + list, part);
+
+  // The chosen in ascending order.
+  int mine = __reduce_add_sync(0xffffffffu, __popcll(chosen));
+  __syncthreads();  // `part` may still be read
+  if (lane == 0) part[0][warp] = mine;
+  __syncthreads();
+  int done = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) done += part[0][w];
+    total += part[0][w];
+  }
+  int* out = a.blocks + list * a.keep;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const bool take = (chosen >> j) & 1;
+    const unsigned m = __ballot_sync(0xffffffffu, take);
+    if (take) out[done + __popc(m & ((1u << lane) - 1))] = first + 32 * j;
+    done += __popc(m);
+  }
+  for (int i = total + threadIdx.x; i < a.keep; i += 32 * kWarps) out[i] = -1;
+  if (threadIdx.x == 0) a.counts[list] = total;
 }
 
 }  // namespace sparse
@@ -577,15 +579,18 @@ int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream) {
 
 int launch_block_select(SelectArgs a, cudaStream_t stream) {
   using namespace sparse;
-  const size_t smem = size_t(a.k_blocks) * 12;
+  // Warps and keys a thread by the number of key blocks: 20 keys in registers
+  // as long as eight warps hold the list, 64 beyond.
+  const size_t smem = size_t(a.k_blocks) * 8;
+  const int form = a.k_blocks <= 2 * 20 * 32 ? 0 : a.k_blocks <= 8 * 20 * 32 ? 1 : 2;
+  void (*const pick)(const SelectArgs) = form == 0 ? pick_kernel<2, 20> : form == 1 ? pick_kernel<8, 20> : pick_kernel<8, 64>;
+  static_assert(8 * 64 * 32 == kSelectMaxBlocks, "the largest list");
   static bool done[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-  if (!done[dev]) {
-    cudaError_t err = cudaFuncSetAttribute(pick_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           kSelectMaxBlocks * 12);
-    if (err == cudaSuccess)
-      err = cudaFuncSetAttribute(pick_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewBlocks * 12);
+  if (form == 2 && !done[dev]) {  // the others stay below 48 KB
+    const cudaError_t err =
+        cudaFuncSetAttribute(pick_kernel<8, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectMaxBlocks * 8);
     if (err != cudaSuccess) return set_cuda_error("block_select: cudaFuncSetAttribute", err);
     done[dev] = true;
   }
@@ -601,9 +606,7 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
     cudaError_t err = launch_after(score_kernel, grid, dim3(kThreads), 0, stream, a.after_means && a.first_unit == 0, a);
     if (err != cudaSuccess) return set_cuda_error("block_select scores launch", err);
     count_launch();
-    const dim3 lists(static_cast<unsigned>(n * rows));
-    err = a.k_blocks <= kFewBlocks ? launch_after(pick_kernel<2>, lists, dim3(64), smem, stream, true, a)
-                                   : launch_after(pick_kernel<8>, lists, dim3(256), smem, stream, true, a);
+    err = launch_after(pick, dim3(static_cast<unsigned>(n * rows)), dim3(form == 0 ? 64 : 256), smem, stream, true, a);
     if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
     count_launch();
   }
