@@ -692,23 +692,34 @@ def block_means(tensors, blocks, lengths, means):
     [B, ceil(L/block), H, 128] each, written (a block without rows: zeros)."""
     lib = _lib.load()
     x = tensors[0]
-    device, batch = x.device, x.shape[0]
-    strides, lens = [], []
-    for t, block, n, out in zip(tensors, blocks, lengths, means):
+    device, batch, dtype = x.device, x.shape[0], x.dtype
+    addresses, strides, lens, rows, heads, out = [], [], [], [], [], []
+    for t, block, n, m in zip(tensors, blocks, lengths, means):
         strides += _row_strides(t, "block_means")
         if block < 1:
             raise ValueError(f"block_means: blocks of {block} rows")
-        if t.dtype != x.dtype or t.shape[0] != batch or t.device != device:
+        b, length, h, d = t.shape
+        if t.dtype != dtype or b != batch or t.device != device:
             raise ValueError("block_means: the tensors need one dtype, batch and device")
-        shape = (batch, -(-t.shape[1] // block), t.shape[2], t.shape[3])
-        if tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or out.device != device:
-            raise ValueError(f"block_means: means must be contiguous fp32 {shape} on {device}")
+        if (m.shape != (batch, -(-length // block), h, d) or m.dtype != torch.float32 or not m.is_contiguous()
+                or m.device != device):
+            raise ValueError(f"block_means: means must be contiguous fp32 {(batch, -(-length // block), h, d)} on {device}")
+        addresses.append(t.data_ptr())
+        rows.append(length)
+        heads.append(h)
+        out.append(m.data_ptr())
         lens.append(_lengths_arg(n, batch, device, "block_means lengths") or 0)
+    n = len(tensors)
     rc = lib.ps_b200_block_means(
-        len(tensors), _lib.ptrs([t.data_ptr() for t in tensors]), _lib.i64(strides), _lib.dtype_code(x.dtype), batch,
-        _lib.i32([t.shape[1] for t in tensors]), _lib.i32([t.shape[2] for t in tensors]), x.shape[3], _lib.i32(blocks),
-        _lib.ptrs(lens), _lib.ptrs([t.data_ptr() for t in means]), _lib.stream_handle(device))
+        n, struct.pack(f"{n}P", *addresses), struct.pack(f"{3 * n}q", *strides), _lib.dtype_code(dtype), batch,
+        struct.pack(f"{n}i", *rows), struct.pack(f"{n}i", *heads), d, struct.pack(f"{n}i", *blocks),
+        struct.pack(f"{n}P", *lens), struct.pack(f"{n}P", *out), _lib.stream_handle(device))
     _lib.check(rc, "ps_b200_block_means")
+
+
+@functools.lru_cache(maxsize=256)
+def _select_workspace_bytes(*sizes) -> int:
+    return _lib.load().ps_b200_block_select_workspace_bytes(*sizes)
 
 
 def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, key_block: int, allowed=None,
@@ -729,14 +740,14 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
     if k_means.shape[0] != batch or k_means.shape[3] != dim:
         raise ValueError("block_select: q_means and k_means differ in batch or head_dim")
     for t, shape, name in ((blocks, (batch, hq, nq, keep), "blocks"), (counts, (batch, hq, nq), "counts")):
-        if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+        if t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
             raise ValueError(f"block_select {name}: expected contiguous int32 {shape} on {device}")
     mask, strides = None, None
     if allowed is not None:
         if allowed.dtype != torch.bool or tuple(allowed.shape) != (batch, hq, nq, nk) or allowed.device != device:
             raise ValueError(f"block_select: allowed must be bool {(batch, hq, nq, nk)} on {device}")
-        mask, strides = allowed.data_ptr(), _lib.i64(allowed.stride())
-    n = lib.ps_b200_block_select_workspace_bytes(batch, hq, hk, nq, nk) if hk else 0
+        mask, strides = allowed.data_ptr(), struct.pack("4q", *allowed.stride())
+    n = _select_workspace_bytes(batch, hq, hk, nq, nk) if hk else 0
     workspace = torch.empty(n, dtype=torch.uint8, device=device)
     rc = lib.ps_b200_block_select(
         q_means.data_ptr(), k_means.data_ptr(), batch, hq, hk, dim, nq, nk, keep, mask, strides,
@@ -749,9 +760,14 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
 def sparse_attention_workspace(batch: int, heads: int, len_q: int, list_len: int, key_block: int, device):
     """Scratch of one ``sparse_attention`` call of these sizes on ``device``
     (None when it needs none); one per call in flight."""
-    with torch.cuda.device(device):
-        n = _lib.load().ps_b200_sparse_attn_workspace_bytes(batch, heads, len_q, list_len, key_block)
+    n = _sparse_workspace_bytes(device.index, batch, heads, len_q, list_len, key_block)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+@functools.lru_cache(maxsize=256)
+def _sparse_workspace_bytes(device_index: int, *sizes) -> int:
+    with torch.cuda.device(device_index):
+        return _lib.load().ps_b200_sparse_attn_workspace_bytes(*sizes)
 
 
 def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: int, scale: float,
@@ -763,7 +779,7 @@ def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: 
     key), counts int32 [B, Hq, ceil(Lq/query_block)] entries in use or None."""
     lib = _lib.load()
     device = q.device
-    st = [_lib.i64(_row_strides(t, f"sparse attention {n}")) for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out"))]
+    st = [_THREE.pack(*_row_strides(t, "sparse attention")) for t in (q, k, v, out)]
     batch, lq, hq, dim = q.shape
     lk, hk = k.shape[1:3]
     if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != dim or out.shape != q.shape:
@@ -790,6 +806,7 @@ def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: 
 
 
 # ps_b200_sparse_call: ten addresses, the strides, eleven sizes and the scale.
+_THREE = struct.Struct("3q")
 _SPARSE_CALL = struct.Struct("@10P16q11qd")
 _NO_STRIDES = (0, 0, 0, 0)
 

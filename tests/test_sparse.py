@@ -127,7 +127,8 @@ def test_refusals_before_any_launch():
 def test_entries_validate_on_the_host():
     from powershard_b200 import _lib
     lib = _lib.load()
-    st = _lib.i64([0, 256, 128])
+    import struct
+    st = struct.pack("3q", 0, 256, 128)
 
     def fwd(dtype=_lib.BF16, heads=2, kv=2, dim=128, lq=300, lk=300, blocks=16, n=4, qb=256, kb=64, scale=0.1, q=16,
             ws=None):
@@ -169,8 +170,9 @@ def test_entries_validate_on_the_host():
     assert select(ws=None) == _lib.ERR_INVALID and select(nbytes=8) == _lib.ERR_INVALID
 
     def means(n=1, dtype=_lib.BF16, dim=128, block=64, length=100, x=16, stride=128):
-        return lib.ps_b200_block_means(n, _lib.ptrs([x]), _lib.i64([0, stride, 128]), dtype, 1, _lib.i32([length]),
-                                       _lib.i32([1]), dim, _lib.i32([block]), None, _lib.ptrs([16]), None)
+        return lib.ps_b200_block_means(n, struct.pack("P", x), struct.pack("3q", 0, stride, 128), dtype, 1,
+                                       struct.pack("i", length), struct.pack("i", 1), dim, struct.pack("i", block), None,
+                                       struct.pack("P", 16), None)
 
     assert means(n=3) == _lib.ERR_INVALID and means(block=0) == _lib.ERR_INVALID and means(x=24) == _lib.ERR_INVALID
     assert means(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED and means(dim=64) == _lib.ERR_UNSUPPORTED
