@@ -53,10 +53,17 @@ def _on(device: torch.device):
 
 
 def _broadcast(allowed, shape):
-    if torch.broadcast_shapes(allowed.shape, shape) != shape:
+    try:
+        return allowed.broadcast_to(shape)
+    except RuntimeError as error:
         raise ValueError(f"allowed {tuple(allowed.shape)} does not broadcast to {shape} "
-                         "(batch, heads, query blocks, key blocks)")
-    return allowed.broadcast_to(shape)
+                         "(batch, heads, query blocks, key blocks)") from error
+
+
+def _no_grad(*tensors):
+    """The kernels run forward only: a call that autograd would record is refused."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise UnsupportedAttention("b200_sparse: forward only, an input requires grad")
 
 
 def block_means(x, block: int, lengths=None):
@@ -118,6 +125,7 @@ def sparse_attention(q, k, v, blocks, counts=None, *, query_block: int = QUERY_B
         ops._check16(t, f"sparse_attention {name}")
         if t.dim() != 4:
             raise ValueError(f"sparse_attention {name}: expected [B, L, H, D], got {tuple(t.shape)}")
+    _no_grad(q, k, v)
     status = _status_for(q.device)
     status.poll()
     q, k, v = _readable(q), _readable(k), _readable(v)
@@ -153,6 +161,7 @@ class SparseProvider(B200Provider):
         super().check(q, k, v, o)
         if o.softmax_scale is not None and not o.softmax_scale > 0:
             raise UnsupportedAttention("b200_sparse: the selection ranks by a positive softmax_scale")
+        _no_grad(q, k, v)
 
     def blocks_kept(self, key_blocks: int) -> int:
         """Key blocks each query block attends, of ``key_blocks``."""

@@ -360,6 +360,14 @@ def test_arguments_are_checked(cuda_lib):
     with pytest.raises(ValueError):
         sparse.SparseProvider(1)(x, x, x, key_means=torch.zeros(1, 2, 2, 128, device=DEV))  # of another length
     assert sparse.SparseProvider(1)(x[:, :0], x, x).shape == (1, 0, 2, 128)
+    from powershard_b200.contract import UnsupportedAttention
+    grad = x.clone().requires_grad_()
+    with pytest.raises(UnsupportedAttention):
+        sparse.SparseProvider(1)(x, grad, x)
+    with pytest.raises(UnsupportedAttention):
+        sparse.sparse_attention(grad, x, x, ok)
+    with torch.no_grad():
+        assert torch.equal(sparse.SparseProvider(1)(x, grad, x), sparse.SparseProvider(1)(x, x, x))
 
 
 @pytest.mark.gpu
