@@ -255,10 +255,16 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
   return launch_attention(tq, tk, tv, tqp, tkp, tvp, a, units, fp16, static_cast<cudaStream_t>(stream));
 }
 
-// How block-sparse attention is cut into CTAs: the last, partial wave's units
-// (query tile pair, head, batch) run as `split` CTAs each over parts of their
-// lists, at least two key tiles a part by the lists' full length (one for few
-// queries, where a part is mostly waiting for its tiles).
+// How block-sparse attention is cut into CTAs: the units (query tile pair,
+// head, batch) of the last, partial wave run in `split` parts of their lists
+// each where that ends sooner.  The time of that wave, from measurements (B200,
+// us): a key tile 2.0, a unit or part 3 more; parts cost 6 for the kernel that
+// merges them and 0.064 each for their traffic (2 x 64 KB written and read).
+// Measured at 44 units left over (192 on 148 SMs): 8 tiles 44.3 us split in
+// three, 41.1 whole; 16 tiles 64.9 and 70.4; 32 tiles 103 and 129.  80 units of
+// 64 tiles: 115 in three, 127 whole.  Few queries (a tile 1.0, a part 2.5, 1.5
+// for the merge) are bound by the keys they read once every SM has a part: 40
+// units of 60 tiles 35.6 in three, 42.8 in seven.
 struct SparsePlan {
   int64_t units, rem;
   int split;
@@ -270,13 +276,21 @@ SparsePlan sparse_plan(int64_t batch, int64_t heads, int64_t len_q, int64_t list
   p.units = (len_q + 255) / 256 * heads * batch;
   p.rem = p.units % sms;
   p.split = 1;
-  if (p.rem > 0) {
-    const int64_t tiles = (list_len * key_block + 127) / 128;
-    int64_t split = sms / p.rem;
-    const int64_t most = len_q <= kMergeRows ? tiles : tiles / 2;
-    split = split < most ? split : most;
-    split = split < kMaxSparseSplit ? split : kMaxSparseSplit;
-    if (split >= 2) p.split = static_cast<int>(split);
+  const int64_t tiles = (list_len * key_block + 127) / 128;
+  const bool few = len_q <= kMergeRows;
+  const double tile = few ? 1.0 : 2.0, part = few ? 2.5 : 3.0;
+  double best = 0;
+  int64_t most = few ? (p.rem > 0 ? sms / p.rem : 1) : tiles / 2 + 1;
+  most = most < tiles ? most : tiles;
+  most = most < kMaxSparseSplit ? most : kMaxSparseSplit;
+  for (int64_t split = 1; p.rem > 0 && split <= most; ++split) {
+    const int64_t rounds = (p.rem * split + sms - 1) / sms;
+    const double merge = split == 1 ? 0 : few ? 1.5 : 6 + 0.064 * double(p.rem * split);
+    const double time = double(rounds) * (double(tiles) / double(split) * tile + part) + merge;
+    if (split == 1 || time < best) {
+      best = time;
+      p.split = static_cast<int>(split);
+    }
   }
   return p;
 }
