@@ -183,6 +183,23 @@ def test_strided_rows_and_a_shared_pool(cuda_lib):
     assert not pool[0].any()
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_lib):
+    """A pool of more than 2^32 codes: rows on its last pages."""
+    pages = 2 ** 32 // (256 * 16 * 128) + 3
+    cache = new_cache(pages, 256, 16, 128, torch.int8)
+    assert cache.k.numel() > 2 ** 32
+    k, v = rows(50, 1, 300, 16, 128), rows(51, 1, 300, 16, 128)
+    table = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device=DEV)
+    cache.write(k.to(DEV), v.to(DEV), table)
+    out = [torch.empty(1, 300, 16, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    cache.read(table, lens(300).to(DEV), *out)
+    for x, y in ((k, out[0]), (v, out[1])):
+        codes, s = quantise(x, torch.int8)
+        assert torch.equal(y.cpu(), (codes.float() * s[..., None]).to(torch.bfloat16))
+    assert not cache.k[:pages - 2].any()
+
+
 # ------------------------------------------------------------------ the operators together
 def ref_streaming(q, k, v, keep, key_block, q_len, k_len):
     from test_sparse import ref_provider

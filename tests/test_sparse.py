@@ -462,3 +462,70 @@ def test_results_do_not_depend_on_what_memory_held(cuda_lib):
     del junk
     b = p(q, k, v, query_lengths=used, key_lengths=used)
     assert torch.equal(a, b) and not b[1].any()
+
+
+@pytest.mark.gpu
+def test_select_in_several_chunks(cuda_lib):
+    """More scores than are held at a time, for a batch with shared key heads."""
+    from powershard_b200 import sparse
+    g = torch.Generator(device=DEV).manual_seed(31)
+    qm = torch.randn(2, 300, 12, 128, device=DEV, generator=g)
+    km = torch.randn(2, 4000, 4, 128, device=DEV, generator=g)
+    used = lens(4000 * 64 - 3, 77 * 64).to(DEV)
+    blocks, counts = sparse.select_blocks(qm, km, 111, key_block=64, key_lengths=used, query_lengths=lens(76800, 70000).to(DEV))
+    score = torch.einsum("bqghd,bkgd->bghqk", qm.double().view(2, 300, 4, 3, 128), km.double()).reshape(2, 12, 300, 4000)
+    score[1, ..., 77:] = -math.inf
+    best = score.sort(dim=-1, descending=True, stable=True).indices[..., :111]
+    best[1, ..., 77:] = 4000
+    best = best.sort(-1).values
+    best[best == 4000] = -1
+    best[1, :, -(-70000 // 256):] = -1
+    assert torch.equal(blocks.long(), best)
+    assert torch.equal(counts.long(), (best >= 0).sum(-1))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_lib):
+    """Keys and values of more than 2^32 bytes and 2^31 elements: means and attention at their far end."""
+    from powershard_b200 import sparse
+    n, heads = 1_100_000, 16
+    g = torch.Generator(device=DEV).manual_seed(32)
+    k, v = (torch.zeros(1, n, heads, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    k[:, -5000:].normal_(generator=g)
+    v[:, -5000:].normal_(generator=g)
+    q = torch.randn(1, 300, heads, 128, dtype=torch.bfloat16, device=DEV, generator=g)
+    means = sparse.block_means(k, 128)
+    nk = means.shape[1]
+    last = ref_means(k[:, (nk - 2) * 128:].cpu(), 128)
+    assert ((means[:, -2:].double().cpu() - last).abs() <= 2.0 ** -22).all() and not means[:, :nk - 60].any()
+    blocks = torch.tensor([0, nk - 30, nk - 2, nk - 1], dtype=torch.int32).expand(1, heads, 2, 4).contiguous()
+    got = sparse.sparse_attention(q, k, v, blocks.to(DEV))
+    # the same blocks from a copy without what lies between
+    first = n - 5000 - (n - 5000) % 128
+    near = lambda x: torch.cat([x[:, :128], x[:, first:]], 1).cpu()  # noqa: E731
+    shift = first // 128 - 1
+    want, mag = ref_attention(q.cpu(), near(k), near(v), torch.where(blocks > 0, blocks - shift, blocks))
+    assert_attention(got, want, mag)
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads(cuda_lib):
+    import threading
+    from powershard_b200 import sparse
+    p = sparse.SparseProvider(3, key_block=64)
+    data = [[rows(40 + 3 * i + j, 1, 900 + 300 * i, 2, 128).to(DEV) for j in range(3)] for i in range(2)]
+    alone = [p(*d) for d in data]
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                out = p(*data[i])
+            torch.cuda.current_stream().synchronize()
+            got[i] = out
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert torch.equal(got[0], alone[0]) and torch.equal(got[1], alone[1])
