@@ -861,7 +861,7 @@ _CACHE_CALL = struct.Struct("@9P6q10q")
 
 def _cache_call(name, pages, scales, rows, table, first, count):
     (k, v), (ks, vs), (x, y) = pages, scales, rows
-    device, shape = k.device, k.shape
+    device, shape, xs = k.device, k.shape, x.shape
     _lib.require_cuda(k, name)
     code = _CODES.get(k.dtype)
     if code is None:
@@ -869,21 +869,26 @@ def _cache_call(name, pages, scales, rows, table, first, count):
     if (len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.device != device
             or not k.is_contiguous() or not v.is_contiguous()):
         raise ValueError(f"{name}: K and V pages must be alike, contiguous [pages, page_rows, H, D] on one device")
-    for s in (ks, vs):
-        if s.shape != shape[:3] or s.dtype != torch.float32 or s.device != device or not s.is_contiguous():
-            raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(shape[:3])} on {device}")
-    strides = *_row_strides(x, name), *_row_strides(y, name)
-    if y.shape != x.shape or x.shape[2:] != shape[2:] or y.dtype != x.dtype or x.device != device or y.device != device:
+    held = shape[:3]
+    if (ks.shape != held or vs.shape != held or ks.dtype != torch.float32 or vs.dtype != torch.float32
+            or ks.device != device or vs.device != device or not ks.is_contiguous() or not vs.is_contiguous()):
+        raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(held)} on {device}")
+    dtype = _lib.dtype_code(x.dtype)
+    if (len(xs) != 4 or y.shape != xs or xs[2:] != shape[2:] or y.dtype != x.dtype or x.device != device
+            or y.device != device):
         raise ValueError(f"{name}: K and V rows must be alike, [B, n, {shape[2]}, {shape[3]}] on {device}")
-    batch, n = x.shape[0], x.shape[1]
-    if (table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != batch or table.stride(1) != 1
+    sx, sy, st = x.stride(), y.stride(), table.stride()
+    if sx[3] != 1 or sy[3] != 1:
+        raise ValueError(f"{name}: rows need a unit inner stride")
+    batch = xs[0]
+    if (table.dtype != torch.int32 or len(st) != 2 or table.shape[0] != batch or st[1] != 1
             or table.device != device):
         raise ValueError(f"{name}: the page table must be int32 [{batch}, pages] with unit inner stride on {device}")
     call = _CACHE_CALL.pack(
         k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), x.data_ptr(), y.data_ptr(), table.data_ptr(),
-        _lengths_arg(first, batch, device, f"{name} first") or 0,
-        _lengths_arg(count, batch, device, f"{name} count") or 0, *strides, _lib.dtype_code(x.dtype), code, batch, n,
-        shape[2], shape[3], shape[0], shape[1], table.stride(0), table.shape[1])
+        _lengths_arg(first, batch, device, "cache first") or 0, _lengths_arg(count, batch, device, "cache count") or 0,
+        sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], dtype, code, batch, xs[1], shape[2], shape[3], shape[0], shape[1],
+        st[0], table.shape[1])
     rc = getattr(_lib.load(), name)(call, _lib.stream_handle(device))
     if rc:
         _lib.check(rc, name)
