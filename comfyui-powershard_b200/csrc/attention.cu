@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 128; ++j)
           if (j >= valid) s[j] = -INFINITY;
       }
-      softmax_row<kFp16, false>(s, i == 0, scale_log2, s_addr, o_addr, bar(kBarPH + t * (kPParts - 1)), bar(kBarP + t),
+      softmax_row<kFp16, false, false>(s, i == 0, scale_log2, s_addr, o_addr, bar(kBarPH + t * (kPParts - 1)), bar(kBarP + t),
                                 m, l);
     }
     if (ok) ok = warp_wait(bar(kBarO), 0, abort_flag, status, kErrO);

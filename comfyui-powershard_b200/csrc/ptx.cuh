@@ -467,6 +467,26 @@ __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
       : "f"(a0), "f"(a1));
 }
 
+// (2^x0, 2^x1) on the FMA pipe, relative error 7.5e-5: with k = round(x) and f =
+// x - k, 2^k times the cubic closest to 2^f on [-1/2, 1/2] in relative error
+// (by the exchange algorithm).  Adding 1.5 * 2^23 + 127 leaves k + 127 in the low
+// bits, which a shift makes 2^k.  Below -126 the result is 2^-126; NaN stays NaN.
+__device__ __forceinline__ void ex2_pair(float& y0, float& y1, float x0, float x1) {
+  asm("{\n\t.reg .b32 a, b;\n\t.reg .b64 x, t, k, f, p, m, c;\n\t"
+      "max.NaN.f32 a, %2, 0fC2FC0000;\n\tmax.NaN.f32 b, %3, 0fC2FC0000;\n\tmov.b64 x, {a, b};\n\t"
+      "mov.b64 m, {%4, %4};\n\tadd.rn.f32x2 t, x, m;\n\t"
+      "mov.b64 c, {%5, %5};\n\tadd.rn.f32x2 k, t, c;\n\t"
+      "sub.rn.f32x2 f, x, k;\n\t"
+      "mov.b64 c, {%6, %6};\n\tmov.b64 m, {%7, %7};\n\tfma.rn.f32x2 p, f, c, m;\n\t"
+      "mov.b64 c, {%8, %8};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%9, %9};\n\tfma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 {a, b}, t;\n\tshl.b32 a, a, 23;\n\tshl.b32 b, b, 23;\n\tmov.b64 t, {a, b};\n\t"
+      "mul.rn.f32x2 p, p, t;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "=f"(y0), "=f"(y1)
+      : "f"(x0), "f"(x1), "f"(12583039.f), "f"(-12583039.f), "f"(0.0551716685295105f), "f"(0.2426111251115799f),
+        "f"(0.6932609677314758f), "f"(0.9999280571937561f));
+}
+
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 128; ++i)
             if ((i & 63) >= (i < 64 ? lo : hi)) s[i] = -INFINITY;
         }
-        softmax_row<kFp16, true>(s, !any, args.scale_log2, s_addr, o_addr, bar(kPH + t * (kPParts - 1)), bar(kP + t), m, l);
+        softmax_row<kFp16, true, false>(s, !any, args.scale_log2, s_addr, o_addr, bar(kPH + t * (kPParts - 1)), bar(kP + t), m, l);
         any = true;
       }
       n = end;
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 128; ++j)
               if ((j & 63) >= (j < 64 ? lo : hi)) s[j] = -INFINITY;
           }
-          softmax_row<kFp16, true>(s, i == 0, scale_log2, s_addr, o_addr, bar(kPH + t * (kPParts - 1)), bar(kP + t), m, l);
+          softmax_row<kFp16, true, true>(s, i == 0, scale_log2, s_addr, o_addr, bar(kPH + t * (kPParts - 1)), bar(kP + t), m, l);
         }
       }
       n += tiles;

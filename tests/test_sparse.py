@@ -9,7 +9,9 @@ block at a time.  Tolerances:
   (u = eps/2) gives u A, the output's u |out|; a score is a 32-bit sum of 128
   products, off by at most 128 * 2^-23 * sum |q k| * scale <= 2^-12 for rows of
   this size (sum |q k| * scale <= 16), which enters numerator and denominator:
-  2^-11 A.
+  2^-11 A; the quarter of the exponentials that is computed on the FMA pipe is
+  off by 2^-13.7 of its terms more, 2^-15.7 A on the average of a row and below
+  the room that the worst case of the scores leaves.
 """
 import math
 
@@ -374,9 +376,26 @@ def test_arguments_are_checked(cuda_lib):
 def test_nan_keys_are_not_hidden(cuda_lib):
     from powershard_b200 import sparse
     q, k, v = (rows(s, 1, 512, 1, 128) for s in (16, 17, 18))
-    k[0, 200, 0, 5] = float("nan")
-    out = sparse.SparseProvider(1)(*cuda(q, k, v))
-    assert torch.isnan(out).all()
+    for key in (0, 129, 200, 300, 3, 260, 388, 453):  # every position of a group of eight
+        bad = k.clone()
+        bad[0, key, 0, 5] = float("nan")
+        out = sparse.SparseProvider(1)(*cuda(q, bad, v))
+        assert torch.isnan(out).all(), key
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [3, 300])
+def test_scores_far_apart(cuda_lib, lq):
+    """Scores of hundreds, most of them far below the largest: exponentials from 1 down to nothing.  A score's
+    error grows with it, so the rows are chosen with products that 32 bits hold exactly."""
+    from powershard_b200 import sparse
+    g = torch.Generator().manual_seed(60)
+    q, k = (torch.randint(-2, 3, (1, n, 2, 128), generator=g).to(torch.bfloat16) for n in (lq, 700))
+    v = rows(61, 1, 700, 2, 128)
+    blocks = torch.tensor([0, 3, 5, 7, 10], dtype=torch.int32).expand(1, 2, -(-lq // 256), 5).contiguous()
+    for scale in (0.5, 8.0, 64.0):
+        got = sparse.sparse_attention(*cuda(q, k, v, blocks), key_block=64, softmax_scale=scale)
+        assert_attention(got, *ref_attention(q, k, v, blocks, key_block=64, scale=scale))
 
 
 # ------------------------------------------------------------------ the provider
