@@ -17,7 +17,7 @@ import torch
 
 from . import _lib, ops
 from .contract import AttentionOptions
-from .sparse import SparseProvider, _on
+from .sparse import SparseProvider, _no_grad, _on
 
 
 class KVCache:
@@ -78,16 +78,20 @@ class StreamingAttention:
 
         start: rows that the sequences hold already, an int for all of them or
         an int32 device tensor [B]; lengths: new rows in use, int32 [B] or None
-        for all; context: rows of the longest sequence with the new ones
-        (needed with a tensor); selection: ``allowed`` of a sparse provider."""
+        for all; context: rows of the longest sequence with the new ones, needed
+        with a tensor (rows behind it are held but not attended); selection:
+        ``allowed`` of a sparse provider."""
+        _no_grad(q, k, v)
         b, n = k.shape[:2]
         ragged = lengths is not None or not isinstance(start, int)
         if ragged and not isinstance(self.provider, SparseProvider):
             raise ValueError("sequences of different lengths need a SparseProvider")
-        if context is None:
-            if not isinstance(start, int):
-                raise ValueError("context: the rows of the longest sequence, with start on the device")
+        if isinstance(start, int):
+            if start < 0 or context not in (None, start + n):
+                raise ValueError(f"start {start} with {n} new rows makes a context of {start + n}, got {context}")
             context = start + n
+        elif context is None:
+            raise ValueError("context: the rows of the longest sequence, with start on the device")
         if isinstance(start, int):
             start = torch.full((b,), start, dtype=torch.int32, device=k.device)
         self.cache.write(k, v, table, start, lengths)

@@ -1230,6 +1230,9 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
   if (int rc = check_blocks(batch, hq, hk, dim, qb, kb)) return rc;
   if (batch == 0 || hq == 0 || lq == 0) return PS_B200_OK;
   if (lk == 0) return set_error(PS_B200_ERR_INVALID, "empty key set");
+  if (int64_t(batch) * hq * ((int64_t(lq) + qb - 1) / qb) > (1 << 30) ||
+      int64_t(batch) * hk * ((int64_t(lk) + kb - 1) / kb) > (1 << 30))
+    return set_error(PS_B200_ERR_UNSUPPORTED, "more than 2^30 blocks");
   const SparseScratch s = sparse_scratch(batch, hq, hk, lq, lk, keep, qb, kb, c->key_means != nullptr);
   if (keep < 1 || keep > s.k_blocks)
     return set_error(PS_B200_ERR_INVALID, "keep %d outside [1, %lld key blocks]", keep, (long long)s.k_blocks);
@@ -1299,6 +1302,7 @@ static int cache_common(bool write, const ps_b200_cache_call* c, void* stream) {
     return set_error(PS_B200_ERR_UNSUPPORTED, "the cache holds heads of 64, 128 or 256 (got %lld)",
                      (long long)c->head_dim);
   const int64_t most = (int64_t(1) << 31) - 64;
+  const int64_t extents[3] = {c->batch, c->n, c->heads};
   if (c->batch < 0 || c->batch > 65535 || c->heads < 0 || c->heads > 4096 || c->n < 0 || c->n > most ||
       c->num_pages < 0 || c->num_pages > most || c->page_rows < 1 || c->page_rows > most || c->table_len < 0 ||
       c->table_len > most || c->table_stride < 0)
@@ -1319,6 +1323,9 @@ static int cache_common(bool write, const ps_b200_cache_call* c, void* stream) {
       a.st[t][i] = c->strides[3 * t + i];
       if (a.st[t][i] < 0 || a.st[t][i] % 8 != 0)
         return set_error(PS_B200_ERR_INVALID, "row strides must be non-negative multiples of 8 elements");
+      if (!write && a.st[t][i] == 0 && extents[i] > 1)
+        return set_error(PS_B200_ERR_INVALID, "a read needs rows of their own: stride 0 of an axis of %lld",
+                         (long long)extents[i]);
     }
   }
   if (int rc = check_device()) return rc;

@@ -786,6 +786,8 @@ def sparse_attention(q, k, v, out, blocks, counts, query_block: int, key_block: 
         raise ValueError("sparse attention: incompatible q/k/v/out shapes")
     if any(t.dtype != q.dtype or t.device != device for t in (k, v, out)):
         raise ValueError("sparse attention: q/k/v/out need one dtype and device")
+    if query_block < 1:
+        raise ValueError(f"sparse attention: query blocks of {query_block} rows")
     nq = -(-lq // query_block)
     if (blocks.dtype != torch.int32 or blocks.dim() != 4 or tuple(blocks.shape[:3]) != (batch, hq, nq)
             or not blocks.is_contiguous() or blocks.device != device):

@@ -70,6 +70,7 @@ def block_means(x, block: int, lengths=None):
     """Mean over the rows in use of each block of ``block`` rows of x [B, L, H, 128]:
     fp32 [B, ceil(L/block), H, 128] (a block without any row in use: zeros)."""
     ops._check16(x, "block_means")
+    _no_grad(x)
     if x.dim() != 4 or block < 1:
         raise ValueError(f"block_means: expected [B, L, H, D] and a positive block, got {tuple(x.shape)}, {block}")
     x = _readable(x)
@@ -93,6 +94,7 @@ def select_blocks(query_means, key_means, keep: int, *, allowed=None, query_bloc
     nk = key_means.shape[1]
     for t in (query_means, key_means):
         _lib.require_cuda(t, "select_blocks")
+    _no_grad(query_means, key_means)
     if keep < 1:
         raise ValueError(f"select_blocks: keep must be at least 1, got {keep}")
     if allowed is not None:
@@ -165,7 +167,8 @@ class SparseProvider(B200Provider):
 
     def blocks_kept(self, key_blocks: int) -> int:
         """Key blocks each query block attends, of ``key_blocks``."""
-        n = math.ceil(self.keep * key_blocks) if isinstance(self.keep, float) else self.keep
+        # 0.07 * 100 is a little above 7
+        n = max(1, math.ceil(self.keep * key_blocks - 1e-9)) if isinstance(self.keep, float) else self.keep
         return min(n, key_blocks)
 
     def __call__(self, q, k, v, o: AttentionOptions | None = None, *, allowed=None, key_means=None,

@@ -55,6 +55,12 @@ def test_refusals_before_any_launch():
         KVCache(0, 16, 2)
     with pytest.raises(ValueError):
         StreamingAttention(cache, object())(rows(0, 1, 4, 2, 128), *[rows(1, 1, 4, 2, 128)] * 2, None, lens(0))
+    x = rows(0, 1, 4, 2, 128)
+    for start, context in ((5, 8), (5, 12), (-1, None)):  # 5 rows held and 4 new ones are 9
+        with pytest.raises(ValueError):
+            StreamingAttention(cache, object())(x, x, x, None, start, context=context)
+    with pytest.raises(UnsupportedAttention):  # forward only
+        StreamingAttention(cache, object())(x, x.clone().requires_grad_(), x, None, 0)
     from powershard_b200 import ops
     with pytest.raises(UnsupportedAttention):  # CPU tensors
         ops.cache_write((k, k), (cache.k_scale,) * 2, (rows(0, 1, 4, 2, 128),) * 2, lens(0)[None])
@@ -80,6 +86,7 @@ def test_entries_validate_on_the_host():
         assert call(write, strides=(0, 250, 128) * 2) == _lib.ERR_INVALID
         assert call(write, table=0) == _lib.ERR_INVALID and call(write, table=18) == _lib.ERR_INVALID
         assert call(write, n=0) == _lib.OK
+    assert call(False, strides=(0, 0, 128) * 2) == _lib.ERR_INVALID and call(False, strides=(0, 256, 0) * 2) == _lib.ERR_INVALID
     assert call(False, count=0) == _lib.ERR_INVALID and b"lengths" in lib.ps_b200_last_error()
     assert lib.ps_b200_kernel_launches() == 0
 

@@ -121,6 +121,7 @@ def test_refusals_before_any_launch():
     p = sparse.SparseProvider(0.25)
     assert [p.blocks_kept(n) for n in (1, 3, 4, 5, 256)] == [1, 1, 1, 2, 64]
     assert sparse.SparseProvider(7).blocks_kept(5) == 5
+    assert sparse.SparseProvider(0.07).blocks_kept(100) == 7 and sparse.SparseProvider(1e-12).blocks_kept(4) == 1
     for o in (AttentionOptions(causal=True), AttentionOptions(softmax_scale=-1.0), AttentionOptions()):
         with pytest.raises(UnsupportedAttention):
             p(x, x, x, o)  # the last one: CPU tensors
@@ -156,6 +157,7 @@ def test_entries_validate_on_the_host():
 
     assert whole(batch=1 << 31) == _lib.ERR_INVALID and whole(lk=0) == _lib.ERR_INVALID and whole(lq=0) == _lib.OK
     assert whole(keep=0) == _lib.ERR_INVALID and whole(keep=6) == _lib.ERR_INVALID and whole(heads=3) == _lib.ERR_INVALID
+    assert whole(batch=60000, heads=60000, kv=60000) == _lib.ERR_UNSUPPORTED  # more blocks than can be counted
     assert whole(scratch=0) == _lib.ERR_INVALID and whole(nbytes=100) == _lib.ERR_INVALID and whole(scratch=272) == _lib.ERR_INVALID
     assert whole(dim=64) == _lib.ERR_UNSUPPORTED and whole(kb=32) == _lib.ERR_UNSUPPORTED
     assert whole(dtype=_lib.FP32) == _lib.ERR_UNSUPPORTED
@@ -267,10 +269,33 @@ def test_select_in_64_bits(cuda_lib, nk):
             got = sparse.select_blocks(*cuda(qm, km), keep)[0].cpu()
             assert torch.equal(got, ref_select(qm, km, keep)[0])
         assert order[1].eq(nk).all()
-    for size in (1e25, 1e-25, 1e-38):
+    for size in (1e25, 2e18, 6e17, 1e-25, 1e-38):
         qm, km = torch.randn(1, 2, 1, 128, generator=g) * size, torch.randn(1, nk, 1, 128, generator=g) * size
         got = sparse.select_blocks(*cuda(qm, km), nk // 3)[0].cpu()
         assert torch.equal(got, ref_select(qm, km, nk // 3)[0])
+
+
+@pytest.mark.gpu
+def test_forward_only(cuda_lib):
+    """What autograd would have to differentiate is refused, and runs where it records nothing."""
+    from powershard_b200 import sparse
+    from powershard_b200.contract import UnsupportedAttention
+    x = rows(31, 1, 300, 2, 128).to(DEV)
+    leaf = x.clone().requires_grad_()
+    m = sparse.block_means(x, 256)
+    mk = sparse.block_means(x, 128)
+    lists = sparse.select_blocks(m, mk, 2)
+    for call in (lambda t: sparse.block_means(t, 64), lambda t: sparse.sparse_attention(x, t, x, *lists),
+                 lambda t: sparse.SparseProvider(2)(t, x, x)):
+        with pytest.raises(UnsupportedAttention):
+            call(leaf)
+        with torch.no_grad():
+            assert torch.equal(call(leaf), call(x))
+    with pytest.raises(UnsupportedAttention):
+        sparse.select_blocks(m.clone().requires_grad_(), mk, 2)
+    for size in (0, -256):
+        with pytest.raises(ValueError):
+            sparse.sparse_attention(x, x, x, *lists, query_block=size)
 
 
 # ------------------------------------------------------------------ attention over lists
