@@ -1107,9 +1107,11 @@ int ps_b200_block_select(const float* q_means, const float* k_means, int batch, 
                          const int64_t allowed_strides[4], const int* q_len, int query_block, const int* k_len,
                          int key_block, int* blocks, int* counts, void* workspace, size_t workspace_bytes,
                          void* stream) {
+  SelectArgs from{};
+  from.after_means = true;  // as a rule
   return block_select(q_means, k_means, batch, heads_q, heads_kv, head_dim, q_blocks, k_blocks, keep, allowed,
                       allowed_strides, q_len, query_block, k_len, key_block, blocks, counts, workspace, workspace_bytes,
-                      stream);
+                      stream, from);
 }
 
 size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv, int q_blocks, int k_blocks) {

@@ -219,7 +219,8 @@ struct SelectArgs {
   int64_t q_st[3];         // batch, row, head strides in elements
   int len_q;
   int fp16;
-  bool after_means;        // launched right after the kernel that writes the means
+  bool after_means;        // launched right after the kernel that writes the means: starts while that one ends (after
+                           // the attention of an earlier call that costs 1.4 us of 27 instead)
   int* zeros;              // n_zeros words that the kernels behind the selection want zeroed
   int n_zeros;
 };

@@ -603,7 +603,7 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
     const int n = units - a.first_unit < step ? units - a.first_unit : step;
     const dim3 grid(static_cast<unsigned>((a.k_blocks + kScoreKeys - 1) / kScoreKeys), static_cast<unsigned>(row_chunks),
                     static_cast<unsigned>(n));
-    cudaError_t err = launch_after(score_kernel, grid, dim3(kThreads), 0, stream, a.after_means && a.first_unit == 0, a);
+    cudaError_t err = launch_after(score_kernel, grid, dim3(kThreads), 0, stream, a.after_means, a);
     if (err != cudaSuccess) return set_cuda_error("block_select scores launch", err);
     count_launch();
     err = launch_after(pick, dim3(static_cast<unsigned>(n * rows)), dim3(form == 0 ? 64 : 256), smem, stream, true, a);

@@ -667,7 +667,7 @@ def _lengths_arg(lengths, batch: int, device, what: str):
     """Device address of an int32 [batch] table of rows in use (None: all)."""
     if lengths is None:
         return None
-    if (lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch or lengths.device != device
+    if (lengths.dtype is not torch.int32 or lengths.shape != (batch,) or lengths.device != device
             or not lengths.is_contiguous()):
         raise ValueError(f"{what}: expected contiguous int32 [{batch}] on {device}, "
                          f"got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
@@ -678,7 +678,7 @@ def _row_strides(t: torch.Tensor, what: str):
     """(batch, row, head) strides of a [B, L, H, D] tensor the kernels can read."""
     _check16(t, what)
     st = t.stride()
-    if t.dim() != 4 or st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
+    if len(st) != 4 or st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
         raise ValueError(f"{what}: expected [B, L, H, D] with unit head-dim stride, other strides multiples of 8 "
                          f"elements and a 16-byte aligned base, got {tuple(t.shape)} / {st}")
     return st[:3]
@@ -693,16 +693,17 @@ def block_means(tensors, blocks, lengths, means):
     lib = _lib.load()
     x = tensors[0]
     device, batch, dtype = x.device, x.shape[0], x.dtype
+    at = x.get_device()
     addresses, strides, lens, rows, heads, out = [], [], [], [], [], []
     for t, block, n, m in zip(tensors, blocks, lengths, means):
         strides += _row_strides(t, "block_means")
         if block < 1:
             raise ValueError(f"block_means: blocks of {block} rows")
         b, length, h, d = t.shape
-        if t.dtype != dtype or b != batch or t.device != device:
+        if t.dtype is not dtype or b != batch or t.get_device() != at:
             raise ValueError("block_means: the tensors need one dtype, batch and device")
-        if (m.shape != (batch, -(-length // block), h, d) or m.dtype != torch.float32 or not m.is_contiguous()
-                or m.device != device):
+        if (m.shape != (batch, -(-length // block), h, d) or m.dtype is not torch.float32 or not m.is_contiguous()
+                or m.get_device() != at):
             raise ValueError(f"block_means: means must be contiguous fp32 {(batch, -(-length // block), h, d)} on {device}")
         addresses.append(t.data_ptr())
         rows.append(length)
@@ -710,11 +711,16 @@ def block_means(tensors, blocks, lengths, means):
         out.append(m.data_ptr())
         lens.append(_lengths_arg(n, batch, device, "block_means lengths") or 0)
     n = len(tensors)
+    pointers, ints, longs = _TABLES[n]
     rc = lib.ps_b200_block_means(
-        n, struct.pack(f"{n}P", *addresses), struct.pack(f"{3 * n}q", *strides), _lib.dtype_code(dtype), batch,
-        struct.pack(f"{n}i", *rows), struct.pack(f"{n}i", *heads), d, struct.pack(f"{n}i", *blocks),
-        struct.pack(f"{n}P", *lens), struct.pack(f"{n}P", *out), _lib.stream_handle(device))
-    _lib.check(rc, "ps_b200_block_means")
+        n, pointers(*addresses), longs(*strides), _lib.dtype_code(dtype), batch, ints(*rows), ints(*heads), d,
+        ints(*blocks), pointers(*lens), pointers(*out), _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, "ps_b200_block_means")
+
+
+# Tables of one or two addresses, ints, and triples of strides.
+_TABLES = {n: tuple(struct.Struct(f"{m}{c}").pack for m, c in ((n, "P"), (n, "i"), (3 * n, "q"))) for n in (1, 2)}
 
 
 @functools.lru_cache(maxsize=256)
@@ -730,17 +736,17 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
     [B, Hq, nq, nk] under any strides (a broadcast view) or None; blocks int32
     [B, Hq, nq, keep] and counts int32 [B, Hq, nq] are written."""
     lib = _lib.load()
-    device = q_means.device
+    device, at = q_means.device, q_means.get_device()
     for t, name in ((q_means, "q_means"), (k_means, "k_means")):
-        _lib.require_cuda(t, f"block_select {name}")
-        if t.dim() != 4 or t.dtype != torch.float32 or not t.is_contiguous() or t.device != device:
+        _lib.require_cuda(t, "block_select")
+        if t.dim() != 4 or t.dtype is not torch.float32 or not t.is_contiguous() or t.get_device() != at:
             raise ValueError(f"block_select {name}: expected contiguous fp32 [B, blocks, H, D] on {device}")
     batch, nq, hq, dim = q_means.shape
     nk, hk = k_means.shape[1:3]
     if k_means.shape[0] != batch or k_means.shape[3] != dim:
         raise ValueError("block_select: q_means and k_means differ in batch or head_dim")
     for t, shape, name in ((blocks, (batch, hq, nq, keep), "blocks"), (counts, (batch, hq, nq), "counts")):
-        if t.shape != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
+        if t.shape != shape or t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != at:
             raise ValueError(f"block_select {name}: expected contiguous int32 {shape} on {device}")
     mask, strides = None, None
     if allowed is not None:
@@ -754,7 +760,8 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
         _lengths_arg(query_lengths, batch, device, "block_select query_lengths"), query_block,
         _lengths_arg(key_lengths, batch, device, "block_select key_lengths"), key_block, blocks.data_ptr(),
         counts.data_ptr(), workspace.data_ptr(), n, _lib.stream_handle(device))
-    _lib.check(rc, "ps_b200_block_select")
+    if rc:
+        _lib.check(rc, "ps_b200_block_select")
 
 
 def sparse_attention_workspace(batch: int, heads: int, len_q: int, list_len: int, key_block: int, device):
@@ -831,8 +838,8 @@ def sparse_forward(q, k, v, out, keep: int, query_block: int, key_block: int, sc
     b, lq, hq, d = q.shape
     _, lk, hk, _ = k_shape = k.shape
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
-    if (v.shape != k_shape or out.shape != q.shape or k.dtype != dtype or v.dtype != dtype or out.dtype != dtype
-            or sq[3] != 1 or sk[3] != 1 or sv[3] != 1 or so[3] != 1):
+    if (v.shape != k_shape or out.shape != q.shape or k.dtype is not dtype or v.dtype is not dtype
+            or out.dtype is not dtype or sq[3] != 1 or sk[3] != 1 or sv[3] != 1 or so[3] != 1):
         raise ValueError("sparse attention: q/out [B, Lq, Hq, 128] and k/v [B, Lk, Hk, 128] need one dtype and a unit "
                          f"inner stride, got {tuple(q.shape)}, {tuple(k_shape)}, {tuple(v.shape)}, {tuple(out.shape)}")
     mask, sm = 0, _NO_STRIDES
@@ -865,32 +872,32 @@ def _cache_call(name, pages, scales, rows, table, first, count):
     (k, v), (ks, vs), (x, y) = pages, scales, rows
     device, shape, xs = k.device, k.shape, x.shape
     _lib.require_cuda(k, name)
-    code = _CODES.get(k.dtype)
+    at, stored, row_dtype = k.get_device(), k.dtype, x.dtype
+    code = _CODES.get(stored)
     if code is None:
-        raise _lib.UnsupportedAttention(f"{name}: pages hold float8_e4m3fn or int8 codes, got {k.dtype}")
-    if (len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.device != device
+        raise _lib.UnsupportedAttention(f"{name}: pages hold float8_e4m3fn or int8 codes, got {stored}")
+    if (len(shape) != 4 or v.shape != shape or v.dtype is not stored or v.get_device() != at
             or not k.is_contiguous() or not v.is_contiguous()):
         raise ValueError(f"{name}: K and V pages must be alike, contiguous [pages, page_rows, H, D] on one device")
     held = shape[:3]
-    if (ks.shape != held or vs.shape != held or ks.dtype != torch.float32 or vs.dtype != torch.float32
-            or ks.device != device or vs.device != device or not ks.is_contiguous() or not vs.is_contiguous()):
+    if (ks.shape != held or vs.shape != held or ks.dtype is not torch.float32 or vs.dtype is not torch.float32
+            or ks.get_device() != at or vs.get_device() != at or not ks.is_contiguous() or not vs.is_contiguous()):
         raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(held)} on {device}")
-    dtype = _lib.dtype_code(x.dtype)
-    if (len(xs) != 4 or y.shape != xs or xs[2:] != shape[2:] or y.dtype != x.dtype or x.device != device
-            or y.device != device):
+    dtype = _lib.dtype_code(row_dtype)
+    if (len(xs) != 4 or y.shape != xs or xs[2] != shape[2] or xs[3] != shape[3] or y.dtype is not row_dtype or x.get_device() != at
+            or y.get_device() != at):
         raise ValueError(f"{name}: K and V rows must be alike, [B, n, {shape[2]}, {shape[3]}] on {device}")
     sx, sy, st = x.stride(), y.stride(), table.stride()
     if sx[3] != 1 or sy[3] != 1:
         raise ValueError(f"{name}: rows need a unit inner stride")
-    batch = xs[0]
-    if (table.dtype != torch.int32 or len(st) != 2 or table.shape[0] != batch or st[1] != 1
-            or table.device != device):
+    batch, n, heads, dim = xs
+    ts = table.shape
+    if table.dtype is not torch.int32 or len(st) != 2 or ts[0] != batch or st[1] != 1 or table.get_device() != at:
         raise ValueError(f"{name}: the page table must be int32 [{batch}, pages] with unit inner stride on {device}")
     call = _CACHE_CALL.pack(
         k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), x.data_ptr(), y.data_ptr(), table.data_ptr(),
         _lengths_arg(first, batch, device, "cache first") or 0, _lengths_arg(count, batch, device, "cache count") or 0,
-        sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], dtype, code, batch, xs[1], shape[2], shape[3], shape[0], shape[1],
-        st[0], table.shape[1])
+        sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], dtype, code, batch, n, heads, dim, shape[0], shape[1], st[0], ts[1])
     rc = getattr(_lib.load(), name)(call, _lib.stream_handle(device))
     if rc:
         _lib.check(rc, name)

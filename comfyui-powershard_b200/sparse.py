@@ -62,8 +62,9 @@ def _broadcast(allowed, shape):
 
 def _no_grad(*tensors):
     """The kernels run forward only: a call that autograd would record is refused."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise UnsupportedAttention("b200_sparse: forward only, an input requires grad")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise UnsupportedAttention("b200_sparse: forward only, an input requires grad")
 
 
 def block_means(x, block: int, lengths=None):
@@ -71,11 +72,12 @@ def block_means(x, block: int, lengths=None):
     fp32 [B, ceil(L/block), H, 128] (a block without any row in use: zeros)."""
     ops._check16(x, "block_means")
     _no_grad(x)
-    if x.dim() != 4 or block < 1:
-        raise ValueError(f"block_means: expected [B, L, H, D] and a positive block, got {tuple(x.shape)}, {block}")
+    shape = x.shape
+    if len(shape) != 4 or block < 1:
+        raise ValueError(f"block_means: expected [B, L, H, D] and a positive block, got {tuple(shape)}, {block}")
     x = _readable(x)
-    b, n, h, d = x.shape
-    out = torch.empty((b, -(-n // block), h, d), dtype=torch.float32, device=x.device)
+    b, n, h, d = shape
+    out = x.new_empty((b, -(-n // block), h, d), dtype=torch.float32)
     with _on(x.device):
         ops.block_means([x], [block], [lengths], [out])
     return out
@@ -101,8 +103,8 @@ def select_blocks(query_means, key_means, keep: int, *, allowed=None, query_bloc
         allowed = _broadcast(allowed, (b, h, nq, nk))
     keep = min(int(keep), nk)
     device = query_means.device
-    blocks = torch.empty((b, h, nq, keep), dtype=torch.int32, device=device)
-    counts = torch.empty((b, h, nq), dtype=torch.int32, device=device)
+    blocks = query_means.new_empty((b, h, nq, keep), dtype=torch.int32)
+    counts = query_means.new_empty((b, h, nq), dtype=torch.int32)
     with _on(device):
         ops.block_select(query_means, key_means, keep, blocks, counts, query_block, key_block, allowed, query_lengths,
                          key_lengths)
@@ -160,7 +162,14 @@ class SparseProvider(B200Provider):
         self.identity["provider"] = NAME
 
     def check(self, q, k, v, o: AttentionOptions):
-        super().check(q, k, v, o)
+        # What needs no word is seen at a glance (the checks one by one take 3 us
+        # of a 25 us call); anything else gets them, and their errors.
+        dtype, at, qs, ks = q.dtype, q.get_device(), q.shape, k.shape
+        if not (o is _DEFAULT and (dtype is torch.bfloat16 or dtype is torch.float16) and len(qs) == len(ks) == 4
+                and qs[3] == ks[3] == 128 and v.shape == ks and qs[0] == ks[0] > 0 and ks[1] and qs[2] and ks[2]
+                and qs[2] % ks[2] == 0 and k.dtype is dtype and v.dtype is dtype
+                and at == k.get_device() == v.get_device() >= 0):
+            super().check(q, k, v, o)
         if o.softmax_scale is not None and not o.softmax_scale > 0:
             raise UnsupportedAttention("b200_sparse: the selection ranks by a positive softmax_scale")
         _no_grad(q, k, v)
