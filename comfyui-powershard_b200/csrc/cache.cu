@@ -19,6 +19,7 @@
 // stores 174-179 us.
 #include "ps_b200.h"
 #include "internal.h"
+#include "ptx.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -68,20 +69,27 @@ __device__ __forceinline__ uint4 narrow8(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// inv is 0 (of inf) or NaN in a row that has inf or NaN.
 template <bool kInt8>
 __device__ __forceinline__ uint2 encode8(const float (&f)[8], float inv) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    float y[4];
     if constexpr (kInt8) {
-      uint32_t b[4];
+      // Adding 1.5 * 2^23 rounds to a whole number and leaves it in the low bits.
+      // (In pairs the two instructions become one fused one, which rounds once.)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = static_cast<uint32_t>(__float2int_rn(f[4 * i + j] * inv)) & 0xffu;
-      w[i] = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
+      for (int j = 0; j < 4; ++j) y[j] = __fadd_rn(__fmul_rn(f[4 * i + j], inv), 12582912.f);
+      const uint32_t lo = __byte_perm(__float_as_uint(y[0]), __float_as_uint(y[1]), 0x0040);
+      const uint32_t hi = __byte_perm(__float_as_uint(y[2]), __float_as_uint(y[3]), 0x0040);
+      w[i] = inv > 0.f ? __byte_perm(lo, hi, 0x5410) : 0u;
     } else {
+      mul2(y[0], y[1], f[4 * i], f[4 * i + 1], inv);
+      mul2(y[2], y[3], f[4 * i + 2], f[4 * i + 3], inv);
       uint16_t lo, hi;
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(f[4 * i + 1] * inv), "f"(f[4 * i] * inv));
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(f[4 * i + 3] * inv), "f"(f[4 * i + 2] * inv));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
       w[i] = lo | (static_cast<uint32_t>(hi) << 16);
     }
   }
@@ -102,8 +110,7 @@ __device__ __forceinline__ void decode8(const uint2& v, float scale, float (&f)[
         uint32_t h;
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(w[i] >> (16 * j))));
         const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        f[4 * i + 2 * j] = t.x * scale;
-        f[4 * i + 2 * j + 1] = t.y * scale;
+        mul2(f[4 * i + 2 * j], f[4 * i + 2 * j + 1], t.x, t.y, scale);
       }
     }
   }
@@ -119,52 +126,71 @@ __device__ __forceinline__ int64_t pool_row(const CacheArgs& a, int batch, int64
   return static_cast<int64_t>(page) * a.page_rows + (pos - at * a.page_rows);
 }
 
+// The largest magnitude of two rows in one reduction: the bits of |x| order
+// like the numbers (NaN above inf), so the rows' maxima are the 16-bit halves
+// of a word.  Half of a row's lanes then work on each row's scale.
+//
 // grid: (groups of `tokens` rows, batch, K or V)
 template <bool kFp16, bool kInt8, int kLanes>
 __global__ void __launch_bounds__(kThreads, 8) cache_write_kernel(const CacheArgs a, int tokens, unsigned magic) {
-  constexpr int kDim = kLanes * 8, kRows = kThreads / kLanes, kUnroll = 2;
-  __shared__ int64_t slot[kMaxTokens];
+  constexpr int kDim = kLanes * 8, kRows = kThreads / kLanes;
+  __shared__ int64_t slot[kMaxTokens];  // of head 0, or -1
   const int batch = blockIdx.y, t = blockIdx.z;
   const int i0 = blockIdx.x * tokens;
   if (threadIdx.x < tokens) {
     const int i = i0 + threadIdx.x;
     const int used = a.count ? min(a.count[batch], a.n) : a.n;
-    slot[threadIdx.x] = i < used ? pool_row(a, batch, int64_t(i) + (a.first ? a.first[batch] : 0)) : -1;
+    const int64_t row = i < used ? pool_row(a, batch, int64_t(i) + (a.first ? a.first[batch] : 0)) : -1;
+    slot[threadIdx.x] = row < 0 ? -1 : row * a.heads;
   }
   __syncthreads();
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
   const int rows = tokens * a.heads;
   const uint16_t* x = static_cast<const uint16_t*>(a.rows[t]) + batch * a.st[t][0] + i0 * a.st[t][1] + lane * 8;
   constexpr float kMost = kInt8 ? 127.f : 448.f;
-  for (int j0 = 0; j0 < rows; j0 += kRows * kUnroll) {
-    uint4 v[kUnroll];
-    int64_t at[kUnroll];
+  for (int j0 = 0; j0 < rows; j0 += kRows * 2) {
+    uint4 v[2];
+    int64_t at[2];
+    uint32_t big[2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < 2; ++u) {
       const int j = j0 + u * kRows + grp;
       at[u] = -1;
       v[u] = make_uint4(0, 0, 0, 0);
       if (j < rows) {
         const int tok = a.heads == 1 ? j : __umulhi(j, magic), h = j - tok * a.heads;
         if (slot[tok] >= 0) {
-          at[u] = slot[tok] * a.heads + h;
+          at[u] = slot[tok] + h;
           v[u] = __ldcs(reinterpret_cast<const uint4*>(x + tok * a.st[t][1] + h * a.st[t][2]));
         }
       }
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < 2; ++u)
+      big[u] = __vmaxu2(__vmaxu2(v[u].x & 0x7fff7fffu, v[u].y & 0x7fff7fffu),
+                        __vmaxu2(v[u].z & 0x7fff7fffu, v[u].w & 0x7fff7fffu));
+    uint32_t both = __vmaxu2(__byte_perm(big[0], big[1], 0x5410), __byte_perm(big[0], big[1], 0x7632));
+#pragma unroll
+    for (int o = kLanes / 2; o; o >>= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, o));
+    const bool second = lane & (kLanes / 2);
+    float m;
+    if constexpr (kFp16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&both));
+      m = second ? f.y : f.x;
+    } else {
+      m = __uint_as_float(second ? both & 0xffff0000u : both << 16);
+    }
+    m = max_nan(m, kFloor);
+    const float inv = __fdiv_rn(kMost, m);
+    const int64_t mine = second ? at[1] : at[0];
+    if (lane % (kLanes / 2) == 0 && mine >= 0) a.scales[t][mine] = m * (1.f / kMost);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float by = __shfl_sync(0xffffffffu, inv, u * (kLanes / 2), kLanes);
+      if (at[u] < 0) continue;
       float f[8];
       widen8<kFp16>(v[u], f);
-      float m = kFloor;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max_nan(m, fabsf(f[e]));
-#pragma unroll
-      for (int o = kLanes / 2; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (at[u] < 0) continue;
-      const float inv = __fdiv_rn(kMost, m);
-      static_cast<uint2*>(a.pages[t])[at[u] * (kDim / 8) + lane] = encode8<kInt8>(f, inv);
-      if (lane == 0) a.scales[t][at[u]] = m * (1.f / kMost);
+      static_cast<uint2*>(a.pages[t])[at[u] * (kDim / 8) + lane] = encode8<kInt8>(f, by);
     }
   }
 }
@@ -179,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 8) cache_read_kernel(const CacheArgs
   if (threadIdx.x < tokens) {
     const int i = i0 + threadIdx.x;
     const int64_t pos = int64_t(i) + (a.first ? a.first[batch] : 0);
-    slot[threadIdx.x] = i < a.n && pos < a.count[batch] ? pool_row(a, batch, pos) : kSkip;
+    const int64_t row = i < a.n && pos < a.count[batch] ? pool_row(a, batch, pos) : kSkip;
+    slot[threadIdx.x] = row < 0 ? row : row * a.heads;
   }
   __syncthreads();
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
@@ -199,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 8) cache_read_kernel(const CacheArgs
         const int tok = a.heads == 1 ? j : __umulhi(j, magic), h = j - tok * a.heads;
         if (slot[tok] != kSkip) to[u] = y + tok * a.st[t][1] + h * a.st[t][2];
         if (slot[tok] >= 0) {
-          const int64_t at = slot[tok] * a.heads + h;
+          const int64_t at = slot[tok] + h;
           v[u] = __ldcs(static_cast<const uint2*>(a.pages[t]) + at * (kDim / 8) + lane);
           scale[u] = a.scales[t][at];
         }

@@ -467,6 +467,14 @@ __device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1) {
       : "f"(a0), "f"(a1));
 }
 
+// (a0, a1) * b.
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b) {
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b));
+}
+
 // (2^x0, 2^x1) on the FMA pipe, relative error 7.5e-5: with k = round(x) and f =
 // x - k, 2^k times the cubic closest to 2^f on [-1/2, 1/2] in relative error
 // (by the exchange algorithm).  Adding 1.5 * 2^23 + 127 leaves k + 127 in the low
