@@ -13,6 +13,10 @@ hand-written CUDA kernels (libps_b200.so, C ABI in include/ps_b200.h):
 * ``image.SequenceAttention`` - the Flux block attention override
   (powershard/image_parallel.py:67-110) on the Ulysses exchange and the
   joint [text; image] kernel;
+* ``SparseProvider`` - block-sparse attention behind the same provider API
+  (``sparse``: its steps one by one);
+* ``KVCache``, ``StreamingAttention`` - keys and values of earlier tokens in 8
+  bits and pages, and attention over them;
 * ``probe`` - the provider certification probe (powershard/attention_probe.py).
 
 The package directory doubles as a ComfyUI custom-node folder (it registers
@@ -27,6 +31,7 @@ NODE_DISPLAY_NAME_MAPPINGS: dict = {}
 __all__ = [
     "AttentionOptions", "UnsupportedAttention", "validate", "UlyssesGeometry", "shard_bounds",
     "ImageLayout", "split_sizes", "B200Provider", "UlyssesAttention", "SequenceAttention",
+    "SparseProvider", "KVCache", "StreamingAttention",
     "NODE_CLASS_MAPPINGS", "NODE_DISPLAY_NAME_MAPPINGS",
 ]
 
@@ -41,4 +46,10 @@ def __getattr__(name):  # lazy: importing the package never needs a GPU
     if name == "SequenceAttention":
         from .image import SequenceAttention
         return SequenceAttention
+    if name == "SparseProvider":
+        from .sparse import SparseProvider
+        return SparseProvider
+    if name in ("KVCache", "StreamingAttention"):
+        from . import cache
+        return getattr(cache, name)
     raise AttributeError(name)

@@ -127,6 +127,15 @@ def test_refusals_before_any_launch():
             p(x, x, x, o)  # the last one: CPU tensors
 
 
+def test_public_names():
+    import powershard_b200
+    from powershard_b200 import cache, sparse
+    assert powershard_b200.SparseProvider is sparse.SparseProvider
+    assert powershard_b200.KVCache is cache.KVCache and powershard_b200.StreamingAttention is cache.StreamingAttention
+    assert {"SparseProvider", "KVCache", "StreamingAttention"} <= set(powershard_b200.__all__)
+    assert callable(sparse.SparseProvider(2)) and sparse.SparseProvider(2).identity["provider"] == sparse.NAME
+
+
 def test_entries_validate_on_the_host():
     from powershard_b200 import _lib
     lib = _lib.load()
