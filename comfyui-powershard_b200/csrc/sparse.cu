@@ -560,6 +560,149 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
   if (threadIdx.x == 0) a.counts[list] = total;
 }
 
+// Few key blocks: scores and list in one kernel, all in 64 bits.
+//
+// A CTA makes one list.  Eight lanes take a key mean, 16 values each; then each
+// block's place is the number of better ones, counted by as many threads as
+// there are for it.  Against the two kernels above that saves a launch and the
+// wait between them, but every CTA reads and converts the key means again and
+// makes k_blocks^2 comparisons.  Measured (us, here and there): 12 lists of 32
+// blocks 2.8 and 8-10, 192 of 32 3.5 and 10, 720 of 79 10.1 and 17.5, 40 of 250
+// 8.4 and 11.3, 640 of 128 12.1 and 16.7; 160 of 256 13.6 and 11.9, 3000 of 64
+// 26.6 and 24.2, 1280 of 256 38 and 22.
+constexpr int kRankBlocks = 256;
+bool rank_pays(int64_t lists, int k_blocks) {
+  return k_blocks <= kRankBlocks && lists * k_blocks * (k_blocks + 256) <= (1 << 25);
+}
+
+__global__ void __launch_bounds__(kThreads, 4) rank_kernel(const SelectArgs a) {
+  __shared__ __align__(16) double qs[kHeadDim];
+  __shared__ double sums[kWarps][kHeadDim];
+  __shared__ unsigned long long keys[kRankBlocks];
+  __shared__ int better[kRankBlocks];
+  __shared__ int taken[kWarps];  // chosen of each 32 blocks
+  launch_dependents();
+  wait_for_previous();  // the means
+  const int rows = a.group * a.q_blocks;  // of one key head
+  const int unit = blockIdx.x / rows, row = blockIdx.x - unit * rows;
+  const int batch = unit / a.kv_heads, kv = unit - batch * a.kv_heads;
+  const int heads = a.kv_heads * a.group;
+  const int h = kv * a.group + row / a.q_blocks, qb = row % a.q_blocks;
+  const int64_t list = (static_cast<int64_t>(batch) * heads + h) * a.q_blocks + qb;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n_used = qb < blocks_in_use(a.q_len, batch, a.query_block, a.q_blocks)
+                         ? blocks_in_use(a.k_len, batch, a.key_block, a.k_blocks)
+                         : 0;
+  if (a.zeros && blockIdx.x == 0)
+    for (int i = tid; i < a.n_zeros; i += kThreads) a.zeros[i] = 0;
+
+  const int part = lane & 7;
+  const float4* km = reinterpret_cast<const float4*>(a.k_means) +
+                     (static_cast<int64_t>(batch) * a.k_blocks * a.kv_heads + kv) * (kHeadDim / 4) + part;
+  auto load = [&](int j, float4 (&v)[4]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      v[c] = j < n_used ? __ldg(km + static_cast<int64_t>(j) * a.kv_heads * (kHeadDim / 4) + 8 * c) : make_float4(0, 0, 0, 0);
+  };
+  float4 v[4];
+  load(warp * 4 + (lane >> 3), v);
+
+  if (a.q) {  // few query rows: their mean is taken here, a row to a warp
+    const int len = a.q_len ? min(max(a.q_len[batch], 0), a.len_q) : a.len_q;
+    const int n = min(max(len - qb * a.query_block, 0), a.query_block);
+    const uint16_t* x = static_cast<const uint16_t*>(a.q) + batch * a.q_st[0] +
+                        static_cast<int64_t>(qb) * a.query_block * a.q_st[1] + h * a.q_st[2] + 4 * lane;
+    double sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = warp; i < n; i += kWarps) {
+      const uint2 w2 = __ldg(reinterpret_cast<const uint2*>(x + i * a.q_st[1]));
+      const uint32_t w[2] = {w2.x, w2.y};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 f = a.fp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[e]))
+                                : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+        sum[2 * e] += static_cast<double>(f.x);
+        sum[2 * e + 1] += static_cast<double>(f.y);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[warp][4 * lane + e] = sum[e];
+    __syncthreads();
+    if (tid < kHeadDim) {
+      double total = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) total += sums[w][tid];
+      qs[tid] = n ? static_cast<double>(static_cast<float>(total / n)) : 0.0;
+    }
+  } else if (tid < kHeadDim) {
+    qs[tid] = static_cast<double>(
+        __ldg(a.q_means + ((static_cast<int64_t>(batch) * a.q_blocks + qb) * heads + h) * kHeadDim + tid));
+  }
+  better[tid] = 0;
+  __syncthreads();
+
+  double q[16];  // the lane's pieces part, part + 8, ... of 16 bytes
+#pragma unroll
+  for (int i = 0; i < 16; ++i) q[i] = qs[4 * (part + 8 * (i >> 2)) + (i & 3)];
+  const uint8_t* allowed = a.allowed ? a.allowed + batch * a.allowed_st[0] + h * a.allowed_st[1] + qb * a.allowed_st[2]
+                                     : nullptr;
+  for (int j0 = 0; j0 < a.k_blocks; j0 += 4 * kWarps) {
+    const int j = j0 + warp * 4 + (lane >> 3);
+    bool may = j < n_used;
+    if (may && allowed && part == 0) may = allowed[j * a.allowed_st[3]] != 0;
+    double d[2] = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      d[0] = fma(q[4 * c], double(v[c].x), d[0]);
+      d[1] = fma(q[4 * c + 1], double(v[c].y), d[1]);
+      d[0] = fma(q[4 * c + 2], double(v[c].z), d[0]);
+      d[1] = fma(q[4 * c + 3], double(v[c].w), d[1]);
+    }
+    load(j + 4 * kWarps, v);
+    d[0] += d[1];
+#pragma unroll
+    for (int o = 4; o; o >>= 1) d[0] += __shfl_xor_sync(0xffffffffu, d[0], o);
+    if (part == 0 && j < a.k_blocks) keys[j] = may ? order_key(d[0]) : 0ull;
+  }
+  __syncthreads();
+
+  // Thread tid counts a share of the blocks better than block tid % span.
+  const int span = (a.k_blocks + 31) & ~31, shares = kThreads / span;
+  const int share = tid / span, j = tid - share * span;
+  if (share < shares && j < a.k_blocks) {
+    // Of equals the lower index is better: before the warp's 32 blocks a key
+    // counts from `key` on, behind them above it.  (What 0 counts does not matter, it is never chosen.)
+    const unsigned long long key = keys[j], below = key - 1;
+    const int begin = a.k_blocks * share / shares, end = a.k_blocks * (share + 1) / shares;
+    const int own = j & ~31;
+    int n = 0, i = begin;
+#pragma unroll 8
+    for (; i < min(own, end); ++i) n += keys[i] > below;
+    for (; i < min(own + 32, end); ++i) n += keys[i] > (i < j ? below : key);
+#pragma unroll 8
+    for (; i < end; ++i) n += keys[i] > key;
+    if (shares == 1)
+      better[j] = n;
+    else if (n)
+      atomicAdd(&better[j], n);
+  }
+  __syncthreads();
+  const bool take = tid < a.k_blocks && keys[tid] != 0 && better[tid] < a.keep;
+  const unsigned m = __ballot_sync(0xffffffffu, take);
+  if (lane == 0) taken[warp] = __popc(m);
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? taken[w] : 0;
+    total += taken[w];
+  }
+  int* out = a.blocks + list * a.keep;
+  if (take) out[before + __popc(m & ((1u << lane) - 1))] = tid;
+  for (int i = total + tid; i < a.keep; i += kThreads) out[i] = -1;
+  if (tid == 0) a.counts[list] = total;
+}
+
 }  // namespace sparse
 
 int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream) {
@@ -598,6 +741,13 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
   const int64_t row_chunks = (rows + kScoreRows - 1) / kScoreRows;
   if (row_chunks > 65535) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^22 lists a key head");
   const int units = a.batch * a.kv_heads;
+  if (rank_pays(units * rows, a.k_blocks)) {
+    const cudaError_t err = launch_after(rank_kernel, dim3(static_cast<unsigned>(units * rows)), dim3(kThreads), 0,
+                                         stream, a.after_means, a);
+    if (err != cudaSuccess) return set_cuda_error("block_select launch", err);
+    count_launch();
+    return 0;
+  }
   const int step = select_units(a.batch, a.kv_heads, a.group, a.q_blocks, a.k_blocks);
   for (a.first_unit = 0; a.first_unit < units; a.first_unit += step) {
     const int n = units - a.first_unit < step ? units - a.first_unit : step;

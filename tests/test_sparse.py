@@ -215,7 +215,8 @@ def test_block_means(cuda_lib, n, heads, block, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,nq,nk,heads,kv,keep", [
     (1, 1, 1, 1, 1, 1), (2, 3, 7, 4, 2, 3), (1, 9, 300, 2, 2, 40), (1, 1, 513, 5, 1, 100), (2, 1, 64, 2, 2, 64),
-    (1, 2, 2600, 1, 1, 260), (1, 5, 4000, 1, 1, 17), (1, 17, 33, 3, 3, 32)])
+    (1, 2, 2600, 1, 1, 260), (1, 5, 4000, 1, 1, 17), (1, 17, 33, 3, 3, 32),
+    (1, 2, 256, 2, 1, 100), (2, 1, 255, 1, 1, 254), (1, 4, 97, 4, 2, 50), (1, 150, 200, 4, 2, 20)])
 def test_select_blocks(cuda_lib, b, nq, nk, heads, kv, keep):
     from powershard_b200 import sparse
     qm, km = rows(2, b, nq, heads, 128, dtype=torch.float32), rows(3, b, nk, kv, 128, dtype=torch.float32)
@@ -235,20 +236,22 @@ def test_select_blocks(cuda_lib, b, nq, nk, heads, kv, keep):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("nq", [1, 6])
-def test_select_ties_and_nan(cuda_lib, nq):
+@pytest.mark.parametrize("nk", [40, 400])  # the two forms of the selection
+def test_select_ties_and_nan(cuda_lib, nq, nk):
     """Equal scores go to the lower index (0 and -0 among them), NaN is chosen, infinities rank as they are."""
     from powershard_b200 import sparse
-    qm, km = torch.zeros(1, nq, 1, 128), torch.zeros(1, 40, 1, 128)
+    qm, km = torch.zeros(1, nq, 1, 128), torch.zeros(1, nk, 1, 128)
     qm[..., 0] = 1.0
-    km[0, :, 0, 0] = torch.tensor([0.0, -0.0] * 10 + [1.0] * 12 + [-1.0] * 8)
-    for keep in (1, 5, 12, 13, 20, 32, 35, 40):
+    km[0, :, 0, 0] = torch.tensor(([0.0, -0.0] * 10 + [1.0] * 12 + [-1.0] * 8) * (nk // 40))
+    for keep in (1, 5, 12, 13, 20, 32, 35, 40, nk // 2 + 1, nk):
         got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
         want = ref_select(qm, km, keep)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
     qm[..., 1] = 1.0
     km[0, 37, 0, 0], km[0, 38, 0, 0] = float("nan"), float("-inf")
     km[0, 36, 0, 0] = float("inf")
-    for keep in (1, 2, 3, 39, 40):
+    km[0, nk - 1, 0, 1] = float("nan")
+    for keep in (1, 2, 3, 39, 40, nk - 1, nk):
         got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
         want = ref_select(qm, km, keep)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
@@ -444,7 +447,8 @@ def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,lq,lk,heads,kv,qb,kb,keep,ragged", [
     (1, 1000, 1000, 2, 2, 256, 128, 3, False), (2, 777, 777, 4, 2, 256, 64, 5, True), (1, 1, 4096, 3, 1, 256, 128, 8, False),
-    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (2, 7, 9000, 6, 3, 256, 64, 50, True), (4, 16, 2000, 50, 10, 256, 128, 9, True), (5, 1, 1, 2, 2, 256, 64, 1, True)])
+    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (2, 7, 9000, 6, 3, 256, 64, 50, True), (4, 16, 2000, 50, 10, 256, 128, 9, True), (5, 1, 1, 2, 2, 256, 64, 1, True),
+    (2, 31, 20000, 2, 1, 256, 64, 40, True)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_provider(cuda_lib, b, lq, lk, heads, kv, qb, kb, keep, ragged, dtype):
     from powershard_b200 import sparse
