@@ -260,10 +260,11 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
 // each where that ends sooner.  The time of that wave, from measurements (B200,
 // us): a key tile 2.0, a unit or part 3 more; parts cost 6 for the kernel that
 // merges them and 0.064 each for their traffic (2 x 64 KB written and read).
+// Tiles are not divided: 12 units of 8 tiles take 15 us in four parts, 18 in five.
 // Measured at 44 units left over (192 on 148 SMs): 8 tiles 44.3 us split in
 // three, 41.1 whole; 16 tiles 64.9 and 70.4; 32 tiles 103 and 129.  80 units of
 // 64 tiles: 115 in three, 127 whole.  Few queries (a tile 1.0, a part 2.5, 1.5
-// for the merge) are bound by the keys they read once every SM has a part: 40
+// or 3.5 for the merge) are bound by the keys they read once every SM has a part: 40
 // units of 60 tiles 35.6 in three, 42.8 in seven.
 struct SparsePlan {
   int64_t units, rem;
@@ -285,8 +286,8 @@ SparsePlan sparse_plan(int64_t batch, int64_t heads, int64_t len_q, int64_t list
   most = most < kMaxSparseSplit ? most : kMaxSparseSplit;
   for (int64_t split = 1; p.rem > 0 && split <= most; ++split) {
     const int64_t rounds = (p.rem * split + sms - 1) / sms;
-    const double merge = split == 1 ? 0 : few ? 1.5 : 6 + 0.064 * double(p.rem * split);
-    const double time = double(rounds) * (double(tiles) / double(split) * tile + part) + merge;
+    const double merge = split == 1 ? 0 : len_q <= kTicketRows ? 1.5 : few ? 3.5 : 6 + 0.064 * double(p.rem * split);
+    const double time = double(rounds) * (double((tiles + split - 1) / split) * tile + part) + merge;
     if (split == 1 || time < best) {
       best = time;
       p.split = static_cast<int>(split);
@@ -338,7 +339,7 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   const SparsePlan plan = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count());
   s.workspace_bytes = plan.workspace_bytes();
   s.workspace = take(s.workspace_bytes);
-  s.n_tickets = plan.split > 1 && len_q <= kMergeRows ? plan.rem : 0;
+  s.n_tickets = plan.split > 1 && len_q <= kTicketRows ? plan.rem : 0;
   s.tickets = take(s.n_tickets * sizeof(int));
   s.total = at;
   return s;
@@ -1245,11 +1246,12 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
   float* k_means = reinterpret_cast<float*>(base + s.k_means);
   int* blocks = reinterpret_cast<int*>(base + s.blocks);
   int* counts = reinterpret_cast<int*>(base + s.counts);
-  // The means of a few query rows are taken by the selection itself (one launch
-  // less: 2.4 us on the GPU and 3 us on the host for one row; at 32 rows their
-  // reading, one row after the other, takes as long as the launch saved).
+  // With kept key means, those of a few query rows are taken by the selection
+  // itself, a launch less.  rank_kernel has eight warps for the rows: 2.3 us less up
+  // to 128, 1.4 at 256; score_kernel one: at 32 rows their reading takes as long
+  // as the launch saved.
   SelectArgs from{};
-  if (lq <= 32) {
+  if (c->key_means && (lq <= 32 || (lq <= 256 && select_is_small(batch * hq * s.q_blocks, int(s.k_blocks))))) {
     if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
     if (!c->q || !aligned16(c->q)) return set_error(PS_B200_ERR_INVALID, "queries null or not 16-byte aligned");
     from.q = c->q;

@@ -62,6 +62,12 @@ struct AttnArgs {
 constexpr int kMaxSplit = 8;
 constexpr int kMaxSparseSplit = 32;
 constexpr int kMergeRows = 16;  // query rows up to which sparse attention runs in its form for few queries
+// ... and up to which the parts of a split unit are merged in it, by the warp
+// that ends last.  That saves a launch, but the warp takes two rows after the
+// other: 12 lists of 8 tiles, 1 row 15.0 us and (merged by a kernel) as much, with
+// the host in the steady state 18.0 and 19.9; 4 rows 16.0 and 16.1; 8 rows 18.7 and
+// 16.7; 16 rows 24.4 and 16.9.
+constexpr int kTicketRows = 4;
 // Workspace bytes for up to 160 SMs: one partial (O, lse) per CTA of a wave.
 constexpr int64_t kAttnWorkspaceBytes = int64_t(160) * 2 * 128 * (128 + 1) * 4;
 
@@ -225,6 +231,7 @@ struct SelectArgs {
   int n_zeros;
 };
 int launch_block_select(SelectArgs a, cudaStream_t stream);
+bool select_is_small(int64_t lists, int k_blocks);  // one kernel makes the lists (rank_kernel)
 
 // 8-bit key/value cache (cache.cu).
 struct CacheArgs {

@@ -571,9 +571,6 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
 // 8.4 and 11.3, 640 of 128 12.1 and 16.7; 160 of 256 13.6 and 11.9, 3000 of 64
 // 26.6 and 24.2, 1280 of 256 38 and 22.
 constexpr int kRankBlocks = 256;
-bool rank_pays(int64_t lists, int k_blocks) {
-  return k_blocks <= kRankBlocks && lists * k_blocks * (k_blocks + 256) <= (1 << 25);
-}
 
 __global__ void __launch_bounds__(kThreads, 4) rank_kernel(const SelectArgs a) {
   __shared__ __align__(16) double qs[kHeadDim];
@@ -705,6 +702,10 @@ __global__ void __launch_bounds__(kThreads, 4) rank_kernel(const SelectArgs a) {
 
 }  // namespace sparse
 
+bool select_is_small(int64_t lists, int k_blocks) {
+  return k_blocks <= sparse::kRankBlocks && lists * k_blocks * (k_blocks + 256) <= (1 << 25);
+}
+
 int launch_block_means(const MeansArgs& a, bool fp16, cudaStream_t stream) {
   using namespace sparse;
   const int64_t ctas = a.t[0].ctas + a.t[1].ctas;
@@ -741,7 +742,7 @@ int launch_block_select(SelectArgs a, cudaStream_t stream) {
   const int64_t row_chunks = (rows + kScoreRows - 1) / kScoreRows;
   if (row_chunks > 65535) return set_error(PS_B200_ERR_UNSUPPORTED, "block_select: more than 2^22 lists a key head");
   const int units = a.batch * a.kv_heads;
-  if (rank_pays(units * rows, a.k_blocks)) {
+  if (select_is_small(units * rows, a.k_blocks)) {
     const cudaError_t err = launch_after(rank_kernel, dim3(static_cast<unsigned>(units * rows)), dim3(kThreads), 0,
                                          stream, a.after_means, a);
     if (err != cudaSuccess) return set_cuda_error("block_select launch", err);

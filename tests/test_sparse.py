@@ -447,7 +447,7 @@ def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,lq,lk,heads,kv,qb,kb,keep,ragged", [
     (1, 1000, 1000, 2, 2, 256, 128, 3, False), (2, 777, 777, 4, 2, 256, 64, 5, True), (1, 1, 4096, 3, 1, 256, 128, 8, False),
-    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (2, 7, 9000, 6, 3, 256, 64, 50, True), (4, 16, 2000, 50, 10, 256, 128, 9, True), (5, 1, 1, 2, 2, 256, 64, 1, True),
+    (3, 900, 1500, 2, 1, 512, 192, 2, True), (1, 2049, 300, 1, 1, 256, 64, 5, False), (2, 7, 9000, 6, 3, 256, 64, 50, True), (4, 16, 2000, 50, 10, 256, 128, 9, True), (5, 1, 1, 2, 2, 256, 64, 1, True), (1, 200, 3000, 2, 1, 256, 128, 6, False), (2, 8, 5000, 3, 3, 256, 64, 30, False), (1, 30, 20000, 2, 1, 256, 64, 40, False),
     (2, 31, 20000, 2, 1, 256, 64, 40, True)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_provider(cuda_lib, b, lq, lk, heads, kv, qb, kb, keep, ragged, dtype):
