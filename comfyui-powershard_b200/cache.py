@@ -33,6 +33,9 @@ class KVCache:
                  dtype: torch.dtype = torch.float8_e4m3fn, device=None):
         if min(pages, page_rows, heads) < 1:
             raise ValueError("KVCache: pages, page_rows and heads must be positive")
+        if dtype not in ops._CODES or head_dim not in (64, 128, 256):
+            raise _lib.UnsupportedAttention("KVCache: float8_e4m3fn or int8 codes and heads of 64, 128 or 256, "
+                                            f"got {dtype} and {head_dim}")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         shape = (pages, page_rows, heads, head_dim)
         self._set(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2)),

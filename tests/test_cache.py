@@ -53,6 +53,9 @@ def test_refusals_before_any_launch():
     cache = KVCache.over(k, k, torch.zeros(4, 16, 2), torch.zeros(4, 16, 2))
     with pytest.raises(ValueError):
         KVCache(0, 16, 2)
+    for dim, dtype in ((96, torch.int8), (128, torch.float16), (128, torch.float8_e5m2)):
+        with pytest.raises(UnsupportedAttention):
+            KVCache(4, 16, 2, dim, dtype)
     with pytest.raises(ValueError):
         StreamingAttention(cache, object())(rows(0, 1, 4, 2, 128), *[rows(1, 1, 4, 2, 128)] * 2, None, lens(0))
     x = rows(0, 1, 4, 2, 128)
