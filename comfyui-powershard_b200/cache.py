@@ -17,7 +17,7 @@ import torch
 
 from . import _lib, ops
 from .contract import AttentionOptions
-from .sparse import SparseProvider, _no_grad, _on
+from .sparse import SparseProvider, _no_grad
 
 
 class KVCache:
@@ -54,16 +54,12 @@ class KVCache:
     def write(self, k, v, table, start=None, lengths=None):
         """Rows i < lengths[b] (None: all) of k, v [B, n, heads, head_dim] to
         positions start[b] + i (None: i) of sequence b.  Rows without a page are dropped."""
-        _lib.require_cuda(self.k, "cache pages")
-        with _on(self.k.device):
-            ops.cache_write((self.k, self.v), (self.k_scale, self.v_scale), (k, v), table, start, lengths)
+        ops.cache_write((self.k, self.v), (self.k_scale, self.v_scale), (k, v), table, start, lengths)
 
     def read(self, table, lengths, k_out, v_out, first=None):
         """Positions first[b] + i (None: i) below lengths[b] into row i of k_out,
         v_out [B, n, heads, head_dim] (bf16 or fp16); the other rows stay as they are."""
-        _lib.require_cuda(self.k, "cache pages")
-        with _on(self.k.device):
-            ops.cache_read((self.k, self.v), (self.k_scale, self.v_scale), (k_out, v_out), table, lengths, first)
+        ops.cache_read((self.k, self.v), (self.k_scale, self.v_scale), (k_out, v_out), table, lengths, first)
 
 
 class StreamingAttention:

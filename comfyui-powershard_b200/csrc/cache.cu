@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 8) cache_write_kernel(const CacheArg
   }
   __syncthreads();
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int rows = tokens * a.heads;
+  const int rows = min(tokens, a.n - i0) * a.heads;
   const uint16_t* x = static_cast<const uint16_t*>(a.rows[t]) + batch * a.st[t][0] + i0 * a.st[t][1] + lane * 8;
   constexpr float kMost = kInt8 ? 127.f : 448.f;
   for (int j0 = 0; j0 < rows; j0 += kRows * 2) {
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 8) cache_read_kernel(const CacheArgs
   }
   __syncthreads();
   const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int rows = tokens * a.heads;
+  const int rows = min(tokens, a.n - i0) * a.heads;
   uint16_t* y = static_cast<uint16_t*>(a.rows[t]) + batch * a.st[t][0] + i0 * a.st[t][1] + lane * 8;
   for (int j0 = 0; j0 < rows; j0 += kRows * kUnroll) {
     uint2 v[kUnroll];
@@ -246,8 +246,16 @@ __global__ void __launch_bounds__(kThreads, 8) cache_read_kernel(const CacheArgs
 
 template <bool kWrite, bool kFp16, bool kInt8, int kLanes>
 int launch(const CacheArgs& a, cudaStream_t stream) {
-  // About 128 rows of one head a CTA: eight for each group of lanes.
-  int tokens = (128 + a.heads - 1) / a.heads;
+  // About 128 rows of one head a CTA; fewer, down to one pass, while all CTAs
+  // still (nearly) run at a time, 8 on each of 148 SMs.  (us, 128 rows and fewer:
+  // writing 8 rows of 12 heads 3.8 and 2.5, 3 x 311 of 10 5.8 and 4.1, 2 x 1000 of
+  // 4 heads of 256 7.4 and 4.5; reading 1000 of 40 7.6 and 6.8, but 4 x 2000 of 8
+  // heads of 64 in two rounds 5.8 and 6.4.)
+  constexpr int kOnce = 2 * kThreads / kLanes;  // rows of one pass
+  const int64_t all = int64_t(a.n) * a.batch * a.heads * 2;
+  int per = 128;
+  while (per > kOnce && all <= int64_t(per) * 5 * 148) per /= 2;
+  int tokens = (per + a.heads - 1) / a.heads;
   tokens = tokens > kMaxTokens ? kMaxTokens : tokens;
   const int64_t groups = (int64_t(a.n) + tokens - 1) / tokens;
   const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(a.batch), 2);

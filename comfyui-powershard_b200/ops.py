@@ -871,8 +871,9 @@ _CACHE_CALL = struct.Struct("@9P6q10q")
 def _cache_call(name, pages, scales, rows, table, first, count):
     (k, v), (ks, vs), (x, y) = pages, scales, rows
     device, shape, xs = k.device, k.shape, x.shape
-    _lib.require_cuda(k, name)
     at, stored, row_dtype = k.get_device(), k.dtype, x.dtype
+    if at < 0:
+        _lib.require_cuda(k, name)
     code = _CODES.get(stored)
     if code is None:
         raise _lib.UnsupportedAttention(f"{name}: pages hold float8_e4m3fn or int8 codes, got {stored}")
@@ -884,8 +885,8 @@ def _cache_call(name, pages, scales, rows, table, first, count):
             or ks.get_device() != at or vs.get_device() != at or not ks.is_contiguous() or not vs.is_contiguous()):
         raise ValueError(f"{name}: scales must be contiguous fp32 {tuple(held)} on {device}")
     dtype = _lib.dtype_code(row_dtype)
-    if (len(xs) != 4 or y.shape != xs or xs[2] != shape[2] or xs[3] != shape[3] or y.dtype is not row_dtype or x.get_device() != at
-            or y.get_device() != at):
+    if (len(xs) != 4 or y.shape != xs or xs[2] != shape[2] or xs[3] != shape[3] or y.dtype is not row_dtype
+            or x.get_device() != at or y.get_device() != at):
         raise ValueError(f"{name}: K and V rows must be alike, [B, n, {shape[2]}, {shape[3]}] on {device}")
     sx, sy, st = x.stride(), y.stride(), table.stride()
     if sx[3] != 1 or sy[3] != 1:
@@ -898,7 +899,12 @@ def _cache_call(name, pages, scales, rows, table, first, count):
         k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), x.data_ptr(), y.data_ptr(), table.data_ptr(),
         _lengths_arg(first, batch, device, "cache first") or 0, _lengths_arg(count, batch, device, "cache count") or 0,
         sx[0], sx[1], sx[2], sy[0], sy[1], sy[2], dtype, code, batch, n, heads, dim, shape[0], shape[1], st[0], ts[1])
-    rc = getattr(_lib.load(), name)(call, _lib.stream_handle(device))
+    entry, stream = getattr(_lib.load(), name), _lib.stream_handle(device)
+    if at == torch.cuda.current_device():
+        rc = entry(call, stream)
+    else:
+        with torch.cuda.device(at):
+            rc = entry(call, stream)
     if rc:
         _lib.check(rc, name)
 
