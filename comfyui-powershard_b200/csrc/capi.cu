@@ -336,8 +336,9 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   s.k_means = take(key_means ? 0 : size_t(batch * heads_kv * s.k_blocks) * 128 * sizeof(float));
   s.blocks = take(lists * keep * sizeof(int));
   s.counts = take(lists * sizeof(int));
-  s.scores_bytes =
-      size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, s.q_blocks, s.k_blocks)) * sizeof(float);
+  if (!select_is_small(batch * heads_q * s.q_blocks, int(s.k_blocks)))
+    s.scores_bytes =
+        size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, s.q_blocks, s.k_blocks)) * sizeof(float);
   s.scores = take(s.scores_bytes);
   const SparsePlan plan = sparse_plan(batch, heads_q, len_q, keep, key_block, sm_count());
   s.workspace_bytes = plan.workspace_bytes();
@@ -1079,7 +1080,7 @@ static int block_select(const float* q_means, const float* k_means, int batch, i
     return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
   if (allowed && !allowed_strides) return set_error(PS_B200_ERR_INVALID, "allowed needs strides");
   const size_t need = ps_b200_block_select_workspace_bytes(batch, heads_q, heads_kv, q_blocks, k_blocks);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < need)
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return set_error(PS_B200_ERR_INVALID, "this call needs a 16-byte aligned workspace of %zu bytes (got %zu)", need,
                      workspace ? workspace_bytes : size_t(0));
   if (int rc = check_device()) return rc;
@@ -1100,9 +1101,11 @@ static int block_select(const float* q_means, const float* k_means, int batch, i
   for (int i = 0; i < 4; ++i) a.allowed_st[i] = allowed ? allowed_strides[i] : 0;
   a.blocks = blocks;
   a.counts = counts;
-  a.scores = static_cast<float*>(workspace);
-  a.k_sq = reinterpret_cast<uint32_t*>(a.scores + int64_t(select_units(batch, a.kv_heads, a.group, q_blocks, k_blocks)) *
-                                                      a.group * q_blocks * k_blocks);
+  if (need > 0) {
+    a.scores = static_cast<float*>(workspace);
+    a.k_sq = reinterpret_cast<uint32_t*>(a.scores + int64_t(select_units(batch, a.kv_heads, a.group, q_blocks, k_blocks)) *
+                                                        a.group * q_blocks * k_blocks);
+  }
   return launch_block_select(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -1120,6 +1123,7 @@ int ps_b200_block_select(const float* q_means, const float* k_means, int batch, 
 
 size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv, int q_blocks, int k_blocks) {
   if (batch <= 0 || heads_q <= 0 || heads_kv <= 0 || q_blocks <= 0 || k_blocks <= 0) return 0;
+  if (select_is_small(int64_t(batch) * heads_q * q_blocks, k_blocks)) return 0;
   return size_t(select_score_floats(batch, heads_kv, heads_q / heads_kv, q_blocks, k_blocks)) * sizeof(float);
 }
 

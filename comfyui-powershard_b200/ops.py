@@ -754,12 +754,12 @@ def block_select(q_means, k_means, keep: int, blocks, counts, query_block: int, 
             raise ValueError(f"block_select: allowed must be bool {(batch, hq, nq, nk)} on {device}")
         mask, strides = allowed.data_ptr(), struct.pack("4q", *allowed.stride())
     n = _select_workspace_bytes(batch, hq, hk, nq, nk) if hk else 0
-    workspace = torch.empty(n, dtype=torch.uint8, device=device)
+    workspace = torch.empty(n, dtype=torch.uint8, device=device) if n else None
     rc = lib.ps_b200_block_select(
         q_means.data_ptr(), k_means.data_ptr(), batch, hq, hk, dim, nq, nk, keep, mask, strides,
         _lengths_arg(query_lengths, batch, device, "block_select query_lengths"), query_block,
         _lengths_arg(key_lengths, batch, device, "block_select key_lengths"), key_block, blocks.data_ptr(),
-        counts.data_ptr(), workspace.data_ptr(), n, _lib.stream_handle(device))
+        counts.data_ptr(), *_ws(workspace), _lib.stream_handle(device))
     if rc:
         _lib.check(rc, "ps_b200_block_select")
 

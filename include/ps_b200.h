@@ -447,8 +447,8 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
  *   score of NaN ranks above all numbers.  blocks [batch][heads_q][q_blocks]
  *   [keep]: the chosen in ascending order, -1 behind them; counts
  *   [batch][heads_q][q_blocks].  keep <= k_blocks <= 16384.  workspace: device
- *   scratch (16-byte aligned) of ps_b200_block_select_workspace_bytes(...) bytes,
- *   owned by one call at a time.
+ *   scratch (16-byte aligned) of ps_b200_block_select_workspace_bytes(...) bytes
+ *   (0: none), owned by one call at a time.
  */
 int ps_b200_block_select(const float* q_means, const float* k_means, int batch, int heads_q, int heads_kv,
                          int head_dim, int q_blocks, int k_blocks, int keep, const unsigned char* allowed,

@@ -180,7 +180,9 @@ def test_entries_validate_on_the_host():
     assert select(nk=30000) == _lib.ERR_UNSUPPORTED and b"larger blocks" in lib.ps_b200_last_error()
     assert select(means=20) == _lib.ERR_INVALID and select(lists=None) == _lib.ERR_INVALID
     assert select(nq=0) == _lib.OK
-    assert select(ws=None) == _lib.ERR_INVALID and select(nbytes=8) == _lib.ERR_INVALID
+    assert select(nk=300, ws=None) == _lib.ERR_INVALID and select(nk=300, nbytes=8) == _lib.ERR_INVALID
+    need = lib.ps_b200_block_select_workspace_bytes
+    assert need(1, 2, 2, 2, 300) >= 4 * 300 * 4 and need(1, 2, 2, 2, 5) == 0  # a few short lists need none
 
     def means(n=1, dtype=_lib.BF16, dim=128, block=64, length=100, x=16, stride=128):
         return lib.ps_b200_block_means(n, struct.pack("P", x), struct.pack("3q", 0, stride, 128), dtype, 1,
