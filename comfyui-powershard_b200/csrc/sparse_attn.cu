@@ -57,8 +57,9 @@ enum SparseBar : int {
                            // (few queries: V_{n-2}), whose PV was issued before
   kP = kFree + kRing,      // [2] P_t written
   kPH = kP + 2,            // [2][kPParts-1]
-  kO = kPH + 2 * (kPParts - 1),  // O_0 and O_1 of a unit final
-  kDrain = kO + 1,
+  kO = kPH + 2 * (kPParts - 1),  // [2] O_t of a unit final; of units in which group t has a tile: such a unit's P_t
+                                 // comes after the last one's O_t, so that no phase passes a waiting group by
+  kDrain = kO + 2,
   kTail = kDrain + 1,      // V rows of a partly used tile loaded
   kMeta = kTail + 1,       // [kMetaRing] rows in use of a tile published
   kWork = kMeta + kMetaRing,  // [2] a unit published
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kMetaRing; ++i) mbar_init(bar(kMeta + i), 1);
     mbar_init(bar(kO), 1);
+    mbar_init(bar(kO + 1), 1);
     mbar_init(bar(kDrain), 1);
     mbar_init(bar(kTail), 1);
     mbar_init(bar(kNext), 1);
@@ -410,6 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           n = n0 + w.tiles;
+          for (int t = 0; t < 2 && ok; ++t)
+            if (w.tiles > 1 || (n0 & 1) == t) umma_commit(bar(kO + t));
         } else {
           // Issue order per key tile: S0_i, PV1_{i-1}, S1_i, PV0_i.  The first S
           // of a unit follow the last PV of the one before on the tensor pipe.
@@ -431,8 +435,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok) ok = pv(0, st, n & 1u, i > 0);
           }
           if (ok && two) ok = pv(1, (n - 1) & 1, (n1 - 1) & 1u, w.tiles > 1);
+          if (ok) umma_commit(bar(kO));
+          if (ok && two) umma_commit(bar(kO + 1));
         }
-        if (ok) umma_commit(bar(kO));
       }
       // All issued UMMAs complete before TMEM is released.
       umma_commit(bar(kDrain));
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + 128 * t, o_addr = tmem + 256 + 128 * t;
     float* rows_o = reinterpret_cast<float*>(smem + kMergeOff);  // of group 1: [kMergeRows][kMergePad], then m, l
     float* rows_ml = rows_o + kMergeRows * kMergePad;
-    int n = 0, loaded = 0;  // tiles; units with tiles
+    int n = 0, loaded = 0, own = 0;  // tiles; units with tiles; units with tiles of this group
     for (int u = 0; (warp & 3) == 0; ++u) {
       const int b = u & 1;
       if (!warp_wait(bar(kWork + b), (u >> 1) & 1u, abort_flag, status, kErrWork)) break;
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       n = end;
       if (tiles > 0) {
-        if (ok) ok = warp_wait(bar(kO), loaded & 1u, abort_flag, status, kErrO);
+        if (ok && any) ok = warp_wait(bar(kO + t), own++ & 1u, abort_flag, status, kErrO);
         // Group 1's staged rows: free to write, or written.
         if (ok && t == 0) ok = warp_wait(bar(kOther), loaded & 1u, abort_flag, status, kErrO);
         if (ok && t == 1 && loaded > 0) ok = warp_wait(bar(kOtherRead), (loaded - 1) & 1u, abort_flag, status, kErrO);
@@ -497,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int rows = args.seg_rows_q;
       // out = (w0 O_0 + w1 O_1) / (w0 l_0 + w1 l_1), w_t = 2^(m_t - max); a group
       // without a tile never wrote its O.
+      // (Without one, group 1 may write here while S_0 reads the query tile: rows of S that nothing reads.)
       if (t == 1) {
         if (tiles == 0) continue;
 #pragma unroll
@@ -594,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_addr = tmem + lane_off + 128 * t;
     const uint32_t o_addr = tmem + lane_off + 256 + 128 * t;
     const float scale_log2 = args.scale_log2;
-    int n = 0, nt = 0, loaded = 0;  // tiles; tiles of this group; units with tiles
+    int n = 0, nt = 0, own = 0;  // tiles; tiles of this group; units with tiles of this group
     for (int u = 0;; ++u) {
       const int b = u & 1;
       if (!warp_wait(bar(kWork + b), (u >> 1) & 1u, abort_flag, status, kErrWork)) break;
@@ -634,10 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       n += tiles;
-      if (tiles > 0) {
-        if (ok && mine) ok = warp_wait(bar(kO), loaded & 1u, abort_flag, status, kErrO);
-        ++loaded;
-      }
+      if (ok && mine && tiles > 0) ok = warp_wait(bar(kO + t), own++ & 1u, abort_flag, status, kErrO);
       if (!ok) break;
       const Work w = small->work[b];
       __syncwarp();

@@ -365,6 +365,28 @@ def test_sparse_attention_lists_of_any_kind(cuda_lib, key_block):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("key_block", [64, 128])
+@pytest.mark.parametrize("b,heads,lq", [(2, 70, 600), (1, 210, 257), (2, 200, 5)])
+def test_units_handed_over(cuda_lib, b, heads, lq, key_block, dtype):
+    """More than 400 units on at most 160 SMs, so that CTAs take unit after unit: units of two query tiles, of one
+    and (few queries) of a few rows, each behind each, with lists of none, one and several key tiles."""
+    from powershard_b200 import sparse
+    lk, n = 700, 5
+    q, k, v = (rows(s, b, m, h, 128, dtype=dtype) for s, m, h in ((70, lq, heads), (71, lk, heads // 10), (72, lk, heads // 10)))
+    nq, nk = -(-lq // 256), -(-lk // key_block)
+    assert b * heads * nq >= 400
+    blocks = random_lists(73, b, heads, nq, nk, n)
+    counts = torch.randint(0, n + 1, (b, heads, nq), generator=torch.Generator().manual_seed(74), dtype=torch.int32)
+    q_len, k_len = lens(lq, lq - lq // 3)[:b], lens(lk, lk - 130)[:b]
+    got = sparse.sparse_attention(*cuda(q, k, v, blocks, counts), key_block=key_block, query_lengths=q_len.to(DEV),
+                                  key_lengths=k_len.to(DEV))
+    torch.cuda.synchronize()
+    sparse._status_for(got.device).check()
+    assert_attention(got, *ref_attention(q, k, v, blocks, counts, 256, key_block, None, q_len, k_len))
+
+
+@pytest.mark.gpu
 def test_sparse_attention_all_blocks_is_dense(cuda_lib):
     """With every block listed in order the result is the dense kernel's."""
     from powershard_b200 import sparse
