@@ -438,7 +438,10 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
     const float len_q = sqrtf(q_sq), len_k = sqrtf(__uint_as_float(longest));
     const float E2 = 6.103515625e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-14, 2^-110
     uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
-    if (kth < ~0u - 1 && len_q * len_k < 1e38f && isfinite(T - E2) && isfinite(T + E2)) {
+    // (Squares below 2^-100 of the lengths may have lost what they were made of to underflow.)
+    const float least_sq = fminf(q_sq, __uint_as_float(longest));
+    if (kth < ~0u - 1 && least_sq > 7.888609052210118e-31f && len_q * len_k < 1e38f && isfinite(T - E2) &&
+        isfinite(T + E2)) {
       lo_key = order_key(T - E2);
       hi_key = order_key(T + E2);
     }

@@ -290,6 +290,22 @@ def test_select_in_64_bits(cuda_lib, nk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_size,k_size", [(1.0, 1e-24), (1e-24, 1.0), (1e-30, 1e10), (3e-16, 1.0), (1e-17, 1e-17)])
+def test_select_of_tiny_rows(cuda_lib, q_size, k_size):
+    """Rows whose squares underflow 32 bits, with neighbouring scores 2^-21 apart: nearer than 32 bits tell them."""
+    from powershard_b200 import sparse
+    g = torch.Generator().manual_seed(33)
+    nk = 700
+    step = 1 + torch.randperm(nk, generator=g).double() * 2.0 ** -21
+    km = (torch.randn(1, 1, 1, 128, generator=g).double() * step[None, :, None, None] * k_size).float()
+    qm = torch.randn(1, 5, 1, 128, generator=g) * q_size
+    for keep in (1, 175, 400):
+        got = [t.cpu() for t in sparse.select_blocks(*cuda(qm, km), keep)]
+        want = ref_select(qm, km, keep)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), keep
+
+
+@pytest.mark.gpu
 def test_forward_only(cuda_lib):
     """What autograd would have to differentiate is refused, and runs where it records nothing."""
     from powershard_b200 import sparse
