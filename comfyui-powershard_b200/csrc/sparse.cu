@@ -126,7 +126,7 @@ __device__ __forceinline__ float of_key(uint32_t k) {
   return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
-// x = hi + lo + at most 2^-18 x, two bf16 numbers; pairs of them packed for the tensor cores.
+// x = hi + lo + at most 2^-17 x, two bf16 numbers (of 8 bits: lo is at most 2^-8 x); pairs of them packed for the tensor cores.
 __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16x2(x, y);
   lo = pack_bf16x2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
@@ -149,10 +149,10 @@ __device__ __forceinline__ int blocks_in_use(const int* len, int batch, int bloc
 // list each) against 128 key blocks, and the largest squared length of their means.
 //
 // On the tensor cores: each mean is split into two bf16 terms and the three
-// larger products are summed in 32 bits, which is off by less than E = 2^-15
-// |q| max |k| (the terms leave 2 * 2^-18, the dropped product 2^-18; 8 sums of
-// the main products, 17 terms each, keep 24 bits of their largest: 2^-16.9; the
-// sums of the small products are 2^-8 of that) plus what may underflow.
+// larger products are summed in 32 bits, which is off by less than E = 2^-14
+// |q| max |k| (the terms leave 2 * 2^-17, the dropped product 2^-16; 8 sums of
+// the main products, 17 terms each, lose at most 2^-23 of their largest a term:
+// 2^-15.9; the sums of the small products 2^-8 of that) plus what may underflow.
 // pick_kernel turns to 64 bits where that decides.  (Two tf32 terms are closer,
 // but take twice the products and, split between them, six times the other
 // arithmetic: 24 against 11 us for 1182 key blocks and 296 query blocks of 5
@@ -304,7 +304,7 @@ struct CtaSum {
 //
 // With T the keep-th largest score, a block above T + 2E is chosen and one
 // below T - 2E is not, in 64 bits too; only the blocks between (the T block
-// alone, in two lists of three) are scored again in 64 bits.
+// alone, in half of the lists) are scored again in 64 bits.
 //
 // T is found by counting the keys above a cut, first where the keep-th of as
 // many normal scores lies, then where the counts at the ends put it on a
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(32 * kWarps) pick_kernel(const SelectArgs a) {
     for (int w = 0; w < kWarps; ++w) kth = min(kth, ends[2][w]);
     const float T = of_key(kth);
     const float len_q = sqrtf(q_sq), len_k = sqrtf(__uint_as_float(longest));
-    const float E2 = 6.103515625e-05f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-14, 2^-110
+    const float E2 = 1.220703125e-04f * len_q * len_k + 7.70371978e-34f * (1.f + len_q + len_k);  // 2^-13, 2^-110
     uint32_t lo_key = 1, hi_key = ~0u - 1;  // undecided: every block, where E says nothing
     // (Squares below 2^-100 of the lengths may have lost what they were made of to underflow.)
     const float least_sq = fminf(q_sq, __uint_as_float(longest));

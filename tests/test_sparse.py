@@ -306,6 +306,28 @@ def test_select_of_tiny_rows(cuda_lib, q_size, k_size):
 
 
 @pytest.mark.gpu
+def test_select_where_two_terms_leave_most(cuda_lib):
+    """Means around 1 + 2^-8, where a second 8-bit term leaves the most (2^-17) and the product of the second
+    terms is largest (2^-16), in both signs: blocks of either kind take turns in the exact order."""
+    from powershard_b200 import sparse
+    g = torch.Generator().manual_seed(34)
+    nk = 600
+    kind = torch.arange(nk) % 2  # second term just below 2^-8 and cut off, just above -2^-8 and rounded up
+    base = torch.where(kind == 0, 1 + 2.0 ** -8 - 2.0 ** -16 + 2.0 ** -17 - 2.0 ** -20,
+                       1 + 2.0 ** -8 + 2.0 ** -16 - 2.0 ** -17 + 2.0 ** -20).double()
+    km = base[:, None].repeat(1, 128)
+    flip = torch.rand(nk, 128, generator=g) < 0.02
+    km = torch.where(flip, km * (1 + 2.0 ** -22), km) * (1 - 2.0 ** -21 * torch.randperm(nk, generator=g)[:, None].double())
+    km = km.float()[None, :, None]
+    for q in (1 + 2.0 ** -8 - 2.0 ** -17, 1 + 2.0 ** -8 + 2.0 ** -17):
+        qm = torch.full((1, 3, 1, 128), q)
+        qm[0, 1, :, ::2] *= -1
+        for keep in (1, 150, 300, 450):
+            got = sparse.select_blocks(*cuda(qm, km), keep)[0].cpu()
+            assert torch.equal(got, ref_select(qm, km, keep)[0]), keep
+
+
+@pytest.mark.gpu
 def test_forward_only(cuda_lib):
     """What autograd would have to differentiate is refused, and runs where it records nothing."""
     from powershard_b200 import sparse
