@@ -26,28 +26,27 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kScoreRows = 64, kScoreKeys = 16 * kWarps;  // of one CTA of score_kernel
 
 template <bool kFp16>
-__device__ __forceinline__ void add8(float (&a)[8], const uint4& v) {
+__device__ __forceinline__ void add8(double (&a)[8], const uint4& v) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if constexpr (kFp16)
-      asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.f16 %0, l, %0;\n\tadd.f32.f16 %1, h, %1;\n\t}"
-          : "+f"(a[2 * i]), "+f"(a[2 * i + 1])
-          : "r"(w[i]));
-    else
-      asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.f32.bf16 %0, l, %0;\n\tadd.f32.bf16 %1, h, %1;\n\t}"
-          : "+f"(a[2 * i]), "+f"(a[2 * i + 1])
-          : "r"(w[i]));
+    const float2 f = kFp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
+                           : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    a[2 * i] += static_cast<double>(f.x);
+    a[2 * i + 1] += static_cast<double>(f.y);
   }
 }
 
 // A warp sums up to 32 rows of one block and pair of heads, 512 bytes a row;
 // the warps that share a block lie in one CTA and add up through shared memory.
-// Four values are added in 32 bits (exact for 16-bit values within a few
-// binades) before the 64-bit sum, which keeps the conversions to 64 bits (16 a
-// clock and SM) at a quarter of the values.  Bound by HBM: every value is read
-// once.  16 loads a thread in flight and three CTAs an SM: 335 MB in 53 us (6.3
-// TB/s), 168 MB in 33.5 us; with 8 loads 36-38 us, with 32 (two CTAs) 37 us.
+// Every value is added in 64 bits, as in the selection where it takes the
+// queries' means itself: sums of values within 2^30 of each other are exact, so
+// that both give the same means, and none overflows.  Bound by HBM and, close
+// behind, the conversions to 64 bits (16 a clock and SM): every value is read
+// once, 16 loads a thread in flight and three CTAs an SM.  97 MB in 23.2 us, 168 in
+// 36.7, 335 in 64.7 (5.2 TB/s); adding four values in 32 bits first, which loses
+// what they cancel, takes 20.7, 33.5 and 59.5, building the 64-bit numbers with
+// whole-number instructions 23.0, 37.1 and 65.9; 8 loads 24.9, 37.4 and 67.8.
 template <bool kFp16>
 __global__ void __launch_bounds__(kThreads, 3) block_means_kernel(const MeansArgs args) {
   __shared__ double part[kWarps][32 * 9];
@@ -85,11 +84,8 @@ __global__ void __launch_bounds__(kThreads, 3) block_means_kernel(const MeansArg
           const int row = r + u * per;
           v[u] = row < rows ? load_once(base + row * step) : make_uint4(0, 0, 0, 0);
         }
-        float a[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < 4; ++u) add8<kFp16>(a, v[u]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] += static_cast<double>(a[e]);
+        for (int u = 0; u < 4; ++u) add8<kFp16>(sum, v[u]);
       }
     }
   }

@@ -429,7 +429,7 @@ int ps_b200_out_proj(const void* src, int64_t src_row_stride, int64_t src_block_
  *   [batch][ceil(len[t]/block[t])][heads[t]][head_dim].  lens (may be NULL, as
  *   may lens[t]): device int [batch], rows in use (clamped to [0, len]); only
  *   those count, and a block without any has mean zero.  Values are added in
- *   64 bits, each four in 32 bits first (so |x| < 2^125).
+ *   64 bits.
  */
 int ps_b200_block_means(int tensors, const void* const* x, const int64_t* strides, int dtype, int batch,
                         const int* len, const int* heads, int head_dim, const int* block, const int* const* lens,

@@ -213,6 +213,56 @@ def test_block_means(cuda_lib, n, heads, block, dtype):
     assert torch.equal(sparse.block_means(wide, block, used.to(DEV))[:, :, 2].double().cpu(), got[:, :, 0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,block", [(4, 64), (1000, 256), (517, 64), (130, 7)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_block_means_of_any_values(cuda_lib, n, block, dtype):
+    """Values of very different size, that cancel, subnormal, near the largest, infinite and NaN.  The means are
+    64-bit sums: 1000 roundings of 2^-53 of the rows' magnitude and one of 2^-24 of the mean (2^-150 where it is
+    subnormal)."""
+    from powershard_b200 import sparse
+    g = torch.Generator().manual_seed(35)
+    span = (30, 24) if dtype == torch.bfloat16 else (14, 10)
+    x = torch.randn(1, n, 3, 128, generator=g) * 2.0 ** torch.randint(-span[0], span[1], (1, n, 3, 128), generator=g)
+    x[:, 1::2, 1] = -x[:, :n - n % 2:2, 1][:, :x[:, 1::2].shape[1]]  # pairs that cancel
+    x = x.to(dtype)
+    most = torch.finfo(dtype).max
+    x[:, :, 2, 0] = most  # sums of it overflow 32 bits in bf16
+    x[:, :, 2, 1] = torch.finfo(dtype).smallest_normal / 4
+    x[:, ::3, 2, 2] = 0
+    x[0, :4, 2, 3] = torch.tensor([60000.0, 0.0015, -60000.0, 0.0]).to(dtype)
+    x[0, 4:, 2, 3] = 0
+    got = sparse.block_means(x.to(DEV), block).double().cpu()
+    want, size = ref_means(x, block), ref_means(x.abs(), block)
+    assert ((got - want).abs() <= 2.0 ** -24 * want.abs() + 1000 * 2.0 ** -53 * size + 2.0 ** -150).all()
+    x[0, n - 1, 0, 5], x[0, 0, 1, 6], x[0, n - 1, 1, 7] = math.inf, -math.inf, math.nan
+    x[0, 0, 0, 8], x[0, min(block, n) - 1, 0, 8] = math.inf, -math.inf
+    got, want = sparse.block_means(x.to(DEV), block).cpu(), ref_means(x, block).float()
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    assert torch.equal(got[odd & ~torch.isnan(want)], want[odd & ~torch.isnan(want)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [20, 200])
+@pytest.mark.parametrize("lk", [3000, 30000])
+def test_provider_means_do_not_depend_on_who_takes_them(cuda_lib, lq, lk):
+    """Queries that cancel except for a few thousandths, which decide the selection: with key means kept and
+    taken, few rows and more."""
+    from powershard_b200 import sparse
+    q, v = torch.zeros(1, lq, 2, 128, dtype=torch.float16), rows(36, 1, lk, 2, 128, dtype=torch.float16)
+    q[:, 0, :, 0], q[:, 8, :, 0], q[:, 16, :, 0] = 60000.0, 0.0015, -60000.0
+    q[:, 0, :, 1] = 0.0002
+    k = torch.zeros(1, lk, 2, 128, dtype=torch.float16)
+    k[:, 640:704, :, 0] = 1.0
+    k[:, 1280:1344, :, 1] = 1.0
+    p = sparse.SparseProvider(1, key_block=64)
+    want = ref_provider(q, k, v, 1, 256, 64)
+    args = cuda(q, k, v)
+    assert_attention(p(*args), *want)
+    assert_attention(p(*args, key_means=sparse.block_means(args[1], 64)), *want)
+
+
 # ------------------------------------------------------------------ selection
 @pytest.mark.gpu
 @pytest.mark.parametrize("b,nq,nk,heads,kv,keep", [
