@@ -478,10 +478,11 @@ __device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, f
 // (2^x0, 2^x1) on the FMA pipe, relative error 7.5e-5: with k = round(x) and f =
 // x - k, 2^k times the cubic closest to 2^f on [-1/2, 1/2] in relative error
 // (by the exchange algorithm).  Adding 1.5 * 2^23 + 127 leaves k + 127 in the low
-// bits, which a shift makes 2^k.  Below -126 the result is 2^-126; NaN stays NaN.
+// bits, which a shift makes 2^k.  Below -126.5 the result is 0 (k = -127 leaves
+// nothing in the exponent), so that a key without weight adds nothing; NaN stays NaN.
 __device__ __forceinline__ void ex2_pair(float& y0, float& y1, float x0, float x1) {
   asm("{\n\t.reg .b32 a, b;\n\t.reg .b64 x, t, k, f, p, m, c;\n\t"
-      "max.NaN.f32 a, %2, 0fC2FC0000;\n\tmax.NaN.f32 b, %3, 0fC2FC0000;\n\tmov.b64 x, {a, b};\n\t"
+      "max.NaN.f32 a, %2, 0fC2FE0000;\n\tmax.NaN.f32 b, %3, 0fC2FE0000;\n\tmov.b64 x, {a, b};\n\t"
       "mov.b64 m, {%4, %4};\n\tadd.rn.f32x2 t, x, m;\n\t"
       "mov.b64 c, {%5, %5};\n\tadd.rn.f32x2 k, t, c;\n\t"
       "sub.rn.f32x2 f, x, k;\n\t"

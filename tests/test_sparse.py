@@ -547,6 +547,24 @@ def test_scores_far_apart(cuda_lib, lq):
         assert_attention(got, *ref_attention(q, k, v, blocks, key_block=64, scale=scale))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq", [3, 300])
+def test_values_of_keys_far_away(cuda_lib, lq):
+    """Keys whose probability is nothing (e^-500 and less) may hold values near the largest."""
+    from powershard_b200 import sparse
+    q, k = (torch.ones(1, n, 2, 128, dtype=torch.bfloat16) for n in (lq, 256))
+    v = rows(63, 1, 256, 2, 128)
+    far = torch.arange(256) % 3 > 0
+    k[:, far] = -1.0
+    v[:, far] = 1e38
+    blocks = torch.tensor([0, 1], dtype=torch.int32).expand(1, 2, -(-lq // 256), 2).contiguous()
+    got = sparse.sparse_attention(*cuda(q, k, v, blocks), softmax_scale=2.0)
+    want, _ = ref_attention(q, k, v, blocks, scale=2.0)
+    near, mag = ref_attention(q, k, torch.where(far[None, :, None, None], torch.zeros_like(v), v), blocks, scale=2.0)
+    assert (want - near).abs().max() <= 1e-100
+    assert_attention(got, near, mag)
+
+
 # ------------------------------------------------------------------ the provider
 def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_len=None, k_len=None, scale=None):
     used = lambda n, block: None if n is None else [-(-int(x) // block) for x in n]  # noqa: E731
