@@ -349,6 +349,17 @@ SparseScratch sparse_scratch(int64_t batch, int64_t heads_q, int64_t heads_kv, i
   return s;
 }
 
+// Batch, row and head strides of 16-bit rows, read or written 16 bytes at a
+// time; that of an axis of at most one entry is never used, so its value says nothing.
+bool row_strides(const int64_t* st, int64_t batch, int64_t rows, int64_t heads, int64_t out[3]) {
+  const int64_t extents[3] = {batch, rows, heads};
+  for (int i = 0; i < 3; ++i) {
+    out[i] = extents[i] > 1 ? st[i] : 0;
+    if (out[i] < 0 || out[i] % 8 != 0) return false;
+  }
+  return true;
+}
+
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 }  // namespace
@@ -1046,11 +1057,8 @@ int ps_b200_block_means(int tensors, const void* const* x, const int64_t* stride
     if (m.ctas == 0) continue;
     if (!x[t] || !aligned16(x[t])) return set_error(PS_B200_ERR_INVALID, "tensor %d null or not 16-byte aligned", t);
     if (!out[t] || !aligned4(out[t])) return set_error(PS_B200_ERR_INVALID, "means %d null or not 4-byte aligned", t);
-    for (int i = 0; i < 3; ++i) {
-      m.st[i] = strides[3 * t + i];
-      if (m.st[i] < 0 || m.st[i] % 8 != 0)
-        return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
-    }
+    if (!row_strides(strides + 3 * t, batch, len[t], heads[t], m.st))
+      return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
     m.x = x[t];
     m.lens = lens ? lens[t] : nullptr;
     if (!aligned4(m.lens)) return set_error(PS_B200_ERR_INVALID, "lengths must be 4-byte aligned");
@@ -1152,9 +1160,9 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
   if (!q || !k || !v || !out) return set_error(PS_B200_ERR_INVALID, "null tensor pointer");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
     return set_error(PS_B200_ERR_INVALID, "tensor pointers must be 16-byte aligned");
-  for (int i = 0; i < 3; ++i)
-    if (out_strides[i] < 0 || out_strides[i] % 8 != 0)
-      return set_error(PS_B200_ERR_INVALID, "output strides must be non-negative multiples of 8 elements");
+  int64_t os[3];
+  if (!row_strides(out_strides, batch, len_q, heads_q, os))
+    return set_error(PS_B200_ERR_INVALID, "output strides must be non-negative multiples of 8 elements");
   if (!blocks || !aligned4(blocks) || !aligned4(counts) || !aligned4(q_len) || !aligned4(k_len))
     return set_error(PS_B200_ERR_INVALID, "list, count and length tables must be 4-byte aligned, the lists not null");
   if (!aligned4(status)) return set_error(PS_B200_ERR_INVALID, "status word must be 4-byte aligned");
@@ -1171,9 +1179,9 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
   if (int rc = make_map(&tk, k, fp16, head_dim, heads_kv, len_k, 1, batch, ks, a.piece)) return rc;
   if (int rc = make_map(&tv, v, fp16, head_dim, heads_kv, len_k, 1, batch, vs, a.piece)) return rc;
   a.seg_out[0] = a.pre_out = out;
-  a.o_stride[0] = out_strides[0];
-  a.o_stride[2] = out_strides[1];
-  a.o_stride[3] = out_strides[2];
+  a.o_stride[0] = os[0];
+  a.o_stride[2] = os[1];
+  a.o_stride[3] = os[2];
   a.seg_rows_q = a.valid_q[0] = len_q;
   a.seg_rows_k = a.valid_k[0] = len_k;
   a.nsegs_q = a.nsegs_k = 1;
@@ -1262,11 +1270,8 @@ int ps_b200_sparse_fwd(const ps_b200_sparse_call* c, void* stream) {
     if (!is16bit(dtype)) return set_error(PS_B200_ERR_UNSUPPORTED, "block-sparse attention supports bf16 and fp16 only");
     if (!c->q || !aligned16(c->q)) return set_error(PS_B200_ERR_INVALID, "queries null or not 16-byte aligned");
     from.q = c->q;
-    for (int i = 0; i < 3; ++i) {
-      from.q_st[i] = c->q_strides[i];
-      if (from.q_st[i] < 0 || from.q_st[i] % 8 != 0)
-        return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
-    }
+    if (!row_strides(c->q_strides, batch, lq, hq, from.q_st))
+      return set_error(PS_B200_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
     from.len_q = lq;
     from.fp16 = dtype == PS_B200_FP16;
   }
@@ -1330,10 +1335,9 @@ static int cache_common(bool write, const ps_b200_cache_call* c, void* stream) {
     a.pages[t] = c->pages[t];
     a.scales[t] = c->scales[t];
     a.rows[t] = c->rows[t];
+    if (!row_strides(c->strides + 3 * t, c->batch, c->n, c->heads, a.st[t]))
+      return set_error(PS_B200_ERR_INVALID, "row strides must be non-negative multiples of 8 elements");
     for (int i = 0; i < 3; ++i) {
-      a.st[t][i] = c->strides[3 * t + i];
-      if (a.st[t][i] < 0 || a.st[t][i] % 8 != 0)
-        return set_error(PS_B200_ERR_INVALID, "row strides must be non-negative multiples of 8 elements");
       if (!write && a.st[t][i] == 0 && extents[i] > 1)
         return set_error(PS_B200_ERR_INVALID, "a read needs rows of their own: stride 0 of an axis of %lld",
                          (long long)extents[i]);

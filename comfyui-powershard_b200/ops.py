@@ -678,6 +678,8 @@ def _row_strides(t: torch.Tensor, what: str):
     """(batch, row, head) strides of a [B, L, H, D] tensor the kernels can read."""
     _check16(t, what)
     st = t.stride()
+    if 1 in t.shape:  # the stride of an axis of one entry says nothing
+        st = tuple(0 if n == 1 and i < 3 else s for i, (s, n) in enumerate(zip(st, t.shape)))
     if len(st) != 4 or st[3] != 1 or st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
         raise ValueError(f"{what}: expected [B, L, H, D] with unit head-dim stride, other strides multiples of 8 "
                          f"elements and a 16-byte aligned base, got {tuple(t.shape)} / {st}")

@@ -194,6 +194,18 @@ def test_strided_rows_and_a_shared_pool(cuda_lib):
 
 
 @pytest.mark.gpu
+def test_strides_of_axes_of_one(cuda_lib):
+    """The stride of an axis with one entry says nothing."""
+    for n, heads in ((9, 2), (1, 2), (9, 1)):
+        x = rows(7, 1, n, heads, 128).to(DEV)
+        st = [3 if m == 1 else s for m, s in zip(x.shape, x.stride())]
+        cache, table, out = new_cache(1, 16, heads, 128, torch.int8), lens(0)[None].to(DEV), [torch.zeros_like(x) for _ in range(2)]
+        cache.write(x.as_strided(x.shape, st), x, table)
+        cache.read(table, lens(n).to(DEV), out[0].as_strided(x.shape, st), out[1])
+        assert torch.equal(*out) and out[0].any()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(cuda_lib):
     """A pool of more than 2^32 codes: rows on its last pages."""
     pages = 2 ** 32 // (256 * 16 * 128) + 3

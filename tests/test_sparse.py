@@ -638,6 +638,26 @@ def test_provider_on_strided_inputs_streams_and_graphs(cuda_lib):
 
 
 @pytest.mark.gpu
+def test_strides_of_axes_of_one(cuda_lib):
+    """The stride of an axis with one entry says nothing."""
+    from powershard_b200 import sparse
+    for lq, heads in ((300, 2), (1, 2), (300, 1), (5, 1)):
+        q, k, v = (rows(s, 1, n, heads, 128).to(DEV) for s, n in ((64, lq), (65, 700), (66, 700)))
+        odd = []
+        for t in (q, k, v):
+            st = [3 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+            odd.append(t.as_strided(t.shape, st))
+            assert odd[-1].is_contiguous()
+        p = sparse.SparseProvider(3)
+        assert torch.equal(p(*odd), p(q, k, v))
+        means = sparse.block_means(k, 128)
+        assert torch.equal(sparse.block_means(odd[1], 128), means)
+        assert torch.equal(p(*odd, key_means=means), p(q, k, v, key_means=means))
+        lists = torch.zeros(1, heads, -(-lq // 256), 1, dtype=torch.int32, device=DEV)
+        assert torch.equal(sparse.sparse_attention(*odd, lists), sparse.sparse_attention(q, k, v, lists))
+
+
+@pytest.mark.gpu
 def test_results_do_not_depend_on_what_memory_held(cuda_lib):
     """Two runs give the same bits, with the allocator's blocks full of NaN in between."""
     from powershard_b200 import sparse
