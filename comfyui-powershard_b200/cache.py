@@ -76,8 +76,8 @@ class StreamingAttention:
         """q, k, v [B, n, H, D] new rows -> [B, n, Hq, D].
 
         start: rows that the sequences hold already, an int for all of them or
-        an int32 device tensor [B]; lengths: new rows in use, int32 [B] or None
-        for all; context: rows of the longest sequence with the new ones, needed
+        an int32 device tensor [B]; lengths: new rows in use, int32 [B] (taken
+        as within [0, n]) or None for all; context: rows of the longest sequence with the new ones, needed
         with a tensor (rows behind it are held but not attended); selection:
         ``allowed`` of a sparse provider."""
         _no_grad(q, k, v)
@@ -93,6 +93,8 @@ class StreamingAttention:
             raise ValueError("context: the rows of the longest sequence, with start on the device")
         if isinstance(start, int):
             start = torch.full((b,), start, dtype=torch.int32, device=k.device)
+        if lengths is not None:
+            lengths = lengths.clamp(0, n)  # of what the write takes
         self.cache.write(k, v, table, start, lengths)
         held = start + (n if lengths is None else lengths)
         keys, values = (torch.empty((b, context, *k.shape[2:]), dtype=k.dtype, device=k.device) for _ in range(2))

@@ -296,3 +296,21 @@ def test_streaming_dense_and_captured(cuda_lib):
     ks2, vs2 = (torch.cat([w[0][:, :100], w[1]], 1) for w in ([a[0] for a in whole], [a[1] for a in whole]))
     every = torch.arange(3, dtype=torch.int32).expand(1, 2, 1, -1)
     assert_attention(graphed.out, *ref_attention(q2, ks2, vs2, every))
+
+
+@pytest.mark.gpu
+def test_streaming_lengths_beyond_the_rows(cuda_lib):
+    """New rows in use are counted from 0 to the rows given: what a sequence held is neither shortened nor is
+    anything attended that this step did not write (a page's earlier content)."""
+    from powershard_b200 import sparse
+    from powershard_b200.cache import StreamingAttention
+    table = tables(9, 2, 4).to(DEV)
+    q, k, v = (rows(80 + i, 2, 40, 2, 128).to(DEV) for i in range(3))
+    old = [rows(83 + i, 2, 256, 2, 128, scale=5.0).to(DEV) for i in range(2)]
+
+    def step(*used):
+        cache = new_cache(10, 64, 2, 128, torch.int8)
+        cache.write(*old, table)  # stale rows behind position 100, earlier tokens before it
+        attend = StreamingAttention(cache, sparse.SparseProvider(1.0, key_block=64))
+        return attend(q, k, v, table, lens(100, 100).to(DEV), context=256, lengths=lens(*used).to(DEV))
+    assert torch.equal(step(90, -30), step(40, 0))
