@@ -79,7 +79,12 @@ class StreamingAttention:
         an int32 device tensor [B]; lengths: new rows in use, int32 [B] (taken
         as within [0, n]) or None for all; context: rows of the longest sequence with the new ones, needed
         with a tensor (rows behind it are held but not attended); selection:
-        ``allowed`` of a sparse provider."""
+        ``allowed`` of a sparse provider.
+
+        The table must name a page for every position below the rows held with
+        the new ones and below ``context``: that it has as many entries is
+        checked, but the pages are on the device, and a position whose page is
+        out of range is attended as a key and a value of zeros."""
         _no_grad(q, k, v)
         b, n = k.shape[:2]
         ragged = lengths is not None or not isinstance(start, int)
@@ -91,6 +96,9 @@ class StreamingAttention:
             context = start + n
         elif context is None:
             raise ValueError("context: the rows of the longest sequence, with start on the device")
+        rows = table.shape[-1] * self.cache.k.shape[1]
+        if context > rows:
+            raise ValueError(f"the page table names {rows} rows of a sequence, a context of {context} needs more pages")
         if isinstance(start, int):
             start = torch.full((b,), start, dtype=torch.int32, device=k.device)
         if lengths is not None:

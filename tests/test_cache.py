@@ -94,6 +94,18 @@ def test_entries_validate_on_the_host():
     assert lib.ps_b200_kernel_launches() == 0
 
 
+def test_streaming_refuses_a_page_table_too_short():
+    from powershard_b200.cache import KVCache, StreamingAttention
+    from powershard_b200.sparse import SparseProvider
+    k = torch.zeros(4, 16, 2, 128, dtype=torch.int8)
+    cache = KVCache.over(k, k, torch.zeros(4, 16, 2), torch.zeros(4, 16, 2))
+    x = rows(0, 1, 4, 2, 128)
+    for table in (torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 0, dtype=torch.int32)):
+        for start, context in ((29, None), (lens(3), 33)):
+            with pytest.raises(ValueError, match="page table"):
+                StreamingAttention(cache, SparseProvider(1.0))(x, x, x, table, start, context=context)
+
+
 # ------------------------------------------------------------------ write and read
 @pytest.mark.gpu
 @pytest.mark.parametrize("stored", [torch.float8_e4m3fn, torch.int8])
