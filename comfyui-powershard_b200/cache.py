@@ -14,6 +14,7 @@ block-sparse).
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib, ops
 from .contract import AttentionOptions
@@ -27,7 +28,9 @@ class KVCache:
     Position p of sequence b is row ``p % page_rows`` of page
     ``table[b, p // page_rows]`` (int32 [B, n], on the cache's device).  Which
     pages a sequence owns is the caller's book-keeping; sequences may share
-    pages that they only read.  One ``write`` must not name a position twice."""
+    pages that they only read.  One ``write`` must not name a position twice.
+    Both calls run forward only (rows that require grad are refused while
+    autograd records) and count as operations in place on what they change."""
 
     def __init__(self, pages: int, page_rows: int, heads: int, head_dim: int = 128,
                  dtype: torch.dtype = torch.float8_e4m3fn, device=None):
@@ -54,12 +57,16 @@ class KVCache:
     def write(self, k, v, table, start=None, lengths=None):
         """Rows i < lengths[b] (None: all) of k, v [B, n, heads, head_dim] to
         positions start[b] + i (None: i) of sequence b.  Rows without a page are dropped."""
+        _no_grad(k, v)
         ops.cache_write((self.k, self.v), (self.k_scale, self.v_scale), (k, v), table, start, lengths)
+        increment_version((self.k, self.v, self.k_scale, self.v_scale))
 
     def read(self, table, lengths, k_out, v_out, first=None):
         """Positions first[b] + i (None: i) below lengths[b] into row i of k_out,
         v_out [B, n, heads, head_dim] (bf16 or fp16); the other rows stay as they are."""
+        _no_grad(k_out, v_out)
         ops.cache_read((self.k, self.v), (self.k_scale, self.v_scale), (k_out, v_out), table, lengths, first)
+        increment_version((k_out, v_out))
 
 
 class StreamingAttention:

@@ -106,6 +106,19 @@ def test_streaming_refuses_a_page_table_too_short():
                 StreamingAttention(cache, SparseProvider(1.0))(x, x, x, table, start, context=context)
 
 
+def test_cache_refuses_what_autograd_would_record():
+    from powershard_b200.cache import KVCache
+    from powershard_b200.contract import UnsupportedAttention
+    k = torch.zeros(4, 16, 2, 128, dtype=torch.int8)
+    cache = KVCache.over(k, k, torch.zeros(4, 16, 2), torch.zeros(4, 16, 2))
+    x, leaf = rows(0, 1, 4, 2, 128), rows(0, 1, 4, 2, 128).requires_grad_()
+    for a, b in ((leaf, x), (x, leaf)):
+        with pytest.raises(UnsupportedAttention, match="grad"):
+            cache.write(a, b, lens(0)[None])
+        with pytest.raises(UnsupportedAttention, match="grad"):
+            cache.read(lens(0)[None], lens(4), a, b)
+
+
 # ------------------------------------------------------------------ write and read
 @pytest.mark.gpu
 @pytest.mark.parametrize("stored", [torch.float8_e4m3fn, torch.int8])
@@ -232,6 +245,31 @@ def test_offsets_past_32_bits(cuda_lib):
         codes, s = quantise(x, torch.int8)
         assert torch.equal(y.cpu(), (codes.float() * s[..., None]).to(torch.bfloat16))
     assert not cache.k[:pages - 2].any()
+
+
+@pytest.mark.gpu
+def test_autograd_sees_what_a_call_overwrites(cuda_lib):
+    """A tensor that autograd keeps for a backward pass and that read or write changes is noticed, as after any
+    other operation in place; inference tensors have no such count."""
+    cache = new_cache(2, 16, 2, 128, torch.int8)
+    table = lens(0)[None].to(DEV)
+    x = rows(90, 1, 4, 2, 128).to(DEV)
+    out = [torch.zeros_like(x) for _ in range(2)]
+    leaf = torch.ones((), device=DEV, dtype=x.dtype, requires_grad=True)
+    for i in range(2):
+        y = (leaf * out[i]).sum()
+        cache.read(table, lens(4).to(DEV), *out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    wide = torch.ones((), device=DEV, requires_grad=True)
+    y = (wide * cache.k_scale).sum()
+    cache.write(x, x, table)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        out = [torch.zeros_like(x) for _ in range(2)]
+        cache.read(table, lens(4).to(DEV), *out)
+    cache.read(table, lens(4).to(DEV), *out)
 
 
 # ------------------------------------------------------------------ the operators together
