@@ -25,6 +25,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from .contract import AttentionOptions, UnsupportedAttention
@@ -61,10 +62,14 @@ def _broadcast(allowed, shape):
 
 
 def _no_grad(*tensors):
-    """The kernels run forward only: a call that autograd would record is refused."""
+    """The kernels run forward only: a call that autograd would record, or whose tangents it would carry on, is refused."""
     for t in tensors:
         if t.requires_grad and torch.is_grad_enabled():
             raise UnsupportedAttention("b200_sparse: forward only, an input requires grad")
+    if forward_ad._current_level >= 0:  # inside a dual_level only
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise UnsupportedAttention("b200_sparse: an input has a forward-mode tangent, which would be lost")
 
 
 def block_means(x, block: int, lengths=None):

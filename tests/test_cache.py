@@ -119,6 +119,23 @@ def test_cache_refuses_what_autograd_would_record():
             cache.read(lens(0)[None], lens(4), a, b)
 
 
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    from powershard_b200 import sparse
+    from powershard_b200.cache import KVCache
+    from powershard_b200.contract import UnsupportedAttention
+    k = torch.zeros(4, 16, 2, 128, dtype=torch.int8)
+    cache = KVCache.over(k, k, torch.zeros(4, 16, 2), torch.zeros(4, 16, 2))
+    x, m = rows(0, 1, 4, 2, 128), torch.zeros(1, 2, 2, 128)
+    with fwd.dual_level():
+        d, dm = fwd.make_dual(x, x), fwd.make_dual(m, m)
+        for call in (lambda: cache.write(x, d, lens(0)[None]), lambda: cache.read(lens(0)[None], lens(4), d, x),
+                     lambda: sparse._no_grad(x, d), lambda: sparse._no_grad(dm)):
+            with pytest.raises(UnsupportedAttention, match="tangent"):
+                call()
+        sparse._no_grad(x, m)
+
+
 # ------------------------------------------------------------------ write and read
 @pytest.mark.gpu
 @pytest.mark.parametrize("stored", [torch.float8_e4m3fn, torch.int8])
