@@ -18,6 +18,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib, ops
 from .contract import AttentionOptions
+from .provider import B200Provider
 from .sparse import SparseProvider, _no_grad
 
 
@@ -84,9 +85,9 @@ class StreamingAttention:
 
         start: rows that the sequences hold already, an int for all of them or
         an int32 device tensor [B]; lengths: new rows in use, int32 [B] (taken
-        as within [0, n]) or None for all; context: rows of the longest sequence with the new ones, needed
-        with a tensor (rows behind it are held but not attended); selection:
-        ``allowed`` of a sparse provider.
+        as within [0, n]) or None for all; context: rows of the longest sequence
+        with the new ones, needed with a tensor (rows behind it are held but not
+        attended); selection: ``allowed`` of a sparse provider.
 
         The table must name a page for every position below the rows held with
         the new ones and below ``context``: that it has as many entries is
@@ -106,13 +107,19 @@ class StreamingAttention:
         rows = table.shape[-1] * self.cache.k.shape[1]
         if context > rows:
             raise ValueError(f"the page table names {rows} rows of a sequence, a context of {context} needs more pages")
+        keys, values = (torch.empty((b, context, *k.shape[2:]), dtype=k.dtype, device=k.device) for _ in range(2))
+        if isinstance(self.provider, B200Provider):  # before the write: a refused step changes nothing
+            self.provider.check(q, keys, values, options or AttentionOptions())
+            if isinstance(self.provider, SparseProvider):
+                self.provider.check_selection(q, keys, selection.get("allowed"), selection.get("key_means"))
+            elif selection:
+                raise ValueError(f"a dense provider takes no {', '.join(selection)}")
         if isinstance(start, int):
             start = torch.full((b,), start, dtype=torch.int32, device=k.device)
         if lengths is not None:
             lengths = lengths.clamp(0, n)  # of what the write takes
         self.cache.write(k, v, table, start, lengths)
         held = start + (n if lengths is None else lengths)
-        keys, values = (torch.empty((b, context, *k.shape[2:]), dtype=k.dtype, device=k.device) for _ in range(2))
         self.cache.read(table, held, keys, values)
         if not ragged:
             return self.provider(q, keys, values, options, **selection)

@@ -179,6 +179,19 @@ class SparseProvider(B200Provider):
             raise UnsupportedAttention("b200_sparse: the selection ranks by a positive softmax_scale")
         _no_grad(q, k, v)
 
+    def check_selection(self, q, k, allowed=None, key_means=None):
+        """(key blocks, allowed broadcast to [B, Hq, query blocks, key blocks]) of a call; errors before any launch."""
+        (b, lq, h, d), (_, lk, hk, _) = q.shape, k.shape
+        nq, nk = -(-lq // self.query_block), -(-lk // self.key_block)
+        if allowed is not None:
+            allowed = _broadcast(allowed, (b, h, nq, nk))
+            if allowed.dtype != torch.bool or allowed.device != q.device:
+                raise ValueError(f"allowed must be bool on {q.device}, got {allowed.dtype} on {allowed.device}")
+        if key_means is not None and (tuple(key_means.shape) != (b, nk, hk, d) or key_means.dtype != torch.float32
+                                      or not key_means.is_contiguous() or key_means.device != q.device):
+            raise ValueError(f"key_means: expected contiguous fp32 {(b, nk, hk, d)} on {q.device}")
+        return nk, allowed
+
     def blocks_kept(self, key_blocks: int) -> int:
         """Key blocks each query block attends, of ``key_blocks``."""
         # 0.07 * 100 is a little above 7
@@ -198,18 +211,11 @@ class SparseProvider(B200Provider):
         status = _status_for(device)
         status.poll()
         q, k, v = _readable(q), _readable(k), _readable(v)
-        b, lq, h, d = q.shape
-        lk, hk = k.shape[1], k.shape[2]
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if lq == 0:
+        if q.shape[1] == 0:
             return out
-        nq, nk = -(-lq // self.query_block), -(-lk // self.key_block)
-        if allowed is not None:
-            allowed = _broadcast(allowed, (b, h, nq, nk))
-        if key_means is not None and (tuple(key_means.shape) != (b, nk, hk, d) or key_means.dtype != torch.float32
-                                      or not key_means.is_contiguous() or key_means.device != device):
-            raise ValueError(f"key_means: expected contiguous fp32 {(b, nk, hk, d)} on {device}")
-        scale = d ** -0.5 if o.softmax_scale is None else float(o.softmax_scale)
+        nk, allowed = self.check_selection(q, k, allowed, key_means)
+        scale = q.shape[-1] ** -0.5 if o.softmax_scale is None else float(o.softmax_scale)
         with _on(device):
             ops.sparse_forward(q, k, v, out, self.blocks_kept(nk), self.query_block, self.key_block, scale, status,
                                key_means, allowed, query_lengths, key_lengths)

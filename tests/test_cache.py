@@ -381,3 +381,22 @@ def test_streaming_lengths_beyond_the_rows(cuda_lib):
         attend = StreamingAttention(cache, sparse.SparseProvider(1.0, key_block=64))
         return attend(q, k, v, table, lens(100, 100).to(DEV), context=256, lengths=lens(*used).to(DEV))
     assert torch.equal(step(90, -30), step(40, 0))
+
+
+@pytest.mark.gpu
+def test_a_refused_step_writes_nothing(cuda_lib):
+    from powershard_b200 import sparse
+    from powershard_b200.cache import StreamingAttention
+    from powershard_b200.contract import AttentionOptions, UnsupportedAttention
+    from powershard_b200.provider import B200Provider
+    cache = new_cache(4, 64, 2, 128, torch.int8)
+    table = lens(0, 1)[None].to(DEV)
+    x = rows(91, 1, 40, 2, 128).to(DEV)
+    for provider in (sparse.SparseProvider(2), B200Provider()):
+        attend = StreamingAttention(cache, provider)
+        for q, options in ((x, AttentionOptions(causal=True)), (x[..., :64], None), (x.float(), None), (x.cpu(), None)):
+            with pytest.raises((UnsupportedAttention, ValueError)):
+                attend(q, x, x, table, 0, options)
+    with pytest.raises(ValueError):
+        StreamingAttention(cache, sparse.SparseProvider(2))(x, x, x, table, 0, allowed=torch.ones(7, 3, dtype=torch.bool, device=DEV))
+    assert not bits(cache.k).any() and not bits(cache.v).any()
