@@ -202,19 +202,24 @@ __device__ __forceinline__ void softmax_row(const float (&s)[128], bool first, f
 }
 
 // Merges the parts of split unit u for 8 columns from c of row r of its query
-// tile t: acc = sum_p w_p o_p with w_p = 2^(lse_p - max lse); returns 1 / sum_p w_p.
+// tile t: acc = sum_p w_p o_p with w_p = 2^(m_p - max m) l_p, or 2^(lse_p - max lse) where
+// the parts hold their logarithm; returns 1 / sum_p w_p.
 __device__ __forceinline__ float merge_parts(const AttnArgs& args, int u, int t, int r, int c, float (&acc)[8]) {
   const int S = args.split;
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
   float mx = -INFINITY;
+  auto m_and_l = [&](int p) {
+    const int at = ((u * S + p) * 2 + t) * kBlockM + r;
+    return args.ws_ml ? args.ws_ml[at] : make_float2(args.ws_lse[at], 1.f);
+  };
 #pragma unroll 4
-  for (int p = 0; p < S; ++p) mx = fmaxf(mx, args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r]);
+  for (int p = 0; p < S; ++p) mx = fmaxf(mx, m_and_l(p).x);
   float wsum = 0.f;
 #pragma unroll 4
   for (int p = 0; p < S; ++p) {
-    const float lse = args.ws_lse[((u * S + p) * 2 + t) * kBlockM + r];
-    const float w = lse == -INFINITY ? 0.f : ex2_approx(lse - mx);
+    const float2 ml = m_and_l(p);
+    const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - mx) * ml.y;
     wsum += w;
     const float4* src = reinterpret_cast<const float4*>(
         args.ws_o + ((static_cast<int64_t>(u * S + p) * 2 + t) * kBlockM + r) * kHeadDim + c);

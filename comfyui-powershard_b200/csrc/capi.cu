@@ -270,7 +270,7 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
 struct SparsePlan {
   int64_t units, rem;
   int split;
-  size_t workspace_bytes() const { return split > 1 ? size_t(rem) * split * 2 * 128 * (128 + 1) * 4 : 0; }
+  size_t workspace_bytes() const { return split > 1 ? size_t(rem) * split * 2 * 128 * (128 + 2) * 4 : 0; }
 };
 
 SparsePlan sparse_plan(int64_t batch, int64_t heads, int64_t len_q, int64_t list_len, int64_t key_block, int sms) {
@@ -1211,7 +1211,7 @@ static int sparse_attn(const void* q, const int64_t q_strides[3], const void* k,
     a.split = plan.split;
     a.full_units = static_cast<int>(plan.units - plan.rem);
     a.ws_o = static_cast<float*>(workspace);
-    a.ws_lse = a.ws_o + plan.rem * plan.split * 2 * 128 * 128;
+    a.ws_ml = reinterpret_cast<float2*>(a.ws_o + plan.rem * plan.split * 2 * 128 * 128);
     a.tickets = tickets;
   }
   return launch_sparse_attention(tq, tk, tv, a, plan.units, fp16, after_select, static_cast<cudaStream_t>(stream));

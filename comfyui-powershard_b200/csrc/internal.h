@@ -44,6 +44,8 @@ struct AttnArgs {
   int split;             // 1: no split
   float* ws_o;           // [slot][2][128][128] fp32: O / l of one part, slot = (unit - full_units) * split + part
   float* ws_lse;         // [slot][2][128] fp32: m + log2(l) of one part (log2 units of the scaled scores)
+  float2* ws_ml;         // in its place m and l of one part (sparse_attn.cu): their sum would round l away where m is
+                         // large, and with it how much parts of like maxima weigh; or null
   // Block lists (sparse_attn.cu only).  Query block i of head h of batch row b attends the key
   // blocks blocks[((b * grid_heads + h) * list_rows + i) * list_len + ...]; one segment of queries and keys.
   const int* blocks;

@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        if (w.slot >= 0 && lane < rows) args.ws_lse[at] = live && total > 0.f ? top + __log2f(total) : -INFINITY;
+        if (w.slot >= 0 && lane < rows) args.ws_ml[at] = live ? make_float2(top, total) : make_float2(-1e30f, 0.f);
         __syncwarp();
         if (lane == 0 && tiles > 0) mbar_arrive(bar(kOtherRead));
         if (w.slot >= 0 && args.tickets) {
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = w.tiles > 0 && row0 + row < w.rows;
       const float inv_l = l > 0.f ? 1.f / l : 0.f;
       if (w.slot >= 0) {
-        // One part of a list: O / l in fp32 and m + log2(l), merged by
+        // One part of a list: O / l in fp32, m and l, merged by
         // attn_combine_kernel, which reads the rows of the tensor only.
         const int64_t at = (static_cast<int64_t>(w.slot) * 2 + t) * kBlockM + row;
         float4* dst = reinterpret_cast<float4*>(args.ws_o + at * kHeadDim);
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (row < rows) args.ws_lse[at] = live && l > 0.f ? m + __log2f(l) : -INFINITY;
+          if (row < rows) args.ws_ml[at] = live ? make_float2(m, l) : make_float2(-1e30f, 0.f);
         }
       } else {
         // Each warp stages 64 columns of its 32 rows (row r, 16-byte chunk k at

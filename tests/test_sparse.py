@@ -565,6 +565,22 @@ def test_values_of_keys_far_away(cuda_lib, lq):
     assert_attention(got, near, mag)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,q_size,k_size", [(torch.float16, 2048.0, 3968.0), (torch.bfloat16, 8192.0, 7936.0),
+                                                 (torch.float16, 2048.0, -3968.0), (torch.bfloat16, 8192.0, -7936.0)])
+@pytest.mark.parametrize("b,lq,heads", [(1, 3, 2), (1, 300, 2), (2, 3, 90), (1, 300, 100)])
+def test_scores_at_the_end_of_the_range(cuda_lib, b, lq, heads, dtype, q_size, k_size):
+    """Scaled scores just below 2^27 (fp16) and 2^30 (bf16), all alike but for one key far behind (all products
+    and sums are exact): every other key counts as much, in whichever part of a list it is."""
+    from powershard_b200 import sparse
+    q, k = (torch.full((b, n, h, 128), x, dtype=dtype) for n, h, x in ((lq, heads, q_size), (2000, 2, k_size)))
+    k[:, 300] *= 0.75 if k_size > 0 else 1.25
+    v = rows(67, b, 2000, 2, 128, dtype=dtype)
+    blocks = random_lists(68, b, heads, -(-lq // 256), 31, 23)
+    got = sparse.sparse_attention(*cuda(q, k, v, blocks), key_block=64)
+    assert_attention(got, *ref_attention(q, k, v, blocks, key_block=64))
+
+
 # ------------------------------------------------------------------ the provider
 def ref_provider(q, k, v, keep, query_block=256, key_block=128, allowed=None, q_len=None, k_len=None, scale=None):
     used = lambda n, block: None if n is None else [-(-int(x) // block) for x in n]  # noqa: E731
