@@ -195,6 +195,42 @@ def test_entries_validate_on_the_host():
     assert lib.ps_b200_kernel_launches() == 0
 
 
+def test_exponentials_of_the_other_pipe():
+    """The pair of exponentials that the wide form computes without the special-function unit, step by step in 32
+    bits with the constants of its source: relative error within 7.5e-5 (and the last product's 2^-24), 0 below
+    -126.5, NaN kept."""
+    import re
+    import numpy as np
+    from pathlib import Path
+    import powershard_b200
+    source = (Path(powershard_b200.__file__).parent / "csrc" / "ptx.cuh").read_text()
+    body = source[source.index("void ex2_pair"):]
+    body = body[:body.index("\n}")]
+    floor = np.frombuffer(bytes.fromhex(re.search(r"0f([0-9A-F]{8})", body).group(1)), ">f4").astype(np.float32)[0]
+    shift, back, *poly = [np.float32(x) for x in re.findall(r'"f"\((-?[0-9.]+)f\)', body)]
+    assert back == -shift and len(poly) == 4
+
+    def fma(a, b, c):  # one rounding: the product of two 32-bit numbers is exact in 64, the sum's rounding there is 2^-29 of a step
+        return (a.astype(np.float64) * b + np.float64(c)).astype(np.float32)
+
+    def pair(x):
+        x = np.where(np.isnan(x), x, np.maximum(x, floor))
+        t = x + shift
+        f = x - (t + back)
+        p = np.full_like(f, poly[0])
+        for c in poly[1:]:
+            p = fma(p, f, c)
+        return p * (t.view(np.uint32) << np.uint32(23)).view(np.float32)
+
+    x = np.concatenate([np.linspace(-126.0, 8.0, 2_000_001), np.arange(-126, 9) + 0.5, np.arange(-125, 9)]).astype(np.float32)
+    got, want = pair(x).astype(np.float64), np.exp2(x.astype(np.float64))
+    normal = want >= 2.0 ** -125  # below, the result may be subnormal
+    assert (np.abs(got / want - 1)[normal] <= 7.5e-5 + 2.0 ** -24).all()
+    assert (np.abs(got - want)[~normal] <= 7.5e-5 * want[~normal] + 2.0 ** -149).all()
+    assert not pair(np.array([-np.inf, -1e30, -200.0, -127.0, -126.6], dtype=np.float32)).any()
+    assert np.isnan(pair(np.array([np.nan], dtype=np.float32)))[0]
+
+
 # ------------------------------------------------------------------ means
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,heads,block", [(1, 1, 64), (300, 3, 64), (1000, 4, 256), (517, 5, 128), (130, 2, 7)])
