@@ -267,6 +267,8 @@ int attention_common(const SegTensor& q, const SegTensor& k, const SegTensor& v,
 // the merge 2.5 and 0.2 a part) are bound by the keys they read once every SM
 // has a part: 40 units of 60 tiles 35.6 in three, 42.8 in seven.  Over 1 to 1500
 // rows, 2 to 40 heads and 3 to 48 tiles the choice is within 8 % of the best.
+// That is for full lists: lengths and counts are on the device and not looked at,
+// so in a padded batch the units cut may be ones that hold nothing.
 struct SparsePlan {
   int64_t units, rem;
   int split;

@@ -16,8 +16,9 @@ a plan (the selected blocks) or the key means between calls:
 Query blocks are multiples of 256 rows (the two query tiles of a CTA share
 their keys), key blocks multiples of 64.  Lengths are int32 device tensors
 [B]: rows behind them are not used whatever they hold, and are zeros in the
-output, as is a query that has no key.  Nothing here synchronises, so every
-call can be captured into a CUDA graph.
+output, as is a query that has no key.  Scores are 32-bit numbers: scaled, times
+log2 e, they may reach 2^27 in magnitude (2^30 in bf16), as in the dense kernel.
+Nothing here synchronises, so every call can be captured into a CUDA graph.
 """
 from __future__ import annotations
 

@@ -466,8 +466,9 @@ size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv
  *   strides (batch, row, head; multiples of 8 elements).  A list entry outside
  *   the key blocks names no key; one that occurs twice counts twice.  q_len /
  *   k_len as above: keys behind k_len are not used whatever they hold, output
- *   rows behind q_len and rows without a key are zeros.  workspace: device
- *   scratch of ps_b200_sparse_attn_workspace_bytes(...) bytes (0: none), owned
+ *   rows behind q_len and rows without a key are zeros.  Scores are 32-bit
+ *   numbers: scaled, times log2 e, they may reach 2^27 in magnitude (2^30 in
+ *   bf16).  workspace: device scratch of ps_b200_sparse_attn_workspace_bytes(...) bytes (0: none), owned
  *   by one call at a time.  status: device or pinned host int (may be NULL).
  */
 size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block);
