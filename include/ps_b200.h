@@ -468,8 +468,9 @@ size_t ps_b200_block_select_workspace_bytes(int batch, int heads_q, int heads_kv
  *   k_len as above: keys behind k_len are not used whatever they hold, output
  *   rows behind q_len and rows without a key are zeros.  Scores are 32-bit
  *   numbers: scaled, times log2 e, they may reach 2^27 in magnitude (2^30 in
- *   bf16).  workspace: device scratch of ps_b200_sparse_attn_workspace_bytes(...) bytes (0: none), owned
- *   by one call at a time.  status: device or pinned host int (may be NULL).
+ *   bf16).  workspace: device scratch of ps_b200_sparse_attn_workspace_bytes(...)
+ *   bytes (0: none), owned by one call at a time.  status: device or pinned host
+ *   int (may be NULL).
  */
 size_t ps_b200_sparse_attn_workspace_bytes(int batch, int heads_q, int len_q, int list_len, int key_block);
 int ps_b200_sparse_attn_fwd(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
